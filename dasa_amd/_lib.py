@@ -47,6 +47,16 @@ class CopySeg(C.Structure):
 COPY_MAX_SEGS = 16
 
 
+class LogitRules(C.Structure):
+    _fields_ = [
+        ("logits", vp), ("ld", i64), ("out", vp), ("ldo", i64), ("history", vp), ("ldh", i64), ("lengths", vp),
+        ("repetition", vp), ("presence", vp), ("frequency", vp), ("bias", vp), ("ldb", i64),
+        ("allowed_bits", vp), ("ldbits", i64), ("allowed_bytes", vp), ("ldbytes", i64), ("choice", vp),
+        ("repetition0", f32), ("presence0", f32), ("frequency0", f32),
+        ("B", i32), ("V", i32), ("L", i32), ("ids_bytes", i32), ("bf16", i32),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "dasa_version": (i32, []),
@@ -122,6 +132,16 @@ SIGNATURES = {
     "dasa_copy2d": (i32, [vp, i64, vp, i64, i32, i32, vp]),
     "dasa_colscale": (i32, [vp, i64, vp, vp, i64, i32, i32, vp]),
     "dasa_gather_rows": (i32, [vp, vp, i32, vp, vp, i32, vp, i32, vp]),
+    "dasa_embedding_fwd": (i32, [vp, i64, vp, i32, i64, i32, i32, f32, i32, vp, i64, vp, vp]),
+    "dasa_embedding_bwd_workspace": (i64, [i64, i32, i32]),
+    "dasa_embedding_bwd": (i32, [vp, i64, vp, i32, i64, i32, i32, f32, i32, i32, vp, i64, i32, vp, i64, vp]),
+    "dasa_w4_weight_bytes": (i64, [i32, i32]),
+    "dasa_w4_scale_count": (i64, [i32, i32, i32]),
+    "dasa_w4_quantize": (i32, [vp, i64, i32, i32, i32, i32, vp, i64, vp, i64, i32, vp]),
+    "dasa_w4_layout": (i32, [vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, vp]),
+    "dasa_gemm_w4": (i32, [vp, i64, i32, vp, vp, i32, i32, vp, i32, f32, vp, i64, i32, i32, i32, vp]),
+    "dasa_logit_rules_workspace": (i64, [i32, i32]),
+    "dasa_logit_rules": (i32, [C.POINTER(LogitRules), vp, i64, vp]),
 }
 
 _LIB = None

@@ -878,3 +878,28 @@ def mha(Q, K, V, addmask, heads, scale, p=0.0, training=False):
     if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
         return MHAFn.apply(Q, K, V, addmask, heads, scale, p, seed)
     return ops.mha(Q, K, V, addmask, heads, scale, p, seed)
+
+
+# ----------------------------------------------------------------------------- token embedding
+class EmbeddingFn(torch.autograd.Function):
+    """table[ids] * scale (nn.Embedding with a factor, model.py:1061); the table's gradient by sorted tokens."""
+
+    @staticmethod
+    def forward(ctx, ids, table, scale, padding_idx):
+        ctx.scale, ctx.pad, ctx.vocab = scale, padding_idx, table.shape[0]
+        ctx.save_for_backward(ids)
+        return ops.embedding(ids, table, scale=scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        return None, ops.embedding_bwd(dy, ids, ctx.vocab, scale=ctx.scale, padding_idx=ctx.pad), None, None
+
+
+def embedding(ids, table, scale=1.0, padding_idx=None):
+    """ops.embedding with a gradient for the table; rows of padding_idx get none (nn.Embedding's padding_idx)."""
+    if padding_idx is not None and not 0 <= padding_idx < table.shape[0]:
+        raise ops._lib.DasaError(f"embedding: padding_idx {padding_idx} is outside the table of {table.shape[0]} rows")
+    if torch.is_grad_enabled() and table.requires_grad:
+        return EmbeddingFn.apply(ids, table, scale, padding_idx)
+    return ops.embedding(ids, table, scale=scale)

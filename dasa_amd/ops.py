@@ -5,6 +5,7 @@ libdasa_hip.so on torch's current stream (so torch.cuda.graph capture records th
 CPU path: a CPU tensor is a usage error and raises.
 """
 import ctypes
+import math
 import os
 import weakref
 
@@ -868,7 +869,8 @@ def _error_word(dev):
 
 _ERR_BITS = {1: "persistent bi-LSTM forward: inter-workgroup barrier timed out (outputs poisoned with NaN)",
              2: "persistent bi-LSTM BPTT: inter-workgroup barrier timed out (gate gradients poisoned with NaN)",
-             4: "D-split attention: group barrier timed out (outputs poisoned with NaN)"}
+             4: "D-split attention: group barrier timed out (outputs poisoned with NaN)",
+             8: "embedding: a token id is not below the vocabulary size (its row is NaN)"}
 
 
 def check_device_errors():
@@ -1029,6 +1031,334 @@ def gather_rows(ta, ia, tb, ib, out):
     _call("dasa_gather_rows", "gather", _lib.lib().dasa_gather_rows, _p(ta), _p(ia), Fa, _p(tb), _p(ib), Fb, _p(out),
           R, _stream(), nbytes=8.0 * R * (Fa + Fb))
     return out
+
+
+# ------------------------------------------------------------------- token ends of a word step
+def _on_device(what, *ts):
+    """Every given tensor lives on the current device (the launch stream is the current device's): else a
+    DasaError, for host tensors as everywhere and for tensors of another GPU."""
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.DasaError(f"{what}: needs device tensors (the HIP path has no CPU fallback)")
+        if t.device.index != cur:
+            raise _lib.DasaError(f"{what}: a tensor is on {t.device}, the current device is cuda:{cur}")
+
+
+def _float_type(t, what):
+    """0 for float32, 1 for bfloat16 (the bf16 argument of the entry points); anything else raises."""
+    if t.dtype == torch.float32:
+        return 0
+    if t.dtype == torch.bfloat16:
+        return 1
+    raise _lib.DasaError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+
+
+def _ids_bytes(ids, what):
+    if ids.dtype == torch.int64:
+        return 8
+    if ids.dtype == torch.int32:
+        return 4
+    raise _lib.DasaError(f"{what}: expected int64 or int32 ids, got {ids.dtype}")
+
+
+def _row_view(t, what):
+    """[..., N] as (2-D tensor of unit inner stride, rows, row stride >= N): a copy where the layout needs one."""
+    N = t.shape[-1]
+    t = t.reshape(-1, N)
+    if N and t.shape[0] and ((N > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < N)):
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else N
+
+
+def _out_rows(out, shape, like, what):
+    """Check a caller's output tensor: shape, type, device, rows of one stride. Returns the row stride."""
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype:
+        raise _lib.DasaError(f"{what}: out must be {tuple(shape)} {like.dtype}, got {tuple(out.shape)} {out.dtype}")
+    if out.numel() == 0:
+        return shape[-1]
+    rows, ld = _rows(out)
+    if rows > 1 and ld < shape[-1]:
+        raise _lib.DasaError(f"{what}: the rows of out overlap")
+    return max(ld, shape[-1])
+
+
+def embedding(ids, table, scale=1.0, out=None):
+    """table[ids] * scale (dasa_embedding_fwd). ids int64 / int32 of any shape; table [V, E] fp32 or bf16, rows may
+    be strided; returns [*ids.shape, E] of the table's type, each value rounded once. A negative id gives a zero
+    row; an id >= V gives a NaN row and is reported by check_device_errors()."""
+    if table.dim() != 2:
+        raise _lib.DasaError(f"embedding: table must be [V, E], got {tuple(table.shape)}")
+    bf16, nb = _float_type(table, "embedding.table"), _ids_bytes(ids, "embedding.ids")
+    _on_device("embedding", ids, table, out)
+    V, E = table.shape
+    if E > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < E:
+        raise _lib.DasaError("embedding: the table's rows must be contiguous")
+    ids = ids.contiguous()
+    if out is None:
+        out = torch.empty(*ids.shape, E, dtype=table.dtype, device=table.device)
+        ldo = E
+    else:
+        ldo = _out_rows(out, (*ids.shape, E), table, "embedding")
+    T = ids.numel()
+    if T == 0 or E == 0:
+        return out
+    if V == 0:
+        raise _lib.DasaError("embedding: the table has no rows")
+    err = _ERR.get(table.device.index)
+    if err is None and not torch.cuda.is_current_stream_capturing():
+        err = _error_word(table.device)
+    _call("dasa_embedding_fwd", "embed", _lib.lib().dasa_embedding_fwd, table.data_ptr(), max(table.stride(0), E),
+          ids.data_ptr(), nb, T, V, E, float(scale), bf16, out.data_ptr(), ldo,
+          None if err is None else err.data_ptr(), _stream(), nbytes=T * (nb + 2.0 * E * table.element_size()))
+    return out
+
+
+def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accumulate=False):
+    """The table's gradient of embedding(): [vocab, E] with row v = scale * sum of dout over the places of id v
+    (dasa_embedding_bwd: sorted tokens, fp32 sums in position order, bitwise reproducible), in dout's type. Rows of
+    padding_idx and of ids that do not occur are zero; ids outside the vocabulary are skipped. With out and
+    accumulate=True the sums are added into out (rows without tokens are not touched)."""
+    bf16, nb = _float_type(dout, "embedding_bwd.dout"), _ids_bytes(ids, "embedding_bwd.ids")
+    _on_device("embedding_bwd", dout, ids, out)
+    vocab = int(vocab)
+    if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise _lib.DasaError(f"embedding_bwd: dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)}")
+    if vocab < 0 or vocab >= 2**31 or ids.numel() >= 2**31 - 65536:
+        raise _lib.DasaError("embedding_bwd: the vocabulary and the tokens must be fewer than 2^31")
+    if padding_idx is None:
+        padding_idx = -1
+    elif not 0 <= padding_idx < vocab:
+        raise _lib.DasaError(f"embedding_bwd: padding_idx {padding_idx} is outside the vocabulary of {vocab}")
+    if accumulate and out is None:
+        raise _lib.DasaError("embedding_bwd: accumulate=True needs out")
+    E = dout.shape[-1]
+    if out is None:
+        out = torch.empty(vocab, E, dtype=dout.dtype, device=dout.device)
+        ldo = E
+    else:
+        ldo = _out_rows(out, (vocab, E), dout, "embedding_bwd")
+    if vocab == 0 or E == 0:
+        return out
+    d, T, ldd = _row_view(dout, "embedding_bwd")
+    ids = ids.contiguous()
+    L = _lib.lib()
+    ws = torch.empty(L.dasa_embedding_bwd_workspace(T, vocab, E), dtype=torch.uint8, device=dout.device)
+    _call("dasa_embedding_bwd", "embed_bwd", L.dasa_embedding_bwd, d.data_ptr(), ldd, ids.data_ptr(), nb, T, vocab, E,
+          float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
+          _stream(), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
+    return out
+
+
+class W4Weight:
+    """A weight [N, K] in 4 bits with one scale for each `group` values of a row, laid out for linear_w4: the value
+    is (code - 8) * scale, code in 0..15. Made once by quantize_w4 or pack_w4 and kept by the program (its tensors
+    are freed with it); the weight it was made from is not referenced."""
+
+    __slots__ = ("tiles", "scales", "shape", "group")
+
+    def __init__(self, tiles, scales, shape, group):
+        self.tiles, self.scales, self.shape, self.group = tiles, scales, tuple(shape), group
+
+    @property
+    def device(self):
+        return self.tiles.device
+
+    def nbytes(self):
+        return self.tiles.numel() * 4 + self.scales.numel() * self.scales.element_size()
+
+    def dequantize(self):
+        """The fp32 weight [N, K] that linear_w4 multiplies with."""
+        N, K = self.shape
+        n16, kb = -(-N // 16), -(-K // 128)
+        w = self.tiles.view(n16, kb, 4, 16, 4)                         # [.., k quarter, column, 32-deep step]
+        q = torch.stack([(w >> (4 * i)) & 15 for i in range(8)], -1)   # two's complement nibbles
+        q = torch.where(q > 7, q - 16, q)
+        q = q.permute(0, 3, 1, 4, 2, 5).reshape(n16 * 16, kb * 128)    # k = 128 block + 32 step + 8 quarter + nibble
+        s = self.scales.view(n16, kb * (128 // self.group), 16).transpose(1, 2).reshape(n16 * 16, -1).float()
+        return (q * s.repeat_interleave(self.group, 1))[:N, :K].contiguous()
+
+
+_W4_GROUPS = (32, 64, 128)
+
+
+def _w4_group(group, what):
+    if group not in _W4_GROUPS:
+        raise _lib.DasaError(f"{what}: the group must be one of {_W4_GROUPS}, got {group}")
+    return int(group)
+
+
+def pack_w4(codes, scales, K, group):
+    """A W4Weight from codes [N, ceil(K / 2)] uint8 (two a byte, the even k in the low half; the weight is
+    (code - 8) * scale) and scales [N, ceil(K / group)] fp32 or bf16 (dasa_w4_layout)."""
+    group, K = _w4_group(group, "pack_w4"), int(K)
+    sbf = _float_type(scales, "pack_w4.scales")
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2 or K < 1 or codes.shape[0] < 1 or \
+            codes.shape[1] != (K + 1) // 2 or tuple(scales.shape) != (codes.shape[0], -(-K // group)):
+        raise _lib.DasaError(f"pack_w4: codes {codes.dtype} {tuple(codes.shape)} and scales {tuple(scales.shape)} do not "
+                             f"describe [N, {K}] in groups of {group}")
+    _on_device("pack_w4", codes, scales)
+    codes, scales = codes.contiguous(), scales.contiguous()
+    N, L = codes.shape[0], _lib.lib()
+    tiles = torch.empty(L.dasa_w4_weight_bytes(N, K) // 4, dtype=torch.int32, device=codes.device)
+    st = torch.empty(L.dasa_w4_scale_count(N, K, group), dtype=scales.dtype, device=codes.device)
+    _call("dasa_w4_layout", "elementwise", L.dasa_w4_layout, codes.data_ptr(), codes.shape[1], scales.data_ptr(),
+          scales.shape[1], sbf, N, K, group, tiles.data_ptr(), st.data_ptr(), _stream(), nbytes=1.0 * N * K)
+    return W4Weight(tiles, st, (N, K), group)
+
+
+def quantize_w4(W, group=64, scale_dtype=torch.float32):
+    """A W4Weight from W [N, K] (fp32 or bf16): scale = max |w| / 7 over each group, code = round(w / scale) + 8
+    (dasa_w4_quantize). Reads W's values back to refuse infinities and NaN, so not while a graph is captured."""
+    group, wbf = _w4_group(group, "quantize_w4"), _float_type(W, "quantize_w4.W")
+    if W.dim() != 2 or 0 in W.shape:
+        raise _lib.DasaError(f"quantize_w4: W must be [N, K], got {tuple(W.shape)}")
+    if scale_dtype not in (torch.float32, torch.bfloat16):
+        raise _lib.DasaError(f"quantize_w4: scales are float32 or bfloat16, not {scale_dtype}")
+    _on_device("quantize_w4", W)
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.DasaError("quantize_w4: quantise before the capture")
+    W = W.detach().contiguous()
+    if not bool(torch.isfinite(W).all()):
+        raise _lib.DasaError("quantize_w4: W holds infinities or NaN")
+    N, K = W.shape
+    codes = torch.empty(N, (K + 1) // 2, dtype=torch.uint8, device=W.device)
+    scales = torch.empty(N, -(-K // group), dtype=scale_dtype, device=W.device)
+    _call("dasa_w4_quantize", "elementwise", _lib.lib().dasa_w4_quantize, W.data_ptr(), K, wbf, N, K, group,
+          codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1],
+          1 if scale_dtype == torch.bfloat16 else 0, _stream(), nbytes=1.0 * W.numel() * W.element_size())
+    return pack_w4(codes, scales, K, group)
+
+
+def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
+    """y = act(x @ W^T + b) (+ beta * out) with a W4Weight (dasa_gemm_w4); forward only. x [..., K] fp32 or bf16
+    (row-strided ok), b [N] fp32, y of x's type. Accumulates in fp32 at fp32 accuracy. Made for the few rows of a
+    decoding step: the weights are read once for every 64 rows."""
+    if not isinstance(w, W4Weight):
+        raise _lib.DasaError("linear_w4: the weight must be a W4Weight (quantize_w4 / pack_w4)")
+    N, K = w.shape
+    bf16 = _float_type(x, "linear_w4.x")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise _lib.DasaError(f"linear_w4: x {tuple(x.shape)} does not end in K = {K}")
+    if b is not None and (b.dtype != torch.float32 or tuple(b.shape) != (N,) or (N > 1 and b.stride(0) != 1)):
+        raise _lib.DasaError(f"linear_w4: the bias must be a contiguous float32 [{N}]")
+    if act not in _ACT_IDS:
+        raise _lib.DasaError(f"linear_w4: unknown activation {act!r}")
+    _on_device("linear_w4", x, w.tiles, b, out)
+    if torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad)):
+        raise _lib.DasaError("linear_w4 is forward only: call it under torch.no_grad()")
+    shape = (*x.shape[:-1], N)
+    if out is None:
+        if beta != 0.0:
+            raise _lib.DasaError("linear_w4: beta needs out")
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        ldo = N
+    else:
+        ldo = _out_rows(out, shape, x, "linear_w4")
+    x2, M, ldx = _row_view(x, "linear_w4")
+    if M == 0:
+        return out
+    _call("dasa_gemm_w4", "gemm_w4", _lib.lib().dasa_gemm_w4, x2.data_ptr(), ldx, bf16, w.tiles.data_ptr(),
+          w.scales.data_ptr(), 1 if w.scales.dtype == torch.bfloat16 else 0, w.group,
+          None if b is None else b.data_ptr(), _ACT_IDS[act], float(beta), out.data_ptr(), ldo, M, N, K, _stream(),
+          flops=2.0 * M * N * K, nbytes=w.nbytes() + (1.0 * M * K + M * N) * x.element_size())
+    return out
+
+
+def _penalty(v, B, what, neutral):
+    """(device pointer or None, number) of a penalty given as None, a number or a float32 [B] tensor."""
+    if v is None:
+        return None, neutral
+    if isinstance(v, torch.Tensor):
+        if v.dtype != torch.float32 or tuple(v.shape) != (B,) or (B > 1 and v.stride(0) != 1):
+            raise _lib.DasaError(f"logit_rules: {what} must be a number or a contiguous float32 [{B}]")
+        _on_device("logit_rules", v)
+        return v.data_ptr(), neutral
+    v = float(v)
+    if not math.isfinite(v) or (what == "repetition" and v <= 0.0):
+        raise _lib.DasaError(f"logit_rules: {what} = {v}")
+    return None, v
+
+
+def logit_rules(logits, history=None, lengths=None, repetition=None, presence=None, frequency=None, bias=None,
+                allowed=None, out=None, want_choice=False):
+    """The logits of a decoding step under its rules (dasa_logit_rules), in this order: for a token v that occurs
+    c > 0 times in history[b, :lengths[b]], x > 0 ? x / repetition : x * repetition, then - frequency * c, then
+    - presence; + bias; -inf where not allowed. Returns the new logits (of the logits' type, rounded once), with
+    want_choice=True also the greedy choice [B] int64: the lowest index of the largest value.
+
+    logits [B, V] fp32 or bf16 (row-strided ok); history [B, L] int64 / int32, ids outside the vocabulary (a pad
+    such as -1) are ignored; lengths [B] int32 / int64 or None for all L; repetition (> 0), presence and frequency a
+    number or float32 [B]; bias float32 [V] or [B, V]; allowed bool / uint8 [V] or [B, V], or int32 bit words
+    [ceil(V / 32)] or [B, ceil(V / 32)] (bit v % 32 of word v // 32). out may be logits itself."""
+    if logits.dim() != 2:
+        raise _lib.DasaError(f"logit_rules: logits must be [B, V], got {tuple(logits.shape)}")
+    bf16 = _float_type(logits, "logit_rules.logits")
+    B, V = logits.shape
+    _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
+    if V == 0 or B > 65535:
+        raise _lib.DasaError(f"logit_rules: logits {tuple(logits.shape)}: 1 token at least, 65535 rows at most")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise _lib.DasaError("logit_rules is forward only: call it under torch.no_grad()")
+    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+        raise _lib.DasaError("logit_rules: the rows of logits must be contiguous")
+    d = _lib.LogitRules()
+    d.B, d.V, d.bf16 = B, V, bf16
+    if history is not None:
+        if history.dim() != 2 or history.shape[0] != B:
+            raise _lib.DasaError(f"logit_rules: history must be [{B}, L], got {tuple(history.shape)}")
+        d.ids_bytes = _ids_bytes(history, "logit_rules.history")
+        d.L = history.shape[1]
+        if d.L and B:
+            history, _, d.ldh = _row_view(history, "logit_rules")
+            d.history = history.data_ptr()
+    if lengths is not None:
+        if history is None or tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+            raise _lib.DasaError(f"logit_rules: lengths must be int32 [{B}] and go with a history")
+        lengths = lengths.to(torch.int32).contiguous()
+        d.lengths = lengths.data_ptr()
+    d.repetition, d.repetition0 = _penalty(repetition, B, "repetition", 1.0)
+    d.presence, d.presence0 = _penalty(presence, B, "presence", 0.0)
+    d.frequency, d.frequency0 = _penalty(frequency, B, "frequency", 0.0)
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((V,), (B, V)):
+            raise _lib.DasaError(f"logit_rules: bias must be float32 [{V}] or [{B}, {V}]")
+        bias = bias.contiguous()
+        d.bias, d.ldb = bias.data_ptr(), V if bias.dim() == 2 else 0
+    if allowed is not None:
+        words = allowed.dtype == torch.int32
+        n = -(-V // 32) if words else V
+        if not (words or allowed.dtype in (torch.bool, torch.uint8)) or tuple(allowed.shape) not in ((n,), (B, n)):
+            raise _lib.DasaError(f"logit_rules: allowed must be bool / uint8 [{V}] or [{B}, {V}], or int32 words "
+                                 f"[{-(-V // 32)}] or [{B}, {-(-V // 32)}]")
+        allowed = allowed.contiguous()
+        ld = n if allowed.dim() == 2 else 0
+        if words:
+            d.allowed_bits, d.ldbits = allowed.data_ptr(), ld
+        else:
+            d.allowed_bytes, d.ldbytes = allowed.data_ptr(), ld
+    if out is None:
+        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+        d.ldo = V
+    else:
+        d.ldo = _out_rows(out, (B, V), logits, "logit_rules")
+    choice = torch.empty(B, dtype=torch.int64, device=logits.device) if want_choice else None
+    if B:
+        d.logits, d.ld = logits.data_ptr(), max(logits.stride(0), V)
+        d.out = out.data_ptr()
+        L = _lib.lib()
+        ws, nws = None, 0
+        if want_choice:
+            d.choice = choice.data_ptr()
+            nws = L.dasa_logit_rules_workspace(B, V)
+            if nws:
+                ws = torch.empty(nws // 8, dtype=torch.int64, device=logits.device)
+        _call("dasa_logit_rules", "logit_rules", L.dasa_logit_rules, ctypes.byref(d),
+              None if ws is None else ws.data_ptr(), nws, _stream(),
+              nbytes=2.0 * B * V * logits.element_size() + 8.0 * B * d.L)
+    return (out, choice) if want_choice else out
 
 
 # DASA_CHECK_FINITE=1|strict: every tensor-producing entry point above checks its outputs (dasa_amd/debug.py)

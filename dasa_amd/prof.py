@@ -33,9 +33,12 @@ FAMILIES = {
     "mha_bwd": ("mfma", "mha_bwd_kernel / mha_bwd_lds_kernel"),
     "layernorm": ("hbm", "ln_fwd_kernel"),
     "layernorm_bwd": ("hbm", "ln_bwd_kernel"),
-    "embed": ("hbm", "embed_kernel"),
+    "embed": ("hbm", "embed_kernel / embedding_fwd_kernel"),
     "ada_gate": ("hbm", "ada_gate_*_kernel"),
     "gather": ("hbm", "gather_rows_kernel"),
+    "embed_bwd": ("hbm", "token_sort_kernel + embedding_bwd_*_kernel"),
+    "gemm_w4": ("hbm", "w4_kernel"),
+    "logit_rules": ("hbm", "logit_rules_kernel (+ logit_choice_kernel)"),
     "elementwise": ("hbm", "various"),
     "lstm_cell": ("hbm", "lstm_cell_*_kernel"),
 }

@@ -362,6 +362,66 @@ int dasa_copy_segments(const dasa_copy_seg* segs, int32_t n, void* stream);
 int dasa_gather_rows(const float* ta, const int32_t* ia, int32_t Fa, const float* tb, const int32_t* ib,
                      int32_t Fb, float* out, int32_t R, void* stream);
 
+/* ---- token embedding (model.py:1061 SpeakerDecoder.embedding, vilmodel.py:161-176 word embeddings) ----------
+ * out[i] = scale * table[ids[i]] for T contiguous ids (ids_bytes 4 or 8: int32 / int64), rows of E elements, fp32
+ * (bf16 = 0) or bf16 (bf16 = 1; the product is rounded once, RNE). A negative id gives a zero row; an id >= V gives
+ * a NaN row and ORs 8 into *err (may be NULL); no memory outside the table is read. ldt / ldo are row strides. */
+int dasa_embedding_fwd(const void* table, int64_t ldt, const void* ids, int32_t ids_bytes, int64_t T, int32_t V,
+                       int32_t E, float scale, int32_t bf16, void* out, int64_t ldo, uint32_t* err, void* stream);
+/* Its gradient: dtable[v] (+= if accumulate) scale * sum over i with ids[i] == v of dout[i], summed in fp32 in an
+ * order fixed by the positions (bitwise reproducible, no float atomics), rounded once to the type of dout / dtable. Rows
+ * no id names are written as zeros, or left alone if accumulate. padding_idx (or -1): an id whose rows are not
+ * summed. Ids outside [0, V) are skipped. T < 2^31 - 65536. ws: dasa_embedding_bwd_workspace(T, V, E) bytes of
+ * scratch, 16-B aligned; nothing in it outlives the call. */
+int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E);
+int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t ids_bytes, int64_t T, int32_t V,
+                       int32_t E, float scale, int32_t padding_idx, int32_t bf16, void* dtable, int64_t ldt,
+                       int32_t accumulate, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- 4-bit weights with group scales (the nn.Linear of a word step, model.py:1066-1078) -----------------------
+ * A weight is (q - 8) * s with q in 0..15 and one scale s for each run of `group` (32, 64 or 128) values of a row.
+ * dasa_w4_quantize: W [N][ldw] (fp32 / bf16) -> codes [N][ldc] (two a byte, the even k in the low half) and scales
+ * [N][lds] (fp32 / bf16), s = max |w| / 7 rounded to its type, q = clamp(rne(w / s), -8, 7) + 8; W must be finite.
+ * dasa_w4_layout: codes / scales -> the tiles that dasa_gemm_w4 reads: `weight` (dasa_w4_weight_bytes, 16-B
+ * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. */
+int64_t dasa_w4_weight_bytes(int32_t N, int32_t K);
+int64_t dasa_w4_scale_count(int32_t N, int32_t K, int32_t group);
+int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int32_t K, int32_t group, uint8_t* codes,
+                     int64_t ldc, void* scales, int64_t lds, int32_t scale_bf16, void* stream);
+int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16, int32_t N,
+                   int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream);
+/* y = act(x W^T + bias) + beta * y: x [M][ldx], y [M][ldy], both fp32 (bf16 = 0) or both bf16; fp32 accumulation at
+ * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. Any M, N, K; made for few rows. */
+int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, const void* scale_tiles,
+                 int32_t scale_bf16, int32_t group, const float* bias, int32_t act, float beta, void* y, int64_t ldy,
+                 int32_t M, int32_t N, int32_t K, void* stream);
+
+/* ---- rules on the logits of a decoding step (speaker.py:319-323) --------------------------------------------
+ * For row b and token v: c = occurrences of v in history[b][0 .. lengths[b]) (ids outside [0, V) are ignored);
+ * x = logits[b][v]; if c > 0: x = (x > 0 ? x / repetition : x * repetition) - frequency * c - presence; x += bias;
+ * -inf where not allowed; out = x rounded once to the type of logits (fp32, or bf16 with bf16 = 1; out may be
+ * logits). Each operation is one rounded fp32 operation in this order. choice[b] (or NULL) = the lowest index of
+ * the row's largest out, NaN counting as largest (a row with nothing allowed chooses 0).
+ * history [B][ldh] int32 / int64 (ids_bytes) or NULL; lengths [B] or NULL (all L); repetition / presence /
+ * frequency [B] or NULL (then the numbers *0); bias [V] (ldb = 0) or [B][ldb] or NULL; allowed as bits (bit v % 32
+ * of word v / 32; ldbits = 0 shared) or as bytes (0 = not allowed; ldbytes = 0 shared) or neither.
+ * ws: dasa_logit_rules_workspace(B, V) bytes of scratch, needed if choice is asked for. B <= 65535. */
+typedef struct dasa_logit_rules_desc {
+  const void* logits; int64_t ld;
+  void* out; int64_t ldo;
+  const void* history; int64_t ldh;
+  const int32_t* lengths;
+  const float* repetition; const float* presence; const float* frequency;
+  const float* bias; int64_t ldb;
+  const uint32_t* allowed_bits; int64_t ldbits;
+  const uint8_t* allowed_bytes; int64_t ldbytes;
+  int64_t* choice;
+  float repetition0, presence0, frequency0;
+  int32_t B, V, L, ids_bytes, bf16;
+} dasa_logit_rules_desc;
+int64_t dasa_logit_rules_workspace(int32_t B, int32_t V);
+int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---- small helpers --------------------------------------------------------------------------- */
 /* Reverse the first lengths[b] rows of x [B][L][H] into out (rest zero), r2rmodel.py:2326-2330. */
 int dasa_reverse_valid(const float* x, const int32_t* lengths, float* out, int32_t B, int32_t L,

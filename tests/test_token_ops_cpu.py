@@ -1,0 +1,106 @@
+"""Refusals of the token operators (dasa_amd.ops): wrong types, shapes and devices raise DasaError on the host, and the
+C entries return hipErrorInvalidValue before anything is launched. No GPU needed."""
+import ctypes
+
+import pytest
+import torch
+
+from dasa_amd import _lib, functional as DF, ops
+from dasa_amd._lib import DasaError
+
+INVALID = 1
+
+
+def _refused(match, f, *a, **k):
+    with pytest.raises(DasaError, match=match):
+        f(*a, **k)
+
+
+def test_host_tensors_are_refused():
+    ids, table = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4)
+    _refused("device tensors", ops.embedding, ids, table)
+    _refused("device tensors", DF.embedding, ids, table)
+    _refused("device tensors", ops.embedding_bwd, torch.zeros(3, 4), ids, 5)
+    _refused("device tensors", ops.quantize_w4, torch.zeros(4, 64))
+    _refused("device tensors", ops.pack_w4, torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1), 64, 64)
+    w = ops.W4Weight(torch.zeros(256, dtype=torch.int32), torch.zeros(32), (4, 64), 64)
+    _refused("device tensors", ops.linear_w4, torch.zeros(2, 64), w)
+    _refused("device tensors", ops.logit_rules, torch.zeros(2, 8))
+
+
+def test_embedding_arguments():
+    ids, table = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4)
+    _refused("float32 or bfloat16", ops.embedding, ids, table.double())
+    _refused("float32 or bfloat16", ops.embedding, ids, table.half())
+    _refused("int64 or int32", ops.embedding, ids.to(torch.int16), table)
+    _refused("int64 or int32", ops.embedding, ids.float(), table)
+    _refused(r"\[V, E\]", ops.embedding, ids, table[0])
+    d = torch.zeros(3, 4)
+    _refused("float32 or bfloat16", ops.embedding_bwd, d.double(), ids, 5)
+    _refused("padding_idx", DF.embedding, ids, table, 1.0, 5)
+    _refused("padding_idx", DF.embedding, ids, table, 1.0, -1)
+
+
+def test_w4_arguments():
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1)
+    for group in (0, 16, 48, 256):
+        _refused("group", ops.pack_w4, codes, scales, 64, group)
+        _refused("group", ops.quantize_w4, torch.zeros(4, 64), group)
+    _refused("describe", ops.pack_w4, codes, scales, 66, 64)
+    _refused("describe", ops.pack_w4, codes, scales, 64, 32)
+    _refused("describe", ops.pack_w4, codes.int(), scales, 64, 64)
+    _refused("describe", ops.pack_w4, codes, scales[:3], 64, 64)
+    _refused("float32 or bfloat16", ops.pack_w4, codes, scales.half(), 64, 64)
+    _refused(r"\[N, K\]", ops.quantize_w4, torch.zeros(4))
+    _refused(r"\[N, K\]", ops.quantize_w4, torch.zeros(0, 4))
+    _refused("scales are", ops.quantize_w4, torch.zeros(4, 64), 64, torch.float16)
+    w = ops.W4Weight(torch.zeros(256, dtype=torch.int32), torch.zeros(32), (4, 64), 64)
+    _refused("W4Weight", ops.linear_w4, torch.zeros(2, 64), torch.zeros(4, 64))
+    _refused("end in K", ops.linear_w4, torch.zeros(2, 65), w)
+    _refused("float32 or bfloat16", ops.linear_w4, torch.zeros(2, 64).double(), w)
+    _refused("bias", ops.linear_w4, torch.zeros(2, 64), w, torch.zeros(5))
+    _refused("bias", ops.linear_w4, torch.zeros(2, 64), w, torch.zeros(4, dtype=torch.bfloat16))
+    _refused("activation", ops.linear_w4, torch.zeros(2, 64), w, None, "swish")
+
+
+def test_logit_rules_arguments():
+    x = torch.zeros(2, 8)
+    _refused(r"\[B, V\]", ops.logit_rules, x[0])
+    _refused("float32 or bfloat16", ops.logit_rules, x.half())
+
+
+def test_entry_points_refuse_before_a_launch():
+    """Addresses are made up: nothing here may reach a launch."""
+    L = _lib.lib()
+    P = 0x100000
+    assert L.dasa_embedding_fwd(P, 8, P, 8, 0, 10, 8, 1.0, 0, P, 8, None, None) == 0           # no tokens
+    for T, V, E, nb, ldt, ldo in ((-1, 10, 8, 8, 8, 8), (4, 0, 8, 8, 8, 8), (4, 10, 8, 2, 8, 8), (4, 10, 8, 8, 7, 8),
+                                  (4, 10, 8, 8, 8, 7), (4, -1, 8, 8, 8, 8)):
+        assert L.dasa_embedding_fwd(P, ldt, P, nb, T, V, E, 1.0, 0, P, ldo, None, None) == INVALID
+    assert L.dasa_embedding_fwd(None, 8, P, 8, 4, 10, 8, 1.0, 0, P, 8, None, None) == INVALID
+    need = L.dasa_embedding_bwd_workspace(100, 50, 8)
+    assert need >= 4 * 151 and L.dasa_embedding_bwd_workspace(2**31, 50, 8) == 0
+    for T, nb, ldd, ldt, ws, n in ((2**31, 8, 8, 8, P, need), (100, 1, 8, 8, P, need), (100, 8, 7, 8, P, need),
+                                   (100, 8, 8, 7, P, need), (100, 8, 8, 8, None, need), (100, 8, 8, 8, P, need - 1),
+                                   (-1, 8, 8, 8, P, need)):
+        assert L.dasa_embedding_bwd(P, ldd, P, nb, T, 50, 8, 1.0, -1, 0, P, ldt, 0, ws, n, None) == INVALID
+    assert L.dasa_w4_weight_bytes(17, 129) == 2 * 2 * 1024 and L.dasa_w4_weight_bytes(0, 4) == 0
+    assert L.dasa_w4_scale_count(17, 129, 64) == 2 * 2 * 2 * 16 and L.dasa_w4_scale_count(17, 129, 16) == 0
+    assert L.dasa_w4_quantize(P, 64, 0, 4, 64, 16, P, 32, P, 4, 0, None) == INVALID
+    assert L.dasa_w4_quantize(P, 63, 0, 4, 64, 64, P, 32, P, 1, 0, None) == INVALID
+    assert L.dasa_w4_layout(P, 31, P, 1, 0, 4, 64, 64, P, P, None) == INVALID
+    assert L.dasa_gemm_w4(P, 64, 0, P, P, 0, 64, None, 0, 0.0, P, 4, 0, 4, 64, None) == 0        # no rows
+    for ldx, w, group, act, ldy, M in ((63, P, 64, 0, 4, 2), (64, P + 8, 64, 0, 4, 2), (64, P, 65, 0, 4, 2),
+                                       (64, P, 64, 9, 4, 2), (64, P, 64, 0, 3, 2), (64, P, 64, 0, 4, -1)):
+        assert L.dasa_gemm_w4(P, ldx, 0, w, P, 0, group, None, act, 0.0, P, ldy, M, 4, 64, None) == INVALID
+    good = dict(B=2, V=9000, L=4, ids_bytes=8, logits=P, ld=9000, out=P, ldo=9000, history=P, ldh=4, repetition0=1.0)
+    def desc(**kw):
+        d = _lib.LogitRules()
+        for k, v in {**good, **kw}.items():
+            setattr(d, k, v)
+        return ctypes.byref(d)
+    for kw in (dict(V=0), dict(B=-1), dict(B=65536), dict(ld=8999), dict(ldo=8999), dict(ids_bytes=3), dict(ldh=3),
+               dict(logits=None), dict(L=-1), dict(bias=P, ldb=8999), dict(allowed_bits=P, ldbits=281),
+               dict(allowed_bytes=P, ldbytes=8999), dict(allowed_bits=P, allowed_bytes=P), dict(choice=P)):
+        assert L.dasa_logit_rules(desc(**kw), None, 0, None) == INVALID, kw
+    assert L.dasa_logit_rules(desc(B=0), None, 0, None) == 0
