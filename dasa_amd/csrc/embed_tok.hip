@@ -18,33 +18,58 @@ namespace {
 
 constexpr unsigned kErrTokenId = 8;   // bit of the error word (ops._ERR_BITS)
 
-template <class T> struct Vec;   // 16 bytes of a row
+// 16 bytes of a row. Rows of odd width or stride start anywhere, so the vector types are element-aligned (global loads
+// and stores take any alignment); the last unit of a row may be partial.
+template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
-  typedef float type __attribute__((ext_vector_type(4)));
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
 };
 template <> struct Vec<__bf16> {
   static constexpr int N = 8;
-  typedef __bf16 type __attribute__((ext_vector_type(8)));
+  typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2)));
 };
+
+template <class T>
+__device__ __forceinline__ typename Vec<T>::type load_unit(const T* p, int left) {
+  typedef typename Vec<T>::type V;
+  if (left >= Vec<T>::N) return *reinterpret_cast<const V*>(p);
+  V v;
+#pragma unroll
+  for (int e = 0; e < Vec<T>::N; ++e) v[e] = e < left ? p[e] : (T)0.f;
+  return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store_unit(T* p, int left, typename Vec<T>::type v) {
+  typedef typename Vec<T>::type V;
+  if (left >= Vec<T>::N) {
+    *reinterpret_cast<V*>(p) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e)
+      if (e < left) p[e] = v[e];
+  }
+}
 
 // ------------------------------------------------------------------ lookup
 struct LookupArgs {
   const void* table; long ldt;
   const void* ids;
   void* out; long ldo;
-  unsigned units;        // VEC-element units per row
+  unsigned units;        // 16-B units per row, the last one partial if the width is odd
   unsigned total;        // rows * units (< 2^31)
-  int V;
+  int V, E;
   float scale;
   unsigned* err;
 };
 
-// Thread = ILP units of VEC elements, the ILP table loads in flight together; consecutive threads take consecutive
-// units, so narrow rows still fill a wave's loads.
-template <class T, class I, int VEC, int ILP>
+// Thread = ILP units, the ILP table loads in flight together; consecutive threads take consecutive units, so narrow
+// rows still fill a wave's loads.
+template <class T, class I, int ILP>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(LookupArgs a) {
-  typedef T V __attribute__((ext_vector_type(VEC)));
+  constexpr int N = Vec<T>::N;
+  typedef typename Vec<T>::type V;
   const unsigned u0 = blockIdx.x * (256u * ILP) + threadIdx.x;
   const I* ids = reinterpret_cast<const I*>(a.ids);
   unsigned row[ILP], c[ILP];
@@ -53,34 +78,34 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(LookupArgs a) {
   for (int k = 0; k < ILP; ++k) {
     const unsigned u = min(u0 + 256u * k, a.total - 1);
     row[k] = u / a.units;
-    c[k] = u - row[k] * a.units;
+    c[k] = (u - row[k] * a.units) * N;
     id[k] = (long)ids[row[k]];
   }
   V v[ILP];
 #pragma unroll
   for (int k = 0; k < ILP; ++k) {
     const long r = (id[k] >= 0 && id[k] < a.V) ? id[k] : 0;
-    v[k] = *reinterpret_cast<const V*>(reinterpret_cast<const T*>(a.table) + r * a.ldt + (long)c[k] * VEC);
+    v[k] = load_unit(reinterpret_cast<const T*>(a.table) + r * a.ldt + c[k], a.E - (int)c[k]);
   }
 #pragma unroll
   for (int k = 0; k < ILP; ++k) {
     if (u0 + 256u * k >= a.total) continue;
     V o;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
+    for (int e = 0; e < N; ++e) {
       float x = (float)v[k][e] * a.scale;
       if (id[k] < 0) x = 0.f;
       if (id[k] >= a.V) x = __builtin_nanf("");
       o[e] = (T)x;
     }
     if (id[k] >= a.V && c[k] == 0 && a.err) atomicOr(a.err, kErrTokenId);
-    *reinterpret_cast<V*>(reinterpret_cast<T*>(a.out) + (long)row[k] * a.ldo + (long)c[k] * VEC) = o;
+    store_unit(reinterpret_cast<T*>(a.out) + (long)row[k] * a.ldo + c[k], a.E - (int)c[k], o);
   }
 }
 
-template <class T, class I, int VEC>
-int launch_fwd(LookupArgs a, long rows, int E, hipStream_t st) {
-  a.units = (unsigned)(E / VEC);
+template <class T, class I>
+int launch_fwd(LookupArgs a, long rows, hipStream_t st) {
+  a.units = (unsigned)((a.E + Vec<T>::N - 1) / Vec<T>::N);
   const long per = ((1L << 31) - 4096) / a.units;    // rows of one launch: 32-bit unit indexes
   const char* ids = reinterpret_cast<const char*>(a.ids);
   char* out = reinterpret_cast<char*>(a.out);
@@ -91,9 +116,9 @@ int launch_fwd(LookupArgs a, long rows, int E, hipStream_t st) {
     a.total = (unsigned)(n * a.units);
     // four units a thread once that still gives every CU eight waves
     if (a.total >= 4u * 256u * 512u)
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, VEC, 4>), dim3((a.total + 1023) / 1024), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 4>), dim3((a.total + 1023) / 1024), dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, VEC, 1>), dim3((a.total + 255) / 256), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 1>), dim3((a.total + 255) / 256), dim3(256), 0, st, a);
     DASA_CHECK_LAUNCH();
   }
   return 0;
@@ -203,72 +228,170 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
 }
 
 // ------------------------------------------------------------------ gradient rows
+// A table row of up to kChunk tokens is summed by one wave per slice of 64 units. Longer (hot) rows are cut at the
+// multiples of kChunk in the sorted order, so that a padding or stop word with a tenth of the tokens does not run on
+// one wave: each chunk leaves the sum of its part of at most two hot rows (one that reaches into it, one that reaches
+// out of it: a hot row is longer than a chunk), and a third launch adds a row's parts in chunk order.
+constexpr int kChunk = 64;
+constexpr int kJoinWaves = 16;
+
 struct BwdArgs {
   const void* dout; long ldd;
+  const void* ids; int ids64;
   const int* start;
   const int* order;
+  float* parts;            // [chunks][2][ldp] sums of hot rows' parts, or null (no row can be hot)
+  long ldp;
   void* dtable; long ldt;
-  int V, E;
+  int V, E, slices;
+  unsigned row_blocks;     // blocks of the rows kernel that take table rows; the others take chunks
   float scale;
   int accumulate;
 };
 
-// One wave = one table row x one slice of 64 VEC columns.
-template <class T, int VEC>
+// acc += the dout rows of n <= 64 tokens whose positions the lanes hold, tokens lane0 .. lane0 + n in order. Four rows
+// are in flight at a time.
+template <class T>
+__device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
+                                         int n) {
+  constexpr int N = Vec<T>::N;
+  typedef typename Vec<T>::type V;
+  int j = 0;
+  for (; j + 4 <= n; j += 4) {
+    V x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      x[k] = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j + k) * ldd, left);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += (float)x[k][e];
+  }
+  for (; j < n; ++j) {
+    const V x = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j) * ldd, left);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += (float)x[e];
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void write_row(const BwdArgs& a, long v, int col, int left, const float (&acc)[Vec<T>::N]) {
+  constexpr int N = Vec<T>::N;
+  T* o = reinterpret_cast<T*>(a.dtable) + v * a.ldt + col;
+  typename Vec<T>::type y;
+  if (a.accumulate) y = load_unit(o, left);
+#pragma unroll
+  for (int e = 0; e < N; ++e) y[e] = (T)(a.accumulate ? (float)y[e] + acc[e] * a.scale : acc[e] * a.scale);
+  store_unit(o, left, y);
+}
+
+__device__ __forceinline__ long id_at(const BwdArgs& a, int pos) {
+  return a.ids64 ? (long)reinterpret_cast<const int64_t*>(a.ids)[pos] : (long)reinterpret_cast<const int32_t*>(a.ids)[pos];
+}
+
+// One wave = (table row, slice) or (chunk, slice).
+template <class T>
 __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
-  typedef T V __attribute__((ext_vector_type(VEC)));
-  const int lane = threadIdx.x & 63;
-  const long v = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (v >= a.V) return;
-  const int col = (blockIdx.y * 64 + lane) * VEC;
-  const int s = a.start[v], e = a.start[v + 1];
-  if (a.accumulate && s == e) return;
-  if (col >= a.E) return;
-  float acc[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  constexpr int N = Vec<T>::N;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int col = (blockIdx.y * 64 + lane) * N, left = a.E - col;
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
-  for (int j = s; j < e; ++j) {
-    const V x = *reinterpret_cast<const V*>(d + (long)a.order[j] * a.ldd);
+  float acc[N];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc[i] += (float)x[i];
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  if (blockIdx.x < a.row_blocks) {
+    const long v = (long)blockIdx.x * 4 + w;
+    if (v >= a.V) return;
+    const int s = a.start[v], n = a.start[v + 1] - s;
+    if (n > kChunk || (a.accumulate && n == 0)) return;
+    const int pos = lane < n ? a.order[s + lane] : 0;
+    if (left > 0) {
+      add_rows<T>(acc, d, a.ldd, left, pos, 0, n);
+      write_row<T>(a, v, col, left, acc);
+    }
+    return;
   }
-  V* o = reinterpret_cast<V*>(reinterpret_cast<T*>(a.dtable) + v * a.ldt + col);
-  V y;
-  if (a.accumulate) {
-    const V old = *o;
+  const long c = (long)(blockIdx.x - a.row_blocks) * 4 + w;
+  const int j0 = (int)(c * kChunk), total = a.start[a.V];
+  if (j0 >= total) return;
+  const int m = min(kChunk, total - j0);
+  const int pos = a.order[j0 + min(lane, m - 1)];
+  const long id = id_at(a, pos);
+  const int rs = a.start[id], re = a.start[id + 1];
+  const bool hot = re - rs > kChunk;
+  float* part = a.parts + c * 2 * a.ldp + col;
+  // the row that owns the chunk's first token, then the row that owns its last
+  const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
+  if (ea > 0 && left > 0) {
+    add_rows<T>(acc, d, a.ldd, left, pos, 0, ea);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) y[i] = (T)((float)old[i] + acc[i] * a.scale);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) y[i] = (T)(acc[i] * a.scale);
+    for (int e = 0; e < N; ++e) part[e] = acc[e];
   }
-  *o = y;
+  const int sb = __builtin_amdgcn_readlane(hot ? max(rs - j0, 0) : m, m - 1);
+  if (sb > 0 && sb < m && left > 0) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    add_rows<T>(acc, d, a.ldd, left, pos, sb, m - sb);
+#pragma unroll
+    for (int e = 0; e < N; ++e) part[a.ldp + e] = acc[e];
+  }
 }
 
-template <class T, int VEC>
-int launch_rows(const BwdArgs& a, hipStream_t st) {
-  const int slices = (a.E + 64 * VEC - 1) / (64 * VEC);
-  hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, VEC>), dim3((a.V + 3) / 4, slices), dim3(256), 0, st, a);
+// One workgroup = (chunk, slice): the hot row that starts in the chunk, if any, as the sum of its parts. The waves
+// take runs of parts, joined in order.
+template <class T>
+__global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(BwdArgs a) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float sum[kJoinWaves][64][N];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int col = (blockIdx.y * 64 + lane) * N, left = a.E - col;
+  const long c = blockIdx.x;
+  const int j0 = (int)(c * kChunk), total = a.start[a.V];
+  if (j0 >= total) return;
+  const int last = min(j0 + kChunk, total) - 1;
+  const long v = id_at(a, a.order[last]);                 // a hot row that starts here reaches past the chunk
+  const int rs = a.start[v], re = a.start[v + 1];
+  if (re - rs <= kChunk || rs < j0) return;
+  const int n = (re - 1) / kChunk - (int)c + 1;           // its parts: chunks c .. c + n - 1
+  const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  if (left > 0)
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+      const float* p = a.parts + ((c + k) * 2 + (k == 0 && rs > j0 ? 1 : 0)) * a.ldp + col;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += p[e];
+    }
+#pragma unroll
+  for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
+  __syncthreads();
+  if (w != 0 || left <= 0) return;
+  for (int k = 1; k < kJoinWaves; ++k)
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
+  write_row<T>(a, v, col, left, acc);
+}
+
+inline long part_stride(int E, int bf16) {      // whole units, so a partial unit's sums stay inside
+  const int n = bf16 ? 8 : 4;
+  return (long)(E + n - 1) / n * n;
+}
+
+template <class T>
+int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
+  a.slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
+  a.row_blocks = (unsigned)((a.V + 3) / 4);
+  const long chunks = a.parts ? (tokens + kChunk - 1) / kChunk : 0;
+  const dim3 grid(a.row_blocks + (unsigned)((chunks + 3) / 4), a.slices);
+  hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
+  if (chunks) {
+    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)chunks, a.slices), dim3(64 * kJoinWaves), 0, st, a);
+    DASA_CHECK_LAUNCH();
+  }
   return 0;
-}
-
-inline bool aligned16(const void* p, long ld, int elem) { return (((uintptr_t)p | (uintptr_t)(ld * elem)) & 15) == 0; }
-
-template <class T>
-int fwd_types(const LookupArgs& a, int64_t rows, int E, bool i64, hipStream_t st) {
-  constexpr int N = Vec<T>::N;
-  const bool vec = E % N == 0 && aligned16(a.table, a.ldt, sizeof(T)) && aligned16(a.out, a.ldo, sizeof(T));
-  if (vec) return i64 ? launch_fwd<T, int64_t, N>(a, rows, E, st) : launch_fwd<T, int32_t, N>(a, rows, E, st);
-  return i64 ? launch_fwd<T, int64_t, 1>(a, rows, E, st) : launch_fwd<T, int32_t, 1>(a, rows, E, st);
-}
-
-template <class T>
-int bwd_types(const BwdArgs& a, hipStream_t st) {
-  constexpr int N = Vec<T>::N;
-  const bool vec = a.E % N == 0 && aligned16(a.dout, a.ldd, sizeof(T)) && aligned16(a.dtable, a.ldt, sizeof(T));
-  return vec ? launch_rows<T, N>(a, st) : launch_rows<T, 1>(a, st);
 }
 
 inline int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
@@ -281,14 +404,16 @@ extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* id
   if (T < 0 || V < 0 || E < 0 || (ids_bytes != 4 && ids_bytes != 8)) return (int)hipErrorInvalidValue;
   if (T == 0 || E == 0) return 0;
   if (V == 0 || !table || !ids || !out || ldt < E || ldo < E) return (int)hipErrorInvalidValue;
-  LookupArgs a{table, (long)ldt, ids, out, (long)ldo, 0, 0, V, scale, err};
-  return bf16 ? fwd_types<__bf16>(a, T, E, ids_bytes == 8, (hipStream_t)stream)
-              : fwd_types<float>(a, T, E, ids_bytes == 8, (hipStream_t)stream);
+  LookupArgs a{table, (long)ldt, ids, out, (long)ldo, 0, 0, V, E, scale, err};
+  hipStream_t st = (hipStream_t)stream;
+  if (bf16) return ids_bytes == 8 ? launch_fwd<__bf16, int64_t>(a, T, st) : launch_fwd<__bf16, int32_t>(a, T, st);
+  return ids_bytes == 8 ? launch_fwd<float, int64_t>(a, T, st) : launch_fwd<float, int32_t>(a, T, st);
 }
 
 extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E) {
   if (T < 0 || T >= (1LL << 31) || V < 0 || E < 0) return 0;
-  return round16(((int64_t)V + 1) * 4) + round16(T * 4);
+  const int64_t chunks = T > kChunk ? (T + kChunk - 1) / kChunk : 0;
+  return round16(((int64_t)V + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4;
 }
 
 extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t ids_bytes, int64_t T,
@@ -313,6 +438,11 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   else
     hipLaunchKernelGGL(token_sort_kernel<int32_t>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
   DASA_CHECK_LAUNCH();
-  BwdArgs ba{dout, (long)ldd, start, order, dtable, (long)ldt, V, E, scale, accumulate};
-  return bf16 ? bwd_types<__bf16>(ba, st) : bwd_types<float>(ba, st);
+  BwdArgs ba{};
+  ba.dout = dout; ba.ldd = (long)ldd; ba.ids = ids; ba.ids64 = ids_bytes == 8;
+  ba.start = start; ba.order = order;
+  if (T > kChunk) ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
+  ba.ldp = part_stride(E, bf16);
+  ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.scale = scale; ba.accumulate = accumulate;
+  return bf16 ? launch_rows<__bf16>(ba, T, st) : launch_rows<float>(ba, T, st);
 }
