@@ -20,21 +20,21 @@
 #include "common.h"
 #include "../../include/dasa_hip.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-constexpr int kWaves = 4;
 
 struct W4Args {
   const void* x; long ldx;
   const uint4* w;           // [N16][Kb][64 lanes] 16 B
-  const void* scales;       // [N16][Kb][128 / g][16]
+  const void* scales;       // [N16][Kb][16][128 / g]
   const float* bias;
   void* y; long ldy;
   float beta;
   int act;
   int M, N, K, Kb, N16;
-  int xvec;                 // 16-B loads of x are aligned
 };
 
 __device__ __forceinline__ float act_of(float v, int act) {
@@ -52,54 +52,60 @@ union Frag {
   bf16x8 v;
 };
 
-// eight two's-complement nibbles -> eight bf16 values (q - 8) / 16, element i = nibble i
+// eight two's-complement nibbles -> eight bf16 values (q - 8) / 16, element i = nibble i: one shift, eight converts
+// (each from one byte of the word, whose low nibble counts), four merges of the high halves, which hold it all
 __device__ __forceinline__ bf16x8 unpack8(unsigned w) {
   Frag f;
   const unsigned h = w >> 4;
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const float e = __builtin_amdgcn_cvt_off_f32_i4((int)(w >> (8 * b)));
-    const float o = __builtin_amdgcn_cvt_off_f32_i4((int)(h >> (8 * b)));
-    f.u[b] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);   // high halves: exact
+    const float e = __builtin_amdgcn_cvt_off_f32_i4((int)((w >> (8 * b)) & 255u));
+    const float o = __builtin_amdgcn_cvt_off_f32_i4((int)((h >> (8 * b)) & 255u));
+    f.u[b] = __builtin_amdgcn_perm(__float_as_uint(o), __float_as_uint(e), 0x07060302u);
   }
   return f.v;
 }
 
-// x = p0 + p1 + p2 with every plane a bf16 (truncated: 8 + 8 + 8 significand bits). Inf and NaN stay in p0 alone.
-__device__ __forceinline__ void split3(float x, unsigned& p0, unsigned& p1, unsigned& p2) {
-  const unsigned u = __float_as_uint(x);
-  p0 = u & 0xffff0000u;
-  float r = x - __uint_as_float(p0);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    r = 0.f;
-    if (u & 0x007fffffu) p0 |= 0x00400000u;     // a NaN whose payload lies in the low half stays a NaN
-  }
-  p1 = __float_as_uint(r) & 0xffff0000u;
-  p2 = __float_as_uint(r - __uint_as_float(p1));
-}
-
+// Eight consecutive activations of one row, as loaded (Raw) and as PL bf16 fragments. Rows start anywhere: element-
+// aligned vectors. `left` <= 8 values exist; the rest are zeros.
 template <class T> struct XFrag;
-// eight consecutive activations of one row -> PL bf16 fragments (zeros past the row's end or for a row past M)
 template <> struct XFrag<float> {
   static constexpr int PL = 3;
-  static __device__ __forceinline__ void load(const float* p, int left, bool vec, bf16x8 (&f)[3]) {
-    float v[8];
-    if (vec && left >= 8) {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
+  typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+  struct Raw { float v[8]; };
+  static __device__ __forceinline__ Raw load(const float* p) {
+    const V a = reinterpret_cast<const V*>(p)[0], b = reinterpret_cast<const V*>(p)[1];
+    return Raw{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+  static __device__ __forceinline__ Raw load_part(const float* p, int left) {
+    Raw r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) r.v[i] = i < left ? p[i] : 0.f;
+    return r;
+  }
+  // x = p0 + p1 + p2, every plane a bf16 (truncated: 8 + 8 + 8 significand bits). A NaN stays one in every plane. An
+  // infinity would leave inf - inf behind, so a fragment that holds one takes the guarded form.
+  static __device__ __forceinline__ void planes(const Raw& r, bf16x8 (&f)[3]) {
+    float m = fmaxf(fabsf(r.v[0]), fabsf(r.v[1]));
+#pragma unroll
+    for (int i = 2; i < 8; ++i) m = fmaxf(m, fabsf(r.v[i]));
+    const bool inf = __any(m == INFINITY);
     Frag q[3];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      unsigned a0, a1, a2, b0, b1, b2;
-      split3(v[2 * i], a0, a1, a2);
-      split3(v[2 * i + 1], b0, b1, b2);
-      q[0].u[i] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
-      q[1].u[i] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
-      q[2].u[i] = __builtin_amdgcn_perm(b2, a2, 0x07060302u);
+      unsigned p0[2], p1[2], p2[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = r.v[2 * i + e];
+        p0[e] = __float_as_uint(x);
+        float d = x - __uint_as_float(p0[e] & 0xffff0000u);
+        if (inf && fabsf(x) == INFINITY) d = 0.f;
+        p1[e] = __float_as_uint(d);
+        p2[e] = __float_as_uint(d - __uint_as_float(p1[e] & 0xffff0000u));
+      }
+      q[0].u[i] = __builtin_amdgcn_perm(p0[1], p0[0], 0x07060302u);
+      q[1].u[i] = __builtin_amdgcn_perm(p1[1], p1[0], 0x07060302u);
+      q[2].u[i] = __builtin_amdgcn_perm(p2[1], p2[0], 0x07060302u);
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) f[k] = q[k].v;
@@ -107,21 +113,37 @@ template <> struct XFrag<float> {
 };
 template <> struct XFrag<__bf16> {
   static constexpr int PL = 1;
-  static __device__ __forceinline__ void load(const __bf16* p, int left, bool vec, bf16x8 (&f)[1]) {
-    if (vec && left >= 8) {
-      f[0] = *reinterpret_cast<const bf16x8*>(p);
-    } else {
+  typedef __bf16 V __attribute__((ext_vector_type(8), aligned(2)));
+  struct Raw { V v; };
+  static __device__ __forceinline__ Raw load(const __bf16* p) { return Raw{*reinterpret_cast<const V*>(p)}; }
+  static __device__ __forceinline__ Raw load_part(const __bf16* p, int left) {
+    Raw r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[0][i] = i < left ? p[i] : (__bf16)0.f;
-    }
+    for (int i = 0; i < 8; ++i) r.v[i] = i < left ? p[i] : (__bf16)0.f;
+    return r;
   }
+  static __device__ __forceinline__ void planes(const Raw& r, bf16x8 (&f)[1]) { f[0] = r.v; }
 };
 
-// MT = 16-row tiles of x, NT = 16-column blocks of a workgroup, GPB = groups of a 128-deep block
-template <class T, class S, int MT, int NT, int GPB>
-__global__ __launch_bounds__(64 * kWaves) void w4_kernel(W4Args a) {
-  constexpr int PL = XFrag<T>::PL;
-  extern __shared__ float4 part[];          // [kWaves][NT][MT][64]
+// the GPB scales of one column of one block
+template <class S, int GPB>
+__device__ __forceinline__ void load_scales(const void* scales, long at, float (&sc)[GPB]) {
+  typedef S V __attribute__((ext_vector_type(GPB)));
+  if constexpr (GPB == 1) {
+    sc[0] = (float)reinterpret_cast<const S*>(scales)[at];
+  } else {
+    const V v = reinterpret_cast<const V*>(scales)[at];
+#pragma unroll
+    for (int g = 0; g < GPB; ++g) sc[g] = (float)v[g];
+  }
+}
+
+// MT = 16-row tiles of x, NT = 16-column blocks of a workgroup, GPB = groups of a 128-deep block, W = waves
+template <class T, class S, int MT, int NT, int GPB, int W>
+__global__ __launch_bounds__(64 * W) void w4_kernel(W4Args a) {
+  typedef XFrag<T> X;
+  constexpr int PL = X::PL;
+  extern __shared__ float4 part[];          // [W][NT][MT][64]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
   const int c16 = lane & 15, kq = lane >> 4;
@@ -130,27 +152,39 @@ __global__ __launch_bounds__(64 * kWaves) void w4_kernel(W4Args a) {
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int m = 0; m < MT; ++m) y[t][m] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const T* x = reinterpret_cast<const T*>(a.x);
-  for (int kb = w; kb < a.Kb; kb += kWaves) {
+  // a row past the last repeats it: it only reaches output rows that are not stored
+  const T* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    x[m] = reinterpret_cast<const T*>(a.x) + (long)min(m0 + m * 16 + c16, a.M - 1) * a.ldx + kq * 8;
+  long blk0[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) blk0[t] = (long)min(nt0 + t, a.N16 - 1) * a.Kb;
+
+  auto block = [&](int kb, auto tail) {
+    constexpr bool TAIL = decltype(tail)::value;
     uint4 wq[NT];
     float sc[NT][GPB];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const long blk = (long)min(nt0 + t, a.N16 - 1) * a.Kb + kb;
-      wq[t] = a.w[blk * 64 + lane];
-#pragma unroll
-      for (int g = 0; g < GPB; ++g) sc[t][g] = (float)reinterpret_cast<const S*>(a.scales)[(blk * GPB + g) * 16 + c16];
+      wq[t] = a.w[(blk0[t] + kb) * 64 + lane];
+      load_scales<S, GPB>(a.scales, (blk0[t] + kb) * 16 + c16, sc[t]);
     }
     floatx4 acc[NT][MT];
+    typename X::Raw raw[4][MT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int k = kb * 128 + j * 32;
+        if constexpr (TAIL) raw[j][m] = X::load_part(x[m] + k, a.K - k - kq * 8);
+        else raw[j][m] = X::load(x[m] + k);
+      }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       bf16x8 xf[MT][PL];
-      const int k = kb * 128 + j * 32 + kq * 8;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = m0 + m * 16 + c16;
-        XFrag<T>::load(x + (long)min(row, a.M - 1) * a.ldx + k, row < a.M ? a.K - k : 0, a.xvec, xf[m]);
-      }
+      for (int m = 0; m < MT; ++m) X::planes(raw[j][m], xf[m]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const unsigned word = j == 0 ? wq[t].x : j == 1 ? wq[t].y : j == 2 ? wq[t].z : wq[t].w;
@@ -169,17 +203,21 @@ __global__ __launch_bounds__(64 * kWaves) void w4_kernel(W4Args a) {
         }
       }
     }
-  }
+  };
+  const int full = a.K / 128;
+  for (int kb = w; kb < full; kb += W) block(kb, std::false_type{});
+  if (full < a.Kb && full % W == w) block(full, std::true_type{});
+
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
       part[((w * NT + t) * MT + m) * 64 + lane] = make_float4(y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]);
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * MT * 64; i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < NT * MT * 64; i += 64 * W) {
     float4 s = part[i];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) {
+    for (int k = 1; k < W; ++k) {
       const float4 v = part[k * NT * MT * 64 + i];
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
@@ -201,22 +239,39 @@ __global__ __launch_bounds__(64 * kWaves) void w4_kernel(W4Args a) {
   }
 }
 
-template <class T, class S, int MT, int NT>
+template <class T, class S, int MT, int NT, int W>
 int launch_g(const W4Args& a, int g, hipStream_t st) {
-  const dim3 grid((a.N16 + NT - 1) / NT, (a.M + 16 * MT - 1) / (16 * MT)), block(64 * kWaves);
-  const size_t lds = (size_t)kWaves * NT * MT * 64 * 16;
-  if (g == 32) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 4>), grid, block, lds, st, a);
-  else if (g == 64) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 2>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 1>), grid, block, lds, st, a);
+  const dim3 grid((a.N16 + NT - 1) / NT, (a.M + 16 * MT - 1) / (16 * MT)), block(64 * W);
+  const size_t lds = (size_t)W * NT * MT * 64 * 16;
+  if (g == 32) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 4, W>), grid, block, lds, st, a);
+  else if (g == 64) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 2, W>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 1, W>), grid, block, lds, st, a);
   DASA_CHECK_LAUNCH();
   return 0;
 }
 
+#ifdef W4_TUNE
+int g_nt = 1, g_w = 4;
+template <class T, class S, int MT, int NT>
+int launch_w(const W4Args& a, int g, hipStream_t st) {
+  if (g_w == 4) return launch_g<T, S, MT, NT, 4>(a, g, st);
+  if (g_w == 8) return launch_g<T, S, MT, NT, 8>(a, g, st);
+  if constexpr (NT * MT <= 4) return launch_g<T, S, MT, NT, 16>(a, g, st);
+  return 1;
+}
+template <class T, class S, int MT>
+int launch_n(const W4Args& a, int g, hipStream_t st) {
+  if (g_nt == 1) return launch_w<T, S, MT, 1>(a, g, st);
+  if (g_nt == 2) return launch_w<T, S, MT, 2>(a, g, st);
+  return launch_w<T, S, MT, 4>(a, g, st);
+}
+#else
 template <class T, class S, int MT>
 int launch_n(const W4Args& a, int g, hipStream_t st) {
   // two column blocks a workgroup once that still gives every CU one (halves the re-read of x)
-  return a.N16 >= 512 ? launch_g<T, S, MT, 2>(a, g, st) : launch_g<T, S, MT, 1>(a, g, st);
+  return a.N16 >= 512 ? launch_g<T, S, MT, 2, 4>(a, g, st) : launch_g<T, S, MT, 1, 4>(a, g, st);
 }
+#endif
 
 template <class T, class S>
 int launch_m(const W4Args& a, int g, hipStream_t st) {
@@ -250,7 +305,7 @@ __global__ __launch_bounds__(256) void w4_layout_kernel(LayoutArgs a) {
   a.w[blk * 256 + tid] = word;
   const int gpb = 128 / a.g, groups = (a.K + a.g - 1) / a.g;
   if (tid < gpb * 16) {
-    const int nn = nt * 16 + (tid & 15), gi = kb * gpb + (tid >> 4);
+    const int nn = nt * 16 + tid / gpb, gi = kb * gpb + tid % gpb;
     const bool in = nn < a.N && gi < groups;
     reinterpret_cast<S*>(a.ws)[blk * gpb * 16 + tid] =
         in ? reinterpret_cast<const S*>(a.scales)[(long)nn * a.lds_ + gi] : (S)0.f;
@@ -347,9 +402,8 @@ extern "C" int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void
   if (M == 0) return 0;
   if (!x || !weight || !scale_tiles || !y || ldx < K || ldy < N || ((uintptr_t)weight & 15) || M > 65535 * 16)
     return (int)hipErrorInvalidValue;
-  const int e = bf16 ? 2 : 4;
   W4Args a{x, (long)ldx, reinterpret_cast<const uint4*>(weight), scale_tiles, bias, y, (long)ldy, beta, act, M, N, K,
-           (K + 127) / 128, (N + 15) / 16, (((uintptr_t)x | (uintptr_t)(ldx * e)) & 15) == 0};
+           (K + 127) / 128, (N + 15) / 16};
   hipStream_t st = (hipStream_t)stream;
   if (bf16) return scale_bf16 ? launch_m<__bf16, __bf16>(a, group, st) : launch_m<__bf16, float>(a, group, st);
   return scale_bf16 ? launch_m<float, __bf16>(a, group, st) : launch_m<float, float>(a, group, st);

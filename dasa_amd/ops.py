@@ -1177,7 +1177,7 @@ class W4Weight:
         q = torch.stack([(w >> (4 * i)) & 15 for i in range(8)], -1)   # two's complement nibbles
         q = torch.where(q > 7, q - 16, q)
         q = q.permute(0, 3, 1, 4, 2, 5).reshape(n16 * 16, kb * 128)    # k = 128 block + 32 step + 8 quarter + nibble
-        s = self.scales.view(n16, kb * (128 // self.group), 16).transpose(1, 2).reshape(n16 * 16, -1).float()
+        s = self.scales.view(n16, kb, 16, 128 // self.group).transpose(1, 2).reshape(n16 * 16, -1).float()
         return (q * s.repeat_interleave(self.group, 1))[:N, :K].contiguous()
 
 
