@@ -139,7 +139,8 @@ SIGNATURES = {
     "dasa_w4_scale_count": (i64, [i32, i32, i32]),
     "dasa_w4_quantize": (i32, [vp, i64, i32, i32, i32, i32, vp, i64, vp, i64, i32, vp]),
     "dasa_w4_layout": (i32, [vp, i64, vp, i64, i32, i32, i32, i32, vp, vp, vp]),
-    "dasa_gemm_w4": (i32, [vp, i64, i32, vp, vp, i32, i32, vp, i32, f32, vp, i64, i32, i32, i32, vp]),
+    "dasa_gemm_w4": (i32, [vp, i64, i32, vp, vp, i32, i32, vp, i32, f32, vp, i64, i32, i32, i32, vp, i64, vp]),
+    "dasa_gemm_w4_workspace": (i64, [i32, i32, i32, i32]),
     "dasa_logit_rules_workspace": (i64, [i32, i32]),
     "dasa_logit_rules": (i32, [C.POINTER(LogitRules), vp, i64, vp]),
 }

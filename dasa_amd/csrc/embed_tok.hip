@@ -126,25 +126,47 @@ int launch_fwd(LookupArgs a, long rows, hipStream_t st) {
 
 // ------------------------------------------------------------------ tokens in sorted order
 constexpr int kSortWaves = 16;
-constexpr int kMaxRange = 960;        // vocabulary rows of one sort workgroup (its counters: 60 KB of LDS)
+constexpr int kMaxRange = 512;        // vocabulary rows of one sort workgroup (its counters: 32 KB of LDS)
+constexpr int kList = 256;            // tokens of its range that a wave notes on the first pass
 
 struct SortArgs {
   const void* ids;
-  int T, V, R, pad;
+  int T, V, R;
   int* start;     // [V + 1] first sorted index of every token id
   int* order;     // [T] positions in sorted order
 };
 
-// Every token of one 64-token step that lies in this workgroup's range, one distinct id at a time: f(bin, same-id
-// lanes). Few tokens of a step lie in one range (64 / gridDim on average), and a frequent id is one turn.
-template <class F>
-__device__ __forceinline__ void each_bin(int bin, bool in, F f) {
+// 64 U ids a call, as 32-bit values: an id outside 32 bits becomes 2^32 - 1, which no vocabulary holds
+template <int U>
+__device__ __forceinline__ void load_ids(const int64_t* ids, int t, int t1, int lane, unsigned (&u)[U]) {
+  uint2 v[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int i = t + 64 * k + lane;
+    v[k] = i < t1 ? reinterpret_cast<const uint2*>(ids)[i] : make_uint2(~0u, ~0u);
+  }
+#pragma unroll
+  for (int k = 0; k < U; ++k) u[k] = v[k].y == 0 ? v[k].x : ~0u;
+}
+template <int U>
+__device__ __forceinline__ void load_ids(const int32_t* ids, int t, int t1, int lane, unsigned (&u)[U]) {
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int i = t + 64 * k + lane;
+    u[k] = i < t1 ? (unsigned)ids[i] : ~0u;
+  }
+}
+
+// Write the positions of up to 64 tokens of the range (lanes with `in`, in lane order) at their ranks, one distinct
+// id at a time: a frequent id is one turn.
+__device__ __forceinline__ void place(int* cursor, int* order, int lane, bool in, int bin, int pos) {
   unsigned long long m = __ballot(in);
   while (m) {
-    const int lead = __builtin_ctzll(m);
-    const int b = __builtin_amdgcn_readlane(bin, lead);
+    const int b = __builtin_amdgcn_readlane(bin, __builtin_ctzll(m));
     const unsigned long long same = __ballot(in && bin == b);
-    f(b, same);
+    const int c = cursor[b];
+    if ((same >> lane) & 1) order[c + __popcll(same & ((1ull << lane) - 1))] = pos;
+    cursor[b] = c + __popcll(same);                  // every lane stores the same value
     m &= ~same;
   }
 }
@@ -153,38 +175,47 @@ template <class I>
 __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a) {
   extern __shared__ int hist[];                    // [waves][R] counts, then write cursors
   __shared__ int below[kSortWaves], wsum[kSortWaves];
+  __shared__ int lpos[kSortWaves][kList];
+  __shared__ unsigned short lbin[kSortWaves][kList];
   const I* ids = reinterpret_cast<const I*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int lo = blockIdx.x * a.R, n = min(a.R, a.V - lo);
+  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
   for (int i = tid; i < kSortWaves * a.R; i += 64 * kSortWaves) hist[i] = 0;
   __syncthreads();
   const int seg = (((a.T + kSortWaves - 1) / kSortWaves) + 63) & ~63;
   const int t0 = min(w * seg, a.T), t1 = min(t0 + seg, a.T);
   int* mine = hist + w * a.R;
-  int nb = 0;
+  int nb = 0, found = 0;
   constexpr int U = 8;                             // id loads in flight
+  unsigned u[U], next[U];
+  load_ids<U>(ids, t0, t1, lane, u);
   for (int t = t0; t < t1; t += 64 * U) {
-    long v[U];
+    load_ids<U>(ids, t + 64 * U, t1, lane, next);
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int i = t + 64 * k + lane;
-      v[k] = i < t1 ? (long)ids[i] : -1;
+      nb += __popcll(__ballot(u[k] < lo));
+      const unsigned bin = u[k] - lo;
+      const unsigned long long m = __ballot(bin < n);
+      if (m) {
+        if (bin < n) {
+          atomicAdd(&mine[bin], 1);
+          const int at = found + __popcll(m & ((1ull << lane) - 1));
+          if (at < kList) {
+            lpos[w][at] = t + 64 * k + lane;
+            lbin[w][at] = (unsigned short)bin;
+          }
+        }
+        found += __popcll(m);
+      }
     }
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const bool ok = v[k] >= 0 && v[k] < a.V && v[k] != a.pad;
-      nb += __popcll(__ballot(ok && v[k] < lo));
-      const int bin = (int)v[k] - lo;
-      each_bin(bin, ok && v[k] >= lo && v[k] < lo + n, [&](int b, unsigned long long same) {
-        mine[b] += __popcll(same);                 // every lane stores the same value
-      });
-    }
+    for (int k = 0; k < U; ++k) u[k] = next[k];
   }
   if (lane == 0) below[w] = nb;
   __syncthreads();
   // exclusive scan over the range's ids (thread = id), then over the waves of one id
   int tot = 0;
-  if (tid < n)
+  if (tid < (int)n)
     for (int k = 0; k < kSortWaves; ++k) tot += hist[k * a.R + tid];
   int incl = tot;
 #pragma unroll
@@ -197,33 +228,27 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   int base = 0;
   for (int k = 0; k < kSortWaves; ++k) base += below[k] + (k < w ? wsum[k] : 0);
   int at = base + incl - tot;
-  if (tid < n) {
+  if (tid < (int)n) {
     a.start[lo + tid] = at;
     for (int k = 0; k < kSortWaves; ++k) {
       const int c = hist[k * a.R + tid];
       hist[k * a.R + tid] = at;
       at += c;
     }
-    if (lo + tid == a.V - 1) a.start[a.V] = at;
+    if ((int)lo + tid == a.V - 1) a.start[a.V] = at;
   }
   __syncthreads();
-  for (int t = t0; t < t1; t += 64 * U) {
-    long v[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const int i = t + 64 * k + lane;
-      v[k] = i < t1 ? (long)ids[i] : -1;
+  if (found <= kList) {
+    for (int i = 0; i < found; i += 64) {
+      const int j = min(i + lane, found - 1);
+      place(mine, a.order, lane, i + lane < found, lbin[w][j], lpos[w][j]);
     }
+    return;
+  }
+  for (int t = t0; t < t1; t += 64 * U) {          // a hot range: its ids again
+    load_ids<U>(ids, t, t1, lane, u);
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      const bool in = v[k] >= lo && v[k] < lo + n && v[k] != a.pad;
-      const int bin = (int)v[k] - lo;
-      each_bin(bin, in, [&](int b, unsigned long long same) {
-        const int c = mine[b];
-        if ((same >> lane) & 1) a.order[c + __popcll(same & ((1ull << lane) - 1))] = t + 64 * k + lane;
-        mine[b] = c + __popcll(same);              // every lane stores the same value
-      });
-    }
+    for (int k = 0; k < U; ++k) place(mine, a.order, lane, u[k] - lo < n, (int)(u[k] - lo), t + 64 * k + lane);
   }
 }
 
@@ -243,35 +268,35 @@ struct BwdArgs {
   float* parts;            // [chunks][2][ldp] sums of hot rows' parts, or null (no row can be hot)
   long ldp;
   void* dtable; long ldt;
-  int V, E, slices;
+  int V, E, pad;           // pad: the id without a gradient, or -1
   unsigned row_blocks;     // blocks of the rows kernel that take table rows; the others take chunks
   float scale;
   int accumulate;
 };
 
-// acc += the dout rows of n <= 64 tokens whose positions the lanes hold, tokens lane0 .. lane0 + n in order. Four rows
-// are in flight at a time.
+// acc += the dout rows of n <= 64 tokens whose positions the lanes hold, tokens lane0 .. lane0 + n in order; K rows in
+// flight at a time.
+template <class T, int K>
+__device__ __forceinline__ int add_rows_by(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
+                                           int j, int n) {
+  for (; j + K <= n; j += K) {
+    typename Vec<T>::type x[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      x[k] = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j + k) * ldd, left);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) acc[e] += (float)x[k][e];
+  }
+  return j;
+}
 template <class T>
 __device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
                                          int n) {
-  constexpr int N = Vec<T>::N;
-  typedef typename Vec<T>::type V;
-  int j = 0;
-  for (; j + 4 <= n; j += 4) {
-    V x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      x[k] = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j + k) * ldd, left);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += (float)x[k][e];
-  }
-  for (; j < n; ++j) {
-    const V x = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j) * ldd, left);
-#pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] += (float)x[e];
-  }
+  int j = add_rows_by<T, 16>(acc, d, ldd, left, pos, lane0, 0, n);
+  j = add_rows_by<T, 4>(acc, d, ldd, left, pos, lane0, j, n);
+  add_rows_by<T, 1>(acc, d, ldd, left, pos, lane0, j, n);
 }
 
 template <class T>
@@ -302,7 +327,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   if (blockIdx.x < a.row_blocks) {
     const long v = (long)blockIdx.x * 4 + w;
     if (v >= a.V) return;
-    const int s = a.start[v], n = a.start[v + 1] - s;
+    const int s = a.start[v], n = v == a.pad ? 0 : a.start[v + 1] - s;
     if (n > kChunk || (a.accumulate && n == 0)) return;
     const int pos = lane < n ? a.order[s + lane] : 0;
     if (left > 0) {
@@ -318,7 +343,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   const int pos = a.order[j0 + min(lane, m - 1)];
   const long id = id_at(a, pos);
   const int rs = a.start[id], re = a.start[id + 1];
-  const bool hot = re - rs > kChunk;
+  const bool hot = re - rs > kChunk && id != a.pad;
   float* part = a.parts + c * 2 * a.ldp + col;
   // the row that owns the chunk's first token, then the row that owns its last
   const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
@@ -351,7 +376,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   const int last = min(j0 + kChunk, total) - 1;
   const long v = id_at(a, a.order[last]);                 // a hot row that starts here reaches past the chunk
   const int rs = a.start[v], re = a.start[v + 1];
-  if (re - rs <= kChunk || rs < j0) return;
+  if (re - rs <= kChunk || rs < j0 || v == a.pad) return;
   const int n = (re - 1) / kChunk - (int)c + 1;           // its parts: chunks c .. c + n - 1
   const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
   float acc[N];
@@ -381,14 +406,14 @@ inline long part_stride(int E, int bf16) {      // whole units, so a partial uni
 
 template <class T>
 int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
-  a.slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
+  const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   a.row_blocks = (unsigned)((a.V + 3) / 4);
   const long chunks = a.parts ? (tokens + kChunk - 1) / kChunk : 0;
-  const dim3 grid(a.row_blocks + (unsigned)((chunks + 3) / 4), a.slices);
+  const dim3 grid(a.row_blocks + (unsigned)((chunks + 3) / 4), slices);
   hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
   if (chunks) {
-    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)chunks, a.slices), dim3(64 * kJoinWaves), 0, st, a);
+    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)chunks, slices), dim3(64 * kJoinWaves), 0, st, a);
     DASA_CHECK_LAUNCH();
   }
   return 0;
@@ -431,7 +456,7 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   if (G < 256) G = V < 256 ? V : 256;
   const int R = (V + G - 1) / G;
   G = (V + R - 1) / R;
-  SortArgs sa{ids, (int)T, V, R, padding_idx, start, order};
+  SortArgs sa{ids, (int)T, V, R, start, order};
   const size_t lds = (size_t)kSortWaves * R * sizeof(int);
   if (ids_bytes == 8)
     hipLaunchKernelGGL(token_sort_kernel<int64_t>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
@@ -443,6 +468,6 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   ba.start = start; ba.order = order;
   if (T > kChunk) ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
   ba.ldp = part_stride(E, bf16);
-  ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.scale = scale; ba.accumulate = accumulate;
+  ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.pad = padding_idx; ba.scale = scale; ba.accumulate = accumulate;
   return bf16 ? launch_rows<__bf16>(ba, T, st) : launch_rows<float>(ba, T, st);
 }

@@ -1260,10 +1260,13 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     x2, M, ldx = _row_view(x, "linear_w4")
     if M == 0:
         return out
-    _call("dasa_gemm_w4", "gemm_w4", _lib.lib().dasa_gemm_w4, x2.data_ptr(), ldx, bf16, w.tiles.data_ptr(),
+    L = _lib.lib()
+    nws = L.dasa_gemm_w4_workspace(M, N, K, bf16)
+    ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None
+    _call("dasa_gemm_w4", "gemm_w4", L.dasa_gemm_w4, x2.data_ptr(), ldx, bf16, w.tiles.data_ptr(),
           w.scales.data_ptr(), 1 if w.scales.dtype == torch.bfloat16 else 0, w.group,
-          None if b is None else b.data_ptr(), _ACT_IDS[act], float(beta), out.data_ptr(), ldo, M, N, K, _stream(),
-          flops=2.0 * M * N * K, nbytes=w.nbytes() + (1.0 * M * K + M * N) * x.element_size())
+          None if b is None else b.data_ptr(), _ACT_IDS[act], float(beta), out.data_ptr(), ldo, M, N, K,
+          None if ws is None else ws.data_ptr(), nws, _stream(), flops=2.0 * M * N * K, nbytes=w.nbytes() + (1.0 * M * K + M * N) * x.element_size())
     return out
 
 

@@ -391,10 +391,12 @@ int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int3
 int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16, int32_t N,
                    int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream);
 /* y = act(x W^T + bias) + beta * y: x [M][ldx], y [M][ldy], both fp32 (bf16 = 0) or both bf16; fp32 accumulation at
- * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. Any M, N, K; made for few rows. */
+ * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. Any M, N, K; made for few rows.
+ * ws: dasa_gemm_w4_workspace(M, N, K, bf16) bytes of scratch, 16-B aligned (0: none). */
+int64_t dasa_gemm_w4_workspace(int32_t M, int32_t N, int32_t K, int32_t bf16);
 int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, const void* scale_tiles,
                  int32_t scale_bf16, int32_t group, const float* bias, int32_t act, float beta, void* y, int64_t ldy,
-                 int32_t M, int32_t N, int32_t K, void* stream);
+                 int32_t M, int32_t N, int32_t K, void* ws, int64_t ws_bytes, void* stream);
 
 /* ---- rules on the logits of a decoding step (speaker.py:319-323) --------------------------------------------
  * For row b and token v: c = occurrences of v in history[b][0 .. lengths[b]) (ids outside [0, V) are ignored);

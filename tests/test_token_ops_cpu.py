@@ -89,10 +89,10 @@ def test_entry_points_refuse_before_a_launch():
     assert L.dasa_w4_quantize(P, 64, 0, 4, 64, 16, P, 32, P, 4, 0, None) == INVALID
     assert L.dasa_w4_quantize(P, 63, 0, 4, 64, 64, P, 32, P, 1, 0, None) == INVALID
     assert L.dasa_w4_layout(P, 31, P, 1, 0, 4, 64, 64, P, P, None) == INVALID
-    assert L.dasa_gemm_w4(P, 64, 0, P, P, 0, 64, None, 0, 0.0, P, 4, 0, 4, 64, None) == 0        # no rows
+    assert L.dasa_gemm_w4(P, 64, 0, P, P, 0, 64, None, 0, 0.0, P, 4, 0, 4, 64, None, 0, None) == 0        # no rows
     for ldx, w, group, act, ldy, M in ((63, P, 64, 0, 4, 2), (64, P + 8, 64, 0, 4, 2), (64, P, 65, 0, 4, 2),
                                        (64, P, 64, 9, 4, 2), (64, P, 64, 0, 3, 2), (64, P, 64, 0, 4, -1)):
-        assert L.dasa_gemm_w4(P, ldx, 0, w, P, 0, group, None, act, 0.0, P, ldy, M, 4, 64, None) == INVALID
+        assert L.dasa_gemm_w4(P, ldx, 0, w, P, 0, group, None, act, 0.0, P, ldy, M, 4, 64, None, 0, None) == INVALID
     good = dict(B=2, V=9000, L=4, ids_bytes=8, logits=P, ld=9000, out=P, ldo=9000, history=P, ldh=4, repetition0=1.0)
     def desc(**kw):
         d = _lib.LogitRules()
