@@ -132,28 +132,45 @@ constexpr int kList = 256;            // tokens of its range that a wave notes o
 struct SortArgs {
   const void* ids;
   int T, V, R;
+  unsigned pad;   // the id without a gradient, or 2^32 - 1
   int* start;     // [V + 1] first sorted index of every token id
   int* order;     // [T] positions in sorted order
 };
 
-// 64 U ids a call, as 32-bit values: an id outside 32 bits becomes 2^32 - 1, which no vocabulary holds
-template <int U>
-__device__ __forceinline__ void load_ids(const int64_t* ids, int t, int t1, int lane, unsigned (&u)[U]) {
-  uint2 v[U];
+// One id as 32 bits: 2^32 - 1, which no vocabulary holds, for the padding id and for ids outside 32 bits.
+__device__ __forceinline__ unsigned token(uint2 v, unsigned pad) { return v.y == 0 && v.x != pad ? v.x : ~0u; }
+__device__ __forceinline__ unsigned token(unsigned v, unsigned pad) { return v != pad ? v : ~0u; }
+__device__ __forceinline__ uint2 no_token(uint2) { return make_uint2(~0u, ~0u); }
+__device__ __forceinline__ unsigned no_token(unsigned) { return ~0u; }
+
+// f(position, token) for the ids [t0, t1) of a wave, 64 at a time, U loads in flight; f is called by whole waves
+template <class W, int U, class F>
+__device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lane, unsigned pad, F f) {
+  int t = t0;
+  if (t + 64 * U <= t1) {
+    W v[U], next[U];
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int i = t + 64 * k + lane;
-    v[k] = i < t1 ? reinterpret_cast<const uint2*>(ids)[i] : make_uint2(~0u, ~0u);
+    for (int k = 0; k < U; ++k) v[k] = ids[t + lane + 64 * k];
+    for (; t + 64 * U <= t1; t += 64 * U) {
+      const W* p = ids + min(t + 64 * U, t1 - 64 * U) + lane;      // the next group, or the last again
+#pragma unroll
+      for (int k = 0; k < U; ++k) next[k] = p[64 * k];
+#pragma unroll
+      for (int k = 0; k < U; ++k) f(t + 64 * k + lane, token(v[k], pad));
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = next[k];
+    }
   }
+  for (; t < t1; t += 64 * 4) {
+    W v[4];
 #pragma unroll
-  for (int k = 0; k < U; ++k) u[k] = v[k].y == 0 ? v[k].x : ~0u;
-}
-template <int U>
-__device__ __forceinline__ void load_ids(const int32_t* ids, int t, int t1, int lane, unsigned (&u)[U]) {
+    for (int k = 0; k < 4; ++k) {
+      const int i = t + 64 * k + lane;
+      v[k] = ids[min(i, t1 - 1)];
+      if (i >= t1) v[k] = no_token(v[k]);
+    }
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const int i = t + 64 * k + lane;
-    u[k] = i < t1 ? (unsigned)ids[i] : ~0u;
+    for (int k = 0; k < 4; ++k) f(t + 64 * k + lane, token(v[k], pad));
   }
 }
 
@@ -171,13 +188,13 @@ __device__ __forceinline__ void place(int* cursor, int* order, int lane, bool in
   }
 }
 
-template <class I>
+template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a) {
   extern __shared__ int hist[];                    // [waves][R] counts, then write cursors
   __shared__ int below[kSortWaves], wsum[kSortWaves];
   __shared__ int lpos[kSortWaves][kList];
   __shared__ unsigned short lbin[kSortWaves][kList];
-  const I* ids = reinterpret_cast<const I*>(a.ids);
+  const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
   for (int i = tid; i < kSortWaves * a.R; i += 64 * kSortWaves) hist[i] = 0;
@@ -186,31 +203,30 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   const int t0 = min(w * seg, a.T), t1 = min(t0 + seg, a.T);
   int* mine = hist + w * a.R;
   int nb = 0, found = 0;
-  constexpr int U = 8;                             // id loads in flight
-  unsigned u[U], next[U];
-  load_ids<U>(ids, t0, t1, lane, u);
-  for (int t = t0; t < t1; t += 64 * U) {
-    load_ids<U>(ids, t + 64 * U, t1, lane, next);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      nb += __popcll(__ballot(u[k] < lo));
-      const unsigned bin = u[k] - lo;
-      const unsigned long long m = __ballot(bin < n);
-      if (m) {
-        if (bin < n) {
-          atomicAdd(&mine[bin], 1);
-          const int at = found + __popcll(m & ((1ull << lane) - 1));
-          if (at < kList) {
-            lpos[w][at] = t + 64 * k + lane;
-            lbin[w][at] = (unsigned short)bin;
-          }
-        }
-        found += __popcll(m);
+  each_token<W, 8>(ids, t0, t1, lane, a.pad, [&](int pos, unsigned u) {
+    nb += __popcll(__ballot(u < lo));
+    const unsigned bin = u - lo;
+    const bool in = bin < n;
+    unsigned long long m = __ballot(in);
+    if (!m) return;
+    const int at = found + __popcll(m & ((1ull << lane) - 1));
+    if (in && at < kList) {
+      lpos[w][at] = pos;
+      lbin[w][at] = (unsigned short)bin;
+    }
+    const int c = __popcll(m);
+    found += c;
+    if (c <= 8) {
+      if (in) atomicAdd(&mine[bin], 1);
+    } else {                                       // dense: a frequent id would be one address for most lanes
+      while (m) {
+        const int b = __builtin_amdgcn_readlane((int)bin, __builtin_ctzll(m));
+        const unsigned long long same = __ballot(in && (int)bin == b);
+        mine[b] += __popcll(same);                 // every lane stores the same value
+        m &= ~same;
       }
     }
-#pragma unroll
-    for (int k = 0; k < U; ++k) u[k] = next[k];
-  }
+  });
   if (lane == 0) below[w] = nb;
   __syncthreads();
   // exclusive scan over the range's ids (thread = id), then over the waves of one id
@@ -245,11 +261,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
     }
     return;
   }
-  for (int t = t0; t < t1; t += 64 * U) {          // a hot range: its ids again
-    load_ids<U>(ids, t, t1, lane, u);
-#pragma unroll
-    for (int k = 0; k < U; ++k) place(mine, a.order, lane, u[k] - lo < n, (int)(u[k] - lo), t + 64 * k + lane);
-  }
+  each_token<W, 8>(ids, t0, t1, lane, a.pad, [&](int pos, unsigned u) {      // a hot range: its ids again
+    place(mine, a.order, lane, u - lo < n, (int)(u - lo), pos);
+  });
 }
 
 // ------------------------------------------------------------------ gradient rows
@@ -257,7 +271,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
 // multiples of kChunk in the sorted order, so that a padding or stop word with a tenth of the tokens does not run on
 // one wave: each chunk leaves the sum of its part of at most two hot rows (one that reaches into it, one that reaches
 // out of it: a hot row is longer than a chunk), and a third launch adds a row's parts in chunk order.
-constexpr int kChunk = 64;
+constexpr int kChunk = 32;
 constexpr int kJoinWaves = 16;
 
 struct BwdArgs {
@@ -268,7 +282,7 @@ struct BwdArgs {
   float* parts;            // [chunks][2][ldp] sums of hot rows' parts, or null (no row can be hot)
   long ldp;
   void* dtable; long ldt;
-  int V, E, pad;           // pad: the id without a gradient, or -1
+  int V, E;
   unsigned row_blocks;     // blocks of the rows kernel that take table rows; the others take chunks
   float scale;
   int accumulate;
@@ -294,8 +308,8 @@ __device__ __forceinline__ int add_rows_by(float (&acc)[Vec<T>::N], const T* d, 
 template <class T>
 __device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
                                          int n) {
-  int j = add_rows_by<T, 16>(acc, d, ldd, left, pos, lane0, 0, n);
-  j = add_rows_by<T, 4>(acc, d, ldd, left, pos, lane0, j, n);
+  int j = add_rows_by<T, 8>(acc, d, ldd, left, pos, lane0, 0, n);
+  j = add_rows_by<T, 2>(acc, d, ldd, left, pos, lane0, j, n);
   add_rows_by<T, 1>(acc, d, ldd, left, pos, lane0, j, n);
 }
 
@@ -327,7 +341,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   if (blockIdx.x < a.row_blocks) {
     const long v = (long)blockIdx.x * 4 + w;
     if (v >= a.V) return;
-    const int s = a.start[v], n = v == a.pad ? 0 : a.start[v + 1] - s;
+    const int s = a.start[v], n = a.start[v + 1] - s;
     if (n > kChunk || (a.accumulate && n == 0)) return;
     const int pos = lane < n ? a.order[s + lane] : 0;
     if (left > 0) {
@@ -343,7 +357,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   const int pos = a.order[j0 + min(lane, m - 1)];
   const long id = id_at(a, pos);
   const int rs = a.start[id], re = a.start[id + 1];
-  const bool hot = re - rs > kChunk && id != a.pad;
+  const bool hot = re - rs > kChunk;
   float* part = a.parts + c * 2 * a.ldp + col;
   // the row that owns the chunk's first token, then the row that owns its last
   const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
@@ -362,33 +376,51 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   }
 }
 
-// One workgroup = (chunk, slice): the hot row that starts in the chunk, if any, as the sum of its parts. The waves
-// take runs of parts, joined in order.
+// parts [k0, k1) of the hot row whose first part is slot `first` of chunk c, added in order
+template <class T>
+__device__ __forceinline__ void add_parts(float (&acc)[Vec<T>::N], const BwdArgs& a, long c, int first, int k0, int k1,
+                                          int col) {
+#pragma unroll 4
+  for (int k = k0; k < k1; ++k) {
+    const float* p = a.parts + ((c + k) * 2 + (k == 0 ? first : 0)) * a.ldp + col;
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e) acc[e] += p[e];
+  }
+}
+
+// One workgroup = (kJoinWaves chunks, slice). A hot row that starts in a chunk reaches past its end, so the chunk's
+// last token names it. Rows of up to kJoinWaves parts: one wave each. The one longer row that may start in the group
+// (it reaches past the group's end) takes the whole workgroup: the waves add runs of parts, joined in order.
 template <class T>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
   __shared__ float sum[kJoinWaves][64][N];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int col = (blockIdx.y * 64 + lane) * N, left = a.E - col;
-  const long c = blockIdx.x;
-  const int j0 = (int)(c * kChunk), total = a.start[a.V];
-  if (j0 >= total) return;
-  const int last = min(j0 + kChunk, total) - 1;
-  const long v = id_at(a, a.order[last]);                 // a hot row that starts here reaches past the chunk
-  const int rs = a.start[v], re = a.start[v + 1];
-  if (re - rs <= kChunk || rs < j0 || v == a.pad) return;
-  const int n = (re - 1) / kChunk - (int)c + 1;           // its parts: chunks c .. c + n - 1
-  const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
+  const int total = a.start[a.V];
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  if (left > 0)
-#pragma unroll 4
-    for (int k = k0; k < k1; ++k) {
-      const float* p = a.parts + ((c + k) * 2 + (k == 0 && rs > j0 ? 1 : 0)) * a.ldp + col;
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += p[e];
+  const long c = (long)blockIdx.x * kJoinWaves + w;
+  const long j0 = c * kChunk;
+  if (j0 < total) {
+    const long v = id_at(a, a.order[min(j0 + kChunk, (long)total) - 1]);
+    const int rs = a.start[v], re = a.start[v + 1], n = (re - 1) / kChunk - (int)c + 1;
+    if (re - rs > kChunk && rs >= j0 && n <= kJoinWaves && left > 0) {
+      add_parts<T>(acc, a, c, rs > j0, 0, n, col);
+      write_row<T>(a, v, col, left, acc);
     }
+  }
+  const long g0 = (long)blockIdx.x * kJoinWaves * kChunk;
+  if (g0 >= total) return;
+  const long v = id_at(a, a.order[min(g0 + kJoinWaves * kChunk, (long)total) - 1]);
+  const int rs = a.start[v], re = a.start[v + 1];
+  const int c0 = rs / kChunk, n = (re - 1) / kChunk - c0 + 1;
+  if (rs < g0 || n <= kJoinWaves) return;
+  const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  if (left > 0) add_parts<T>(acc, a, c0, rs > c0 * kChunk, k0, k1, col);
 #pragma unroll
   for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
   __syncthreads();
@@ -413,7 +445,8 @@ int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
   hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
   if (chunks) {
-    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)chunks, slices), dim3(64 * kJoinWaves), 0, st, a);
+    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
+                       dim3(64 * kJoinWaves), 0, st, a);
     DASA_CHECK_LAUNCH();
   }
   return 0;
@@ -456,18 +489,18 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   if (G < 256) G = V < 256 ? V : 256;
   const int R = (V + G - 1) / G;
   G = (V + R - 1) / R;
-  SortArgs sa{ids, (int)T, V, R, start, order};
+  SortArgs sa{ids, (int)T, V, R, padding_idx < 0 ? ~0u : (unsigned)padding_idx, start, order};
   const size_t lds = (size_t)kSortWaves * R * sizeof(int);
   if (ids_bytes == 8)
-    hipLaunchKernelGGL(token_sort_kernel<int64_t>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
+    hipLaunchKernelGGL(token_sort_kernel<uint2>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
   else
-    hipLaunchKernelGGL(token_sort_kernel<int32_t>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
+    hipLaunchKernelGGL(token_sort_kernel<unsigned>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
   DASA_CHECK_LAUNCH();
   BwdArgs ba{};
   ba.dout = dout; ba.ldd = (long)ldd; ba.ids = ids; ba.ids64 = ids_bytes == 8;
   ba.start = start; ba.order = order;
   if (T > kChunk) ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
   ba.ldp = part_stride(E, bf16);
-  ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.pad = padding_idx; ba.scale = scale; ba.accumulate = accumulate;
+  ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.scale = scale; ba.accumulate = accumulate;
   return bf16 ? launch_rows<__bf16>(ba, T, st) : launch_rows<float>(ba, T, st);
 }

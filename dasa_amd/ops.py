@@ -1034,17 +1034,24 @@ def gather_rows(ta, ia, tb, ib, out):
 
 
 # ------------------------------------------------------------------- token ends of a word step
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def _on_device(what, *ts):
-    """Every given tensor lives on the current device (the launch stream is the current device's): else a
-    DasaError, for host tensors as everywhere and for tensors of another GPU."""
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else None
+    """Every given tensor lives on the current device, whose index is returned (the launch stream is the current
+    device's): else a DasaError, for host tensors as everywhere and for tensors of another GPU."""
+    cur = None
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()
+        if d < 0:
             raise _lib.DasaError(f"{what}: needs device tensors (the HIP path has no CPU fallback)")
-        if t.device.index != cur:
-            raise _lib.DasaError(f"{what}: a tensor is on {t.device}, the current device is cuda:{cur}")
+        if cur is None:
+            cur = _get_device()
+        if d != cur:
+            raise _lib.DasaError(f"{what}: a tensor is on cuda:{d}, the current device is cuda:{cur}")
+    return cur
 
 
 def _float_type(t, what):
@@ -1067,7 +1074,8 @@ def _ids_bytes(ids, what):
 def _row_view(t, what):
     """[..., N] as (2-D tensor of unit inner stride, rows, row stride >= N): a copy where the layout needs one."""
     N = t.shape[-1]
-    t = t.reshape(-1, N)
+    if t.dim() != 2:
+        t = t.reshape(-1, N)
     if N and t.shape[0] and ((N > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < N)):
         t = t.contiguous()
     return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else N
@@ -1092,13 +1100,13 @@ def embedding(ids, table, scale=1.0, out=None):
     if table.dim() != 2:
         raise _lib.DasaError(f"embedding: table must be [V, E], got {tuple(table.shape)}")
     bf16, nb = _float_type(table, "embedding.table"), _ids_bytes(ids, "embedding.ids")
-    _on_device("embedding", ids, table, out)
+    dev = _on_device("embedding", ids, table, out)
     V, E = table.shape
     if E > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < E:
         raise _lib.DasaError("embedding: the table's rows must be contiguous")
     ids = ids.contiguous()
     if out is None:
-        out = torch.empty(*ids.shape, E, dtype=table.dtype, device=table.device)
+        out = table.new_empty((*ids.shape, E))
         ldo = E
     else:
         ldo = _out_rows(out, (*ids.shape, E), table, "embedding")
@@ -1107,12 +1115,12 @@ def embedding(ids, table, scale=1.0, out=None):
         return out
     if V == 0:
         raise _lib.DasaError("embedding: the table has no rows")
-    err = _ERR.get(table.device.index)
+    err = _ERR.get(dev)
     if err is None and not torch.cuda.is_current_stream_capturing():
         err = _error_word(table.device)
     _call("dasa_embedding_fwd", "embed", _lib.lib().dasa_embedding_fwd, table.data_ptr(), max(table.stride(0), E),
           ids.data_ptr(), nb, T, V, E, float(scale), bf16, out.data_ptr(), ldo,
-          None if err is None else err.data_ptr(), _stream(), nbytes=T * (nb + 2.0 * E * table.element_size()))
+          None if err is None else err.data_ptr(), _raw_stream(dev), nbytes=T * (nb + 2.0 * E * table.element_size()))
     return out
 
 
@@ -1122,7 +1130,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     padding_idx and of ids that do not occur are zero; ids outside the vocabulary are skipped. With out and
     accumulate=True the sums are added into out (rows without tokens are not touched)."""
     bf16, nb = _float_type(dout, "embedding_bwd.dout"), _ids_bytes(ids, "embedding_bwd.ids")
-    _on_device("embedding_bwd", dout, ids, out)
+    dev = _on_device("embedding_bwd", dout, ids, out)
     vocab = int(vocab)
     if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise _lib.DasaError(f"embedding_bwd: dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)}")
@@ -1136,7 +1144,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
         raise _lib.DasaError("embedding_bwd: accumulate=True needs out")
     E = dout.shape[-1]
     if out is None:
-        out = torch.empty(vocab, E, dtype=dout.dtype, device=dout.device)
+        out = dout.new_empty((vocab, E))
         ldo = E
     else:
         ldo = _out_rows(out, (vocab, E), dout, "embedding_bwd")
@@ -1148,7 +1156,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     ws = torch.empty(L.dasa_embedding_bwd_workspace(T, vocab, E), dtype=torch.uint8, device=dout.device)
     _call("dasa_embedding_bwd", "embed_bwd", L.dasa_embedding_bwd, d.data_ptr(), ldd, ids.data_ptr(), nb, T, vocab, E,
           float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
-          _stream(), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
+          _raw_stream(dev), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
     return out
 
 
@@ -1157,17 +1165,15 @@ class W4Weight:
     is (code - 8) * scale, code in 0..15. Made once by quantize_w4 or pack_w4 and kept by the program (its tensors
     are freed with it); the weight it was made from is not referenced."""
 
-    __slots__ = ("tiles", "scales", "shape", "group")
+    __slots__ = ("tiles", "scales", "shape", "group", "nbytes")
 
     def __init__(self, tiles, scales, shape, group):
         self.tiles, self.scales, self.shape, self.group = tiles, scales, tuple(shape), group
+        self.nbytes = tiles.numel() * 4 + scales.numel() * scales.element_size()
 
     @property
     def device(self):
         return self.tiles.device
-
-    def nbytes(self):
-        return self.tiles.numel() * 4 + self.scales.numel() * self.scales.element_size()
 
     def dequantize(self):
         """The fp32 weight [N, K] that linear_w4 multiplies with."""
@@ -1246,14 +1252,14 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
         raise _lib.DasaError(f"linear_w4: the bias must be a contiguous float32 [{N}]")
     if act not in _ACT_IDS:
         raise _lib.DasaError(f"linear_w4: unknown activation {act!r}")
-    _on_device("linear_w4", x, w.tiles, b, out)
+    dev = _on_device("linear_w4", x, w.tiles, b, out)
     if torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad)):
         raise _lib.DasaError("linear_w4 is forward only: call it under torch.no_grad()")
     shape = (*x.shape[:-1], N)
     if out is None:
         if beta != 0.0:
             raise _lib.DasaError("linear_w4: beta needs out")
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(shape)
         ldo = N
     else:
         ldo = _out_rows(out, shape, x, "linear_w4")
@@ -1266,7 +1272,7 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     _call("dasa_gemm_w4", "gemm_w4", L.dasa_gemm_w4, x2.data_ptr(), ldx, bf16, w.tiles.data_ptr(),
           w.scales.data_ptr(), 1 if w.scales.dtype == torch.bfloat16 else 0, w.group,
           None if b is None else b.data_ptr(), _ACT_IDS[act], float(beta), out.data_ptr(), ldo, M, N, K,
-          None if ws is None else ws.data_ptr(), nws, _stream(), flops=2.0 * M * N * K, nbytes=w.nbytes() + (1.0 * M * K + M * N) * x.element_size())
+          None if ws is None else ws.data_ptr(), nws, _raw_stream(dev), flops=2.0 * M * N * K, nbytes=w.nbytes + (1.0 * M * K + M * N) * x.element_size())
     return out
 
 
@@ -1275,7 +1281,7 @@ def _penalty(v, B, what, neutral):
     if v is None:
         return None, neutral
     if isinstance(v, torch.Tensor):
-        if v.dtype != torch.float32 or tuple(v.shape) != (B,) or (B > 1 and v.stride(0) != 1):
+        if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != B or (B > 1 and v.stride(0) != 1):
             raise _lib.DasaError(f"logit_rules: {what} must be a number or a contiguous float32 [{B}]")
         _on_device("logit_rules", v)
         return v.data_ptr(), neutral
@@ -1300,36 +1306,38 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
         raise _lib.DasaError(f"logit_rules: logits must be [B, V], got {tuple(logits.shape)}")
     bf16 = _float_type(logits, "logit_rules.logits")
     B, V = logits.shape
-    _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
+    dev = _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
     if V == 0 or B > 65535:
         raise _lib.DasaError(f"logit_rules: logits {tuple(logits.shape)}: 1 token at least, 65535 rows at most")
     if torch.is_grad_enabled() and logits.requires_grad:
         raise _lib.DasaError("logit_rules is forward only: call it under torch.no_grad()")
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         raise _lib.DasaError("logit_rules: the rows of logits must be contiguous")
-    d = _lib.LogitRules()
-    d.B, d.V, d.bf16 = B, V, bf16
+    hist = ldh = hlen = nid = 0
     if history is not None:
         if history.dim() != 2 or history.shape[0] != B:
             raise _lib.DasaError(f"logit_rules: history must be [{B}, L], got {tuple(history.shape)}")
-        d.ids_bytes = _ids_bytes(history, "logit_rules.history")
-        d.L = history.shape[1]
-        if d.L and B:
-            history, _, d.ldh = _row_view(history, "logit_rules")
-            d.history = history.data_ptr()
+        nid = _ids_bytes(history, "logit_rules.history")
+        hlen = history.shape[1]
+        if hlen and B:
+            history, _, ldh = _row_view(history, "logit_rules")
+            hist = history.data_ptr()
     if lengths is not None:
-        if history is None or tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+        if history is None or lengths.dim() != 1 or lengths.shape[0] != B or \
+                lengths.dtype not in (torch.int32, torch.int64):
             raise _lib.DasaError(f"logit_rules: lengths must be int32 [{B}] and go with a history")
         lengths = lengths.to(torch.int32).contiguous()
-        d.lengths = lengths.data_ptr()
-    d.repetition, d.repetition0 = _penalty(repetition, B, "repetition", 1.0)
-    d.presence, d.presence0 = _penalty(presence, B, "presence", 0.0)
-    d.frequency, d.frequency0 = _penalty(frequency, B, "frequency", 0.0)
+    r, r0 = _penalty(repetition, B, "repetition", 1.0)
+    p, p0 = _penalty(presence, B, "presence", 0.0)
+    f, f0 = _penalty(frequency, B, "frequency", 0.0)
+    ldb = 0
     if bias is not None:
         if bias.dtype != torch.float32 or tuple(bias.shape) not in ((V,), (B, V)):
             raise _lib.DasaError(f"logit_rules: bias must be float32 [{V}] or [{B}, {V}]")
         bias = bias.contiguous()
-        d.bias, d.ldb = bias.data_ptr(), V if bias.dim() == 2 else 0
+        ldb = V if bias.dim() == 2 else 0
+    bits = byts = None
+    ldw = 0
     if allowed is not None:
         words = allowed.dtype == torch.int32
         n = -(-V // 32) if words else V
@@ -1337,30 +1345,28 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
             raise _lib.DasaError(f"logit_rules: allowed must be bool / uint8 [{V}] or [{B}, {V}], or int32 words "
                                  f"[{-(-V // 32)}] or [{B}, {-(-V // 32)}]")
         allowed = allowed.contiguous()
-        ld = n if allowed.dim() == 2 else 0
-        if words:
-            d.allowed_bits, d.ldbits = allowed.data_ptr(), ld
-        else:
-            d.allowed_bytes, d.ldbytes = allowed.data_ptr(), ld
+        ldw = n if allowed.dim() == 2 else 0
+        bits, byts = (allowed.data_ptr(), None) if words else (None, allowed.data_ptr())
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
-        d.ldo = V
+        out = logits.new_empty((B, V))
+        ldo = V
     else:
-        d.ldo = _out_rows(out, (B, V), logits, "logit_rules")
-    choice = torch.empty(B, dtype=torch.int64, device=logits.device) if want_choice else None
+        ldo = _out_rows(out, (B, V), logits, "logit_rules")
+    choice = logits.new_empty((B,), dtype=torch.int64) if want_choice else None
     if B:
-        d.logits, d.ld = logits.data_ptr(), max(logits.stride(0), V)
-        d.out = out.data_ptr()
         L = _lib.lib()
         ws, nws = None, 0
         if want_choice:
-            d.choice = choice.data_ptr()
             nws = L.dasa_logit_rules_workspace(B, V)
             if nws:
                 ws = torch.empty(nws // 8, dtype=torch.int64, device=logits.device)
+        d = _lib.LogitRules(logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), ldo, hist, ldh,
+                            None if lengths is None else lengths.data_ptr(), r, p, f,
+                            None if bias is None else bias.data_ptr(), ldb, bits, ldw, byts, ldw,
+                            None if choice is None else choice.data_ptr(), r0, p0, f0, B, V, hlen, nid, bf16)
         _call("dasa_logit_rules", "logit_rules", L.dasa_logit_rules, ctypes.byref(d),
-              None if ws is None else ws.data_ptr(), nws, _stream(),
-              nbytes=2.0 * B * V * logits.element_size() + 8.0 * B * d.L)
+              None if ws is None else ws.data_ptr(), nws, _raw_stream(dev),
+              nbytes=2.0 * B * V * logits.element_size() + 8.0 * B * hlen)
     return (out, choice) if want_choice else out
 
 
