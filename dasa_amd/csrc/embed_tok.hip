@@ -176,13 +176,14 @@ __device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lan
 
 // Write the positions of up to 64 tokens of the range (lanes with `in`, in lane order) at their ranks, one distinct
 // id at a time: a frequent id is one turn.
-__device__ __forceinline__ void place(int* cursor, int* order, int lane, bool in, int bin, int pos) {
+template <class O>
+__device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, int bin, int pos) {
   unsigned long long m = __ballot(in);
   while (m) {
     const int b = __builtin_amdgcn_readlane(bin, __builtin_ctzll(m));
     const unsigned long long same = __ballot(in && bin == b);
     const int c = cursor[b];
-    if ((same >> lane) & 1) order[c + __popcll(same & ((1ull << lane) - 1))] = pos;
+    if ((same >> lane) & 1) order[c + __popcll(same & ((1ull << lane) - 1))] = (O)pos;
     cursor[b] = c + __popcll(same);                  // every lane stores the same value
     m &= ~same;
   }
@@ -267,6 +268,19 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
 }
 
 // ------------------------------------------------------------------ gradient rows
+// A lane's unit of a slice. Lanes past the row's end take its first unit and store nothing, so that whole waves reach
+// every lane exchange.
+struct Unit {
+  int col, left;
+  bool live;
+};
+template <class T>
+__device__ __forceinline__ Unit unit_of(int slice, int lane, int E) {
+  const int col = (slice * 64 + lane) * Vec<T>::N;
+  const bool live = col < E;
+  return Unit{live ? col : 0, live ? E - col : E, live};
+}
+
 // A table row of up to kChunk tokens is summed by one wave per slice of 64 units. Longer (hot) rows are cut at the
 // multiples of kChunk in the sorted order, so that a padding or stop word with a tenth of the tokens does not run on
 // one wave: each chunk leaves the sum of its part of at most two hot rows (one that reaches into it, one that reaches
@@ -279,7 +293,7 @@ struct BwdArgs {
   const void* ids; int ids64;
   const int* start;
   const int* order;
-  float* parts;            // [chunks][2][ldp] sums of hot rows' parts, or null (no row can be hot)
+  float* parts;            // [chunks][2][ldp] sums of hot rows' parts
   long ldp;
   void* dtable; long ldt;
   int V, E;
@@ -333,7 +347,7 @@ template <class T>
 __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int col = (blockIdx.y * 64 + lane) * N, left = a.E - col;
+  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
   float acc[N];
 #pragma unroll
@@ -344,10 +358,8 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
     const int s = a.start[v], n = a.start[v + 1] - s;
     if (n > kChunk || (a.accumulate && n == 0)) return;
     const int pos = lane < n ? a.order[s + lane] : 0;
-    if (left > 0) {
-      add_rows<T>(acc, d, a.ldd, left, pos, 0, n);
-      write_row<T>(a, v, col, left, acc);
-    }
+    add_rows<T>(acc, d, a.ldd, left, pos, 0, n);
+    if (live) write_row<T>(a, v, col, left, acc);
     return;
   }
   const long c = (long)(blockIdx.x - a.row_blocks) * 4 + w;
@@ -361,18 +373,20 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   float* part = a.parts + c * 2 * a.ldp + col;
   // the row that owns the chunk's first token, then the row that owns its last
   const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
-  if (ea > 0 && left > 0) {
+  if (ea > 0) {
     add_rows<T>(acc, d, a.ldd, left, pos, 0, ea);
+    if (live)
 #pragma unroll
-    for (int e = 0; e < N; ++e) part[e] = acc[e];
+      for (int e = 0; e < N; ++e) part[e] = acc[e];
   }
   const int sb = __builtin_amdgcn_readlane(hot ? max(rs - j0, 0) : m, m - 1);
-  if (sb > 0 && sb < m && left > 0) {
+  if (sb > 0 && sb < m) {
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
     add_rows<T>(acc, d, a.ldd, left, pos, sb, m - sb);
+    if (live)
 #pragma unroll
-    for (int e = 0; e < N; ++e) part[a.ldp + e] = acc[e];
+      for (int e = 0; e < N; ++e) part[a.ldp + e] = acc[e];
   }
 }
 
@@ -396,7 +410,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   constexpr int N = Vec<T>::N;
   __shared__ float sum[kJoinWaves][64][N];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int col = (blockIdx.y * 64 + lane) * N, left = a.E - col;
+  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
   const int total = a.start[a.V];
   float acc[N];
 #pragma unroll
@@ -406,9 +420,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   if (j0 < total) {
     const long v = id_at(a, a.order[min(j0 + kChunk, (long)total) - 1]);
     const int rs = a.start[v], re = a.start[v + 1], n = (re - 1) / kChunk - (int)c + 1;
-    if (re - rs > kChunk && rs >= j0 && n <= kJoinWaves && left > 0) {
+    if (re - rs > kChunk && rs >= j0 && n <= kJoinWaves) {
       add_parts<T>(acc, a, c, rs > j0, 0, n, col);
-      write_row<T>(a, v, col, left, acc);
+      if (live) write_row<T>(a, v, col, left, acc);
     }
   }
   const long g0 = (long)blockIdx.x * kJoinWaves * kChunk;
@@ -420,15 +434,130 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  if (left > 0) add_parts<T>(acc, a, c0, rs > c0 * kChunk, k0, k1, col);
+  add_parts<T>(acc, a, c0, rs > c0 * kChunk, k0, k1, col);
 #pragma unroll
   for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
   __syncthreads();
-  if (w != 0 || left <= 0) return;
+  if (w != 0 || !live) return;
   for (int k = 1; k < kJoinWaves; ++k)
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
   write_row<T>(a, v, col, left, acc);
+}
+
+// ------------------------------------------------------------------ few tokens: one launch
+// Up to kFewTokens tokens: workgroup = (vocabulary range, slice). It sorts its range's tokens into LDS as above (every
+// token of a wave's segment fits its list) and sums its rows itself: ids of up to kChunk tokens a wave each, the others
+// by all waves, whose parts are joined in order. Three launches become one, and no workspace is needed.
+constexpr int kFewTokens = 8192;
+constexpr int kFewList = kFewTokens / kSortWaves;
+constexpr int kFewRange = 256;
+
+template <class T, class W>
+__global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdArgs a, SortArgs g) {
+  constexpr int N = Vec<T>::N;
+  __shared__ int hist[kSortWaves][kFewRange], first[kFewRange + 1], wsum[kSortWaves], hot[kFewRange], nhot;
+  __shared__ unsigned short lpos[kSortWaves][kFewList], lbin[kSortWaves][kFewList];
+  __shared__ unsigned short order[kFewTokens];
+  const W* ids = reinterpret_cast<const W*>(a.ids);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const unsigned lo = blockIdx.x * (unsigned)g.R, n = min((unsigned)g.R, a.V - lo);
+  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
+  for (int i = tid; i < kSortWaves * kFewRange; i += 64 * kSortWaves) hist[0][i] = 0;
+  if (tid == 0) nhot = 0;
+  __syncthreads();
+  const int seg = (((g.T + kSortWaves - 1) / kSortWaves) + 63) & ~63;
+  const int t0 = min(w * seg, g.T), t1 = min(t0 + seg, g.T);
+  int found = 0;
+  each_token<W, 4>(ids, t0, t1, lane, g.pad, [&](int pos, unsigned u) {
+    const unsigned bin = u - lo;
+    const bool in = bin < n;
+    const unsigned long long m = __ballot(in);
+    if (!m) return;
+    if (in) {
+      const int at = found + __popcll(m & ((1ull << lane) - 1));
+      lpos[w][at] = (unsigned short)pos;
+      lbin[w][at] = (unsigned short)bin;
+      atomicAdd(&hist[w][bin], 1);
+    }
+    found += __popcll(m);
+  });
+  __syncthreads();
+  int tot = 0;
+  if (tid < (int)n)
+    for (int k = 0; k < kSortWaves; ++k) tot += hist[k][tid];
+  int incl = tot;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 63) wsum[w] = incl;
+  __syncthreads();
+  int at = incl - tot;
+  for (int k = 0; k < w; ++k) at += wsum[k];
+  if (tid <= (int)n) first[tid] = at;              // thread n: the total
+  if (tid < (int)n) {
+    for (int k = 0; k < kSortWaves; ++k) {
+      const int c = hist[k][tid];
+      hist[k][tid] = at;
+      at += c;
+    }
+    if (tot > kChunk) hot[atomicAdd(&nhot, 1)] = tid;
+  }
+  __syncthreads();
+  for (int i = 0; i < found; i += 64) {
+    const int j = min(i + lane, found - 1);
+    place(hist[w], order, lane, i + lane < found, lbin[w][j], lpos[w][j]);
+  }
+  __syncthreads();
+  const T* d = reinterpret_cast<const T*>(a.dout) + col;
+  float acc[N];
+  for (int r = w; r < (int)n; r += kSortWaves) {
+    const int s = first[r], c = first[r + 1] - s;
+    if (c > kChunk || (a.accumulate && c == 0)) continue;
+    const int pos = lane < c ? order[s + lane] : 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    add_rows<T>(acc, d, a.ldd, left, pos, 0, c);
+    if (live) write_row<T>(a, lo + r, col, left, acc);
+  }
+  const int h = nhot;
+  if (h == 0) return;
+  __shared__ float sum[kSortWaves][64][N];
+  for (int i = 0; i < h; ++i) {
+    const int r = hot[i], s = first[r], c = first[r + 1] - s;
+    const int per = (c + kSortWaves - 1) / kSortWaves, k0 = min(w * per, c), k1 = min(k0 + per, c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    for (int k = k0; k < k1; k += 64) {
+      const int pos = order[s + min(k + lane, k1 - 1)];
+      add_rows<T>(acc, d, a.ldd, left, pos, 0, min(64, k1 - k));
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
+    __syncthreads();
+    if (w == 0 && live) {
+      for (int k = 1; k < kSortWaves; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
+      write_row<T>(a, lo + r, col, left, acc);
+    }
+    __syncthreads();
+  }
+}
+
+template <class T>
+int launch_few(const BwdArgs& a, SortArgs g, hipStream_t st) {
+  const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
+  int G = (a.V + kFewRange - 1) / kFewRange;
+  if (G < 256) G = a.V < 256 ? a.V : 256;
+  g.R = (a.V + G - 1) / G;
+  const dim3 grid((a.V + g.R - 1) / g.R, slices), block(64 * kSortWaves);
+  if (a.ids64) hipLaunchKernelGGL((embedding_bwd_few_kernel<T, uint2>), grid, block, 0, st, a, g);
+  else hipLaunchKernelGGL((embedding_bwd_few_kernel<T, unsigned>), grid, block, 0, st, a, g);
+  DASA_CHECK_LAUNCH();
+  return 0;
 }
 
 inline long part_stride(int E, int bf16) {      // whole units, so a partial unit's sums stay inside
@@ -440,15 +569,13 @@ template <class T>
 int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   a.row_blocks = (unsigned)((a.V + 3) / 4);
-  const long chunks = a.parts ? (tokens + kChunk - 1) / kChunk : 0;
+  const long chunks = (tokens + kChunk - 1) / kChunk;
   const dim3 grid(a.row_blocks + (unsigned)((chunks + 3) / 4), slices);
   hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
-  if (chunks) {
-    hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
-                       dim3(64 * kJoinWaves), 0, st, a);
-    DASA_CHECK_LAUNCH();
-  }
+  hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
+                     dim3(64 * kJoinWaves), 0, st, a);
+  DASA_CHECK_LAUNCH();
   return 0;
 }
 
@@ -469,8 +596,8 @@ extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* id
 }
 
 extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E) {
-  if (T < 0 || T >= (1LL << 31) || V < 0 || E < 0) return 0;
-  const int64_t chunks = T > kChunk ? (T + kChunk - 1) / kChunk : 0;
+  if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0) return 0;
+  const int64_t chunks = (T + kChunk - 1) / kChunk;
   return round16(((int64_t)V + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4;
 }
 
@@ -480,27 +607,28 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   if (T < 0 || T >= (1LL << 31) - 65536 || V < 0 || E < 0 || (ids_bytes != 4 && ids_bytes != 8))
     return (int)hipErrorInvalidValue;
   if (V == 0 || E == 0) return 0;
-  if (!dtable || ldt < E || !ws || ws_bytes < dasa_embedding_bwd_workspace(T, V, E)) return (int)hipErrorInvalidValue;
+  if (!dtable || ldt < E || ws_bytes < dasa_embedding_bwd_workspace(T, V, E) || (T > kFewTokens && !ws))
+    return (int)hipErrorInvalidValue;
   if (T > 0 && (!ids || !dout || ldd < E)) return (int)hipErrorInvalidValue;
-  int* start = reinterpret_cast<int*>(ws);
-  int* order = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + round16(((int64_t)V + 1) * 4));
   hipStream_t st = (hipStream_t)stream;
-  int G = (V + kMaxRange - 1) / kMaxRange;
-  if (G < 256) G = V < 256 ? V : 256;
-  const int R = (V + G - 1) / G;
-  G = (V + R - 1) / R;
-  SortArgs sa{ids, (int)T, V, R, padding_idx < 0 ? ~0u : (unsigned)padding_idx, start, order};
-  const size_t lds = (size_t)kSortWaves * R * sizeof(int);
-  if (ids_bytes == 8)
-    hipLaunchKernelGGL(token_sort_kernel<uint2>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
-  else
-    hipLaunchKernelGGL(token_sort_kernel<unsigned>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
-  DASA_CHECK_LAUNCH();
   BwdArgs ba{};
   ba.dout = dout; ba.ldd = (long)ldd; ba.ids = ids; ba.ids64 = ids_bytes == 8;
-  ba.start = start; ba.order = order;
-  if (T > kChunk) ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
-  ba.ldp = part_stride(E, bf16);
   ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.scale = scale; ba.accumulate = accumulate;
+  SortArgs sa{ids, (int)T, V, 0, padding_idx < 0 ? ~0u : (unsigned)padding_idx, nullptr, nullptr};
+  if (T <= kFewTokens) return bf16 ? launch_few<__bf16>(ba, sa, st) : launch_few<float>(ba, sa, st);
+  int* start = reinterpret_cast<int*>(ws);
+  int* order = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + round16(((int64_t)V + 1) * 4));
+  ba.start = sa.start = start;
+  ba.order = sa.order = order;
+  ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
+  ba.ldp = part_stride(E, bf16);
+  int G = (V + kMaxRange - 1) / kMaxRange;
+  if (G < 256) G = V < 256 ? V : 256;
+  sa.R = (V + G - 1) / G;
+  G = (V + sa.R - 1) / sa.R;
+  const size_t lds = (size_t)kSortWaves * sa.R * sizeof(int);
+  if (ids_bytes == 8) hipLaunchKernelGGL(token_sort_kernel<uint2>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
+  else hipLaunchKernelGGL(token_sort_kernel<unsigned>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
+  DASA_CHECK_LAUNCH();
   return bf16 ? launch_rows<__bf16>(ba, T, st) : launch_rows<float>(ba, T, st);
 }

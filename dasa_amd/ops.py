@@ -1153,10 +1153,11 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     d, T, ldd = _row_view(dout, "embedding_bwd")
     ids = ids.contiguous()
     L = _lib.lib()
-    ws = torch.empty(L.dasa_embedding_bwd_workspace(T, vocab, E), dtype=torch.uint8, device=dout.device)
+    nws = L.dasa_embedding_bwd_workspace(T, vocab, E)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dout.device) if nws else None
     _call("dasa_embedding_bwd", "embed_bwd", L.dasa_embedding_bwd, d.data_ptr(), ldd, ids.data_ptr(), nb, T, vocab, E,
-          float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
-          _raw_stream(dev), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
+          float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0,
+          None if ws is None else ws.data_ptr(), nws, _raw_stream(dev), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
     return out
 
 

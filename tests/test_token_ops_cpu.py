@@ -78,11 +78,13 @@ def test_entry_points_refuse_before_a_launch():
                                   (4, 10, 8, 8, 8, 7), (4, -1, 8, 8, 8, 8)):
         assert L.dasa_embedding_fwd(P, ldt, P, nb, T, V, E, 1.0, 0, P, ldo, None, None) == INVALID
     assert L.dasa_embedding_fwd(None, 8, P, 8, 4, 10, 8, 1.0, 0, P, 8, None, None) == INVALID
-    need = L.dasa_embedding_bwd_workspace(100, 50, 8)
-    assert need >= 4 * 151 and L.dasa_embedding_bwd_workspace(2**31, 50, 8) == 0
-    for T, nb, ldd, ldt, ws, n in ((2**31, 8, 8, 8, P, need), (100, 1, 8, 8, P, need), (100, 8, 7, 8, P, need),
-                                   (100, 8, 8, 7, P, need), (100, 8, 8, 8, None, need), (100, 8, 8, 8, P, need - 1),
-                                   (-1, 8, 8, 8, P, need)):
+    assert L.dasa_embedding_bwd_workspace(2**31, 50, 8) == 0 and L.dasa_embedding_bwd_workspace(100, 50, 8) == 0
+    T0 = 100000
+    need = L.dasa_embedding_bwd_workspace(T0, 50, 8)
+    assert need >= 4 * (T0 + 51)
+    for T, nb, ldd, ldt, ws, n in ((2**31, 8, 8, 8, P, need), (T0, 1, 8, 8, P, need), (T0, 8, 7, 8, P, need),
+                                   (T0, 8, 8, 7, P, need), (T0, 8, 8, 8, None, need), (T0, 8, 8, 8, P, need - 1),
+                                   (-1, 8, 8, 8, P, need), (100, 8, 7, 8, None, 0), (100, 8, 8, 7, None, 0)):
         assert L.dasa_embedding_bwd(P, ldd, P, nb, T, 50, 8, 1.0, -1, 0, P, ldt, 0, ws, n, None) == INVALID
     assert L.dasa_w4_weight_bytes(17, 129) == 2 * 2 * 1024 and L.dasa_w4_weight_bytes(0, 4) == 0
     assert L.dasa_w4_scale_count(17, 129, 64) == 2 * 2 * 2 * 16 and L.dasa_w4_scale_count(17, 129, 16) == 0
