@@ -450,23 +450,27 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
 // token of a wave's segment fits its list) and sums its rows itself: ids of up to kChunk tokens a wave each, the others
 // by all waves, whose parts are joined in order. Three launches become one, and no workspace is needed.
 constexpr int kFewTokens = 8192;
-constexpr int kFewList = kFewTokens / kSortWaves;
+constexpr int kFewWaves = 8;
 constexpr int kFewRange = 256;
 
+inline int few_segment(int T) { return (((T + kFewWaves - 1) / kFewWaves) + 63) & ~63; }
+
 template <class T, class W>
-__global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdArgs a, SortArgs g) {
+__global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(BwdArgs a, SortArgs g, int seg) {
   constexpr int N = Vec<T>::N;
-  __shared__ int hist[kSortWaves][kFewRange], first[kFewRange + 1], wsum[kSortWaves], hot[kFewRange], nhot;
-  __shared__ unsigned short lpos[kSortWaves][kFewList], lbin[kSortWaves][kFewList];
-  __shared__ unsigned short order[kFewTokens];
+  __shared__ int hist[kFewWaves][kFewRange], first[kFewRange + 1], wsum[kFewWaves], hot[kFewRange], nhot;
+  // the sorted positions [waves seg]; the waves' tokens [waves][seg] as positions and ids, later the hot rows' sums
+  extern __shared__ __attribute__((aligned(16))) unsigned short order[];
+  unsigned short* const lpos = order + kFewWaves * seg;
+  unsigned short* const lbin = lpos + kFewWaves * seg;
+  float* const sum = reinterpret_cast<float*>(lpos);       // [waves][64][N]
   const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const unsigned lo = blockIdx.x * (unsigned)g.R, n = min((unsigned)g.R, a.V - lo);
   const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
-  for (int i = tid; i < kSortWaves * kFewRange; i += 64 * kSortWaves) hist[0][i] = 0;
+  for (int i = tid; i < kFewWaves * kFewRange; i += 64 * kFewWaves) hist[0][i] = 0;
   if (tid == 0) nhot = 0;
   __syncthreads();
-  const int seg = (((g.T + kSortWaves - 1) / kSortWaves) + 63) & ~63;
   const int t0 = min(w * seg, g.T), t1 = min(t0 + seg, g.T);
   int found = 0;
   each_token<W, 4>(ids, t0, t1, lane, g.pad, [&](int pos, unsigned u) {
@@ -476,8 +480,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
     if (!m) return;
     if (in) {
       const int at = found + __popcll(m & ((1ull << lane) - 1));
-      lpos[w][at] = (unsigned short)pos;
-      lbin[w][at] = (unsigned short)bin;
+      lpos[w * seg + at] = (unsigned short)pos;
+      lbin[w * seg + at] = (unsigned short)bin;
       atomicAdd(&hist[w][bin], 1);
     }
     found += __popcll(m);
@@ -485,7 +489,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
   __syncthreads();
   int tot = 0;
   if (tid < (int)n)
-    for (int k = 0; k < kSortWaves; ++k) tot += hist[k][tid];
+    for (int k = 0; k < kFewWaves; ++k) tot += hist[k][tid];
   int incl = tot;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -498,7 +502,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
   for (int k = 0; k < w; ++k) at += wsum[k];
   if (tid <= (int)n) first[tid] = at;              // thread n: the total
   if (tid < (int)n) {
-    for (int k = 0; k < kSortWaves; ++k) {
+    for (int k = 0; k < kFewWaves; ++k) {
       const int c = hist[k][tid];
       hist[k][tid] = at;
       at += c;
@@ -508,12 +512,12 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
   __syncthreads();
   for (int i = 0; i < found; i += 64) {
     const int j = min(i + lane, found - 1);
-    place(hist[w], order, lane, i + lane < found, lbin[w][j], lpos[w][j]);
+    place(hist[w], order, lane, i + lane < found, lbin[w * seg + j], lpos[w * seg + j]);
   }
   __syncthreads();
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
   float acc[N];
-  for (int r = w; r < (int)n; r += kSortWaves) {
+  for (int r = w; r < (int)n; r += kFewWaves) {
     const int s = first[r], c = first[r + 1] - s;
     if (c > kChunk || (a.accumulate && c == 0)) continue;
     const int pos = lane < c ? order[s + lane] : 0;
@@ -524,10 +528,9 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
   }
   const int h = nhot;
   if (h == 0) return;
-  __shared__ float sum[kSortWaves][64][N];
   for (int i = 0; i < h; ++i) {
     const int r = hot[i], s = first[r], c = first[r + 1] - s;
-    const int per = (c + kSortWaves - 1) / kSortWaves, k0 = min(w * per, c), k1 = min(k0 + per, c);
+    const int per = (c + kFewWaves - 1) / kFewWaves, k0 = min(w * per, c), k1 = min(k0 + per, c);
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
     for (int k = k0; k < k1; k += 64) {
@@ -535,12 +538,12 @@ __global__ __launch_bounds__(64 * kSortWaves) void embedding_bwd_few_kernel(BwdA
       add_rows<T>(acc, d, a.ldd, left, pos, 0, min(64, k1 - k));
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
+    for (int e = 0; e < N; ++e) sum[(w * 64 + lane) * N + e] = acc[e];
     __syncthreads();
     if (w == 0 && live) {
-      for (int k = 1; k < kSortWaves; ++k)
+      for (int k = 1; k < kFewWaves; ++k)
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
+        for (int e = 0; e < N; ++e) acc[e] += sum[(k * 64 + lane) * N + e];
       write_row<T>(a, lo + r, col, left, acc);
     }
     __syncthreads();
@@ -553,9 +556,12 @@ int launch_few(const BwdArgs& a, SortArgs g, hipStream_t st) {
   int G = (a.V + kFewRange - 1) / kFewRange;
   if (G < 256) G = a.V < 256 ? a.V : 256;
   g.R = (a.V + G - 1) / G;
-  const dim3 grid((a.V + g.R - 1) / g.R, slices), block(64 * kSortWaves);
-  if (a.ids64) hipLaunchKernelGGL((embedding_bwd_few_kernel<T, uint2>), grid, block, 0, st, a, g);
-  else hipLaunchKernelGGL((embedding_bwd_few_kernel<T, unsigned>), grid, block, 0, st, a, g);
+  const int seg = few_segment(g.T);
+  const size_t lists = (size_t)kFewWaves * seg * 4, sums = (size_t)kFewWaves * 64 * Vec<T>::N * 4;
+  const size_t lds = (size_t)kFewWaves * seg * 2 + (lists > sums ? lists : sums);
+  const dim3 grid((a.V + g.R - 1) / g.R, slices), block(64 * kFewWaves);
+  if (a.ids64) hipLaunchKernelGGL((embedding_bwd_few_kernel<T, uint2>), grid, block, lds, st, a, g, seg);
+  else hipLaunchKernelGGL((embedding_bwd_few_kernel<T, unsigned>), grid, block, lds, st, a, g, seg);
   DASA_CHECK_LAUNCH();
   return 0;
 }

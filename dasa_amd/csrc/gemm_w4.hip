@@ -53,21 +53,25 @@ struct LayoutArgs {
   int N, K, Kb, N16, g;
 };
 
-// One thread per 32-bit word of the tiled weights; the first threads of a block also place its scales.
+// One thread per 32-bit word (eight codes of a row, which keep their order: code ^ 8 is the stored nibble); the first
+// threads of a block also place its scales.
 template <class S>
 __global__ __launch_bounds__(256) void w4_layout_kernel(LayoutArgs a) {
+  typedef unsigned u32u __attribute__((aligned(1)));
   const long blk = blockIdx.x;                        // (column block, K block)
   const int nt = (int)(blk / a.Kb), kb = (int)(blk % a.Kb);
-  const int tid = threadIdx.x, l = tid >> 2, j = tid & 3;
-  const int n = nt * 16 + (l & 15), k = kb * 128 + j * 32 + (l >> 4) * 8;
+  const int tid = threadIdx.x, c = tid >> 4, unit = tid & 15;      // a row's 64 B are read by 16 threads in a row
+  const int n = nt * 16 + c, k = kb * 128 + unit * 8;
   unsigned word = 0;                                  // two's complement 0: padding adds nothing
   if (n < a.N) {
-    for (int i = 0; i < 8 && k + i < a.K; ++i) {
-      const unsigned c = (a.codes[(long)n * a.ldc + ((k + i) >> 1)] >> (4 * ((k + i) & 1))) & 15u;
-      word |= (c ^ 8u) << (4 * i);
+    const unsigned char* p = a.codes + (long)n * a.ldc + (k >> 1);
+    if (k + 8 <= a.K) {
+      word = *reinterpret_cast<const u32u*>(p) ^ 0x88888888u;
+    } else {
+      for (int i = 0; i < 8 && k + i < a.K; ++i) word |= (((p[i >> 1] >> (4 * (i & 1))) & 15u) ^ 8u) << (4 * i);
     }
   }
-  a.w[blk * 256 + tid] = word;
+  a.w[blk * 256 + ((unit & 3) * 16 + c) * 4 + (unit >> 2)] = word;
   const int gpb = 128 / a.g, groups = (a.K + a.g - 1) / a.g;
   if (tid < gpb * 16) {
     const int nn = nt * 16 + tid / gpb, gi = kb * gpb + tid % gpb;
