@@ -8,9 +8,10 @@
 // Every product, quotient and sum is one rounded fp32 operation in this order (no contraction), so the result does
 // not depend on how a row is split over workgroups.
 //
-// A workgroup owns one row's slice of kSlice tokens: it counts the row's history into LDS (integer atomics: the
-// counts do not depend on their order), then streams the slice once. With one slice a row, the workgroup also makes
-// the choice; else each slice leaves its best key and one wave a row takes the best of them.
+// A workgroup owns a slice of one row, 4 ITER tokens a thread: it asks for its logits, biases and mask words first,
+// counts the row's history into LDS while they come (integer atomics: the counts do not depend on their order), and
+// writes the slice. With one slice a row, the workgroup also makes the choice; else each slice leaves its best key
+// and a second launch takes the best of them, one wave a row.
 #include "common.h"
 #include "../../include/dasa_hip.h"
 
@@ -19,6 +20,7 @@ namespace {
 // 16 B of a row whose start need not be aligned (an odd vocabulary): element-aligned vector accesses
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 b4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32u __attribute__((aligned(1)));
 template <class T> struct V4;
 template <> struct V4<float> { typedef f4u type; };
 template <> struct V4<__bf16> { typedef b4u type; };
@@ -35,7 +37,7 @@ struct RulesArgs {
   const unsigned char* bytes; long ldbytes;
   int64_t* choice;
   unsigned long long* best;    // [B][slices] keys when a row has several slices
-  int V, slices, slice;
+  int V, slices;
 };
 
 // Order-preserving key of a value and its index: larger value first, NaN above all, -0 = +0, then the lower index.
@@ -59,83 +61,114 @@ __device__ __forceinline__ unsigned long long wave_best(unsigned long long k) {
   return k;
 }
 
-template <class T, class I>
+template <class T, class I, int ITER>
 __global__ __launch_bounds__(1024) void logit_rules_kernel(RulesArgs a) {
 #pragma clang fp contract(off)
   typedef typename V4<T>::type V;
-  extern __shared__ int count[];        // [slice] when there is a history
+  extern __shared__ int count[];        // [4 ITER threads] when there is a history
   __shared__ unsigned long long wbest[16];
-  const int b = blockIdx.y, lo = blockIdx.x * a.slice, n = min(a.slice, a.V - lo);
-  const int tid = threadIdx.x, lane = tid & 63, nt = blockDim.x;
-  if (a.history) {
-    for (int i = tid; i < a.slice; i += nt) count[i] = 0;
-    __syncthreads();
-    const I* h = reinterpret_cast<const I*>(a.history) + (long)b * a.ldh;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.L) : a.L;
-    for (int i = tid; i < len; i += nt) {
-      const long v = (long)h[i] - lo;
-      if (v >= 0 && v < n) atomicAdd(&count[v], 1);
-    }
-    __syncthreads();
-  }
-  const float r = a.rep ? a.rep[b] : a.rep0, p = a.pres ? a.pres[b] : a.pres0, f = a.freq ? a.freq[b] : a.freq0;
+  const int tid = threadIdx.x, lane = tid & 63, nt = blockDim.x, slice = 4 * ITER * nt;
+  const int b = blockIdx.y, lo = blockIdx.x * slice, n = min(slice, a.V - lo);
   const T* x0 = reinterpret_cast<const T*>(a.logits) + (long)b * a.ld + lo;
   T* y0 = reinterpret_cast<T*>(a.out) + (long)b * a.ldo + lo;
   const float* bias = a.bias ? a.bias + (long)b * a.ldb + lo : nullptr;
-  const unsigned* bits = a.bits ? a.bits + (long)b * a.ldbits : nullptr;
+  const unsigned* bits = a.bits ? a.bits + (long)b * a.ldbits + (lo >> 5) : nullptr;     // lo % 32 == 0
   const unsigned char* bytes = a.bytes ? a.bytes + (long)b * a.ldbytes + lo : nullptr;
-  unsigned long long best = 0;
-  auto rule = [&](float x, int c, float add, bool open) {
-    if (c > 0) {
-      x = x > 0.f ? x / r : x * r;
-      x = x - f * (float)c;
-      x = x - p;
-    }
-    if (bias) x = x + add;
-    return (T)(open ? x : -INFINITY);
-  };
-  for (int i = 4 * tid; i < n; i += 4 * nt) {
-    unsigned open = 15u;                 // lo and i are multiples of 4: the four bits share a word
-    if (bits) open = (bits[(lo + i) >> 5] >> ((lo + i) & 31)) & 15u;
+  V x[ITER];
+  f4u add[ITER];
+  unsigned open[ITER];                  // the four tokens' bits
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int i = 4 * (tid + k * nt);
+    add[k] = f4u{0.f, 0.f, 0.f, 0.f};
+    open[k] = 15u;
     if (i + 4 <= n) {
-      V x = *reinterpret_cast<const V*>(x0 + i);
-      f4u add = {0.f, 0.f, 0.f, 0.f};
-      if (bias) add = *reinterpret_cast<const f4u*>(bias + i);
-      int4 c = make_int4(0, 0, 0, 0);
-      if (a.history) c = *reinterpret_cast<const int4*>(count + i);
-      const int cc[4] = {c.x, c.y, c.z, c.w};
+      x[k] = *reinterpret_cast<const V*>(x0 + i);
+      if (bias) add[k] = *reinterpret_cast<const f4u*>(bias + i);
+      if (bits) open[k] = bits[i >> 5] >> (i & 31);
+      if (bytes) open[k] = *reinterpret_cast<const u32u*>(bytes + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[k][e] = i + e < n ? x0[i + e] : (T)0.f;
+      if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) add[k][e] = i + e < n ? bias[i + e] : 0.f;
+      if (bits && i < n) open[k] = bits[i >> 5] >> (i & 31);
+      if (bytes) {
+        open[k] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) open[k] |= i + e < n ? (unsigned)bytes[i + e] << (8 * e) : 0u;
+      }
+    }
+  }
+  const float r = a.rep ? a.rep[b] : a.rep0, p = a.pres ? a.pres[b] : a.pres0, f = a.freq ? a.freq[b] : a.freq0;
+  if (a.history) {
+    const I* h = reinterpret_cast<const I*>(a.history) + (long)b * a.ldh;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.L) : a.L;
+    constexpr int U = 8;                // ids in flight
+    long id[U];
+    auto ask = [&](int at) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = at + k * nt + tid;
+        id[k] = i < len ? (long)h[i] - lo : -1;
+      }
+    };
+    ask(0);
+#pragma unroll
+    for (int k = 0; k < ITER; ++k) *reinterpret_cast<int4*>(count + 4 * (tid + k * nt)) = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    for (int at = 0; at < len;) {
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (id[k] >= 0 && id[k] < n) atomicAdd(&count[id[k]], 1);
+      at += U * nt;
+      if (at < len) ask(at);
+    }
+    __syncthreads();
+  }
+  unsigned long long best = 0;
+#pragma unroll
+  for (int k = 0; k < ITER; ++k) {
+    const int i = 4 * (tid + k * nt);
+    int4 c = make_int4(0, 0, 0, 0);
+    if (a.history) c = *reinterpret_cast<const int4*>(count + i);
+    const int cc[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = (float)x[k][e];
+      if (cc[e] > 0) {
+        v = v > 0.f ? v / r : v * r;
+        v = v - f * (float)cc[e];
+        v = v - p;
+      }
+      if (bias) v = v + add[k][e];
+      const bool o = bytes ? (open[k] >> (8 * e)) & 255u : (open[k] >> e) & 1u;
+      x[k][e] = (T)(o ? v : -INFINITY);
+    }
+    if (i + 4 <= n) {
+      *reinterpret_cast<V*>(y0 + i) = x[k];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < n) y0[i + e] = x[k][e];
+    }
+    if (a.choice)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (bytes && !bytes[i + e]) open &= ~(1u << e);
-        x[e] = rule((float)x[e], cc[e], add[e], (open >> e) & 1);
+        const unsigned long long key = i + e < n ? choice_key((float)x[k][e], lo + i + e) : 0;
+        best = key > best ? key : best;
       }
-      *reinterpret_cast<V*>(y0 + i) = x;
-      if (a.choice) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned long long k = choice_key((float)x[e], lo + i + e);
-          best = k > best ? k : best;
-        }
-      }
-    } else {
-      for (int e = 0; i + e < n; ++e) {
-        const bool o = ((open >> e) & 1) && (!bytes || bytes[i + e]);
-        const T y = rule((float)x0[i + e], a.history ? count[i + e] : 0, bias ? bias[i + e] : 0.f, o);
-        y0[i + e] = y;
-        const unsigned long long k = choice_key((float)y, lo + i + e);
-        best = k > best ? k : best;
-      }
-    }
   }
   if (!a.choice) return;
   best = wave_best(best);
   if (lane == 0) wbest[tid >> 6] = best;
   __syncthreads();
-  if (tid == 0) {
-    for (int k = 1; k < nt / 64; ++k) best = wbest[k] > best ? wbest[k] : best;
-    if (a.slices == 1) a.choice[b] = (int64_t)(unsigned)~(unsigned)best;
-    else a.best[(long)b * a.slices + blockIdx.x] = best;
-  }
+  if (tid >= 64) return;
+  best = wave_best(lane < nt / 64 ? wbest[lane] : 0);
+  if (tid != 0) return;
+  if (a.slices == 1) a.choice[b] = (int64_t)(unsigned)~(unsigned)best;
+  else a.best[(long)b * a.slices + blockIdx.x] = best;
 }
 
 // The best of one row's slices: one wave a row.
@@ -149,15 +182,35 @@ __global__ __launch_bounds__(64) void logit_choice_kernel(const unsigned long lo
   if (threadIdx.x == 0) choice[blockIdx.x] = (int64_t)(unsigned)~(unsigned)k;
 }
 
-constexpr int kSlice = 8192;     // tokens of one workgroup: 32 KB of counts
+struct Shape {
+  int iter, threads, slices;
+};
 
-inline int slices_of(int B, int V) { (void)B; return (V + kSlice - 1) / kSlice; }
+// One slice a row up to 8192 tokens (4 or 8 a thread). Else slices of 8 tokens a thread, as wide as still gives every
+// CU a workgroup (each reads the whole history).
+inline Shape shape_of(int B, int V) {
+  auto threads = [&](int iter) { return (V + 256 * iter - 1) / (256 * iter) * 64; };
+  if (V <= 4096) return {1, threads(1), 1};
+  if (V <= 8192) return {2, threads(2), 1};
+  for (int nt = 1024;; nt /= 2) {
+    const int s = (V + 8 * nt - 1) / (8 * nt);
+    if ((long)B * s >= 256 || nt == 256) return {2, nt, s};
+  }
+}
+
+template <class T, class I>
+void launch(const RulesArgs& a, const Shape& s, int B, hipStream_t st) {
+  const size_t lds = a.history ? (size_t)4 * s.iter * s.threads * sizeof(int) : 0;
+  const dim3 grid(s.slices, B), block(s.threads);
+  if (s.iter == 1) hipLaunchKernelGGL((logit_rules_kernel<T, I, 1>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((logit_rules_kernel<T, I, 2>), grid, block, lds, st, a);
+}
 
 }  // namespace
 
 extern "C" int64_t dasa_logit_rules_workspace(int32_t B, int32_t V) {
   if (B <= 0 || V <= 0) return 0;
-  const int s = slices_of(B, V);
+  const int s = shape_of(B, V).slices;
   return s > 1 ? (int64_t)B * s * 8 : 0;
 }
 
@@ -171,7 +224,8 @@ extern "C" int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_
       (d->allowed_bits && d->ldbits != 0 && d->ldbits < (d->V + 31) / 32) ||
       (d->allowed_bytes && d->ldbytes != 0 && d->ldbytes < d->V))
     return (int)hipErrorInvalidValue;
-  const int slices = slices_of(d->B, d->V);
+  const Shape sh = shape_of(d->B, d->V);
+  const int slices = sh.slices;
   if (d->choice && slices > 1 && (!ws || ws_bytes < dasa_logit_rules_workspace(d->B, d->V)))
     return (int)hipErrorInvalidValue;
   RulesArgs a{};
@@ -183,21 +237,10 @@ extern "C" int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_
   a.bits = d->allowed_bits; a.ldbits = d->ldbits; a.bytes = d->allowed_bytes; a.ldbytes = d->ldbytes;
   a.choice = d->choice; a.best = reinterpret_cast<unsigned long long*>(ws);
   a.V = d->V; a.slices = slices;
-  a.slice = slices > 1 ? kSlice : ((d->V + 3) & ~3);
-  const int work = d->V < a.slice ? d->V : a.slice;
-  int nt = (((work + 3) / 4 + 63) / 64) * 64;
-  if (a.history && nt < 256) nt = 256;
-  if (nt > 1024) nt = 1024;
-  const size_t lds = a.history ? (size_t)a.slice * sizeof(int) : 0;
-  const dim3 grid(slices, d->B), block(nt);
   hipStream_t st = (hipStream_t)stream;
-  if (d->bf16) {
-    if (d->ids_bytes == 4) hipLaunchKernelGGL((logit_rules_kernel<__bf16, int32_t>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((logit_rules_kernel<__bf16, int64_t>), grid, block, lds, st, a);
-  } else {
-    if (d->ids_bytes == 4) hipLaunchKernelGGL((logit_rules_kernel<float, int32_t>), grid, block, lds, st, a);
-    else hipLaunchKernelGGL((logit_rules_kernel<float, int64_t>), grid, block, lds, st, a);
-  }
+  const bool narrow = d->ids_bytes == 4;
+  if (d->bf16) narrow ? launch<__bf16, int32_t>(a, sh, d->B, st) : launch<__bf16, int64_t>(a, sh, d->B, st);
+  else narrow ? launch<float, int32_t>(a, sh, d->B, st) : launch<float, int64_t>(a, sh, d->B, st);
   DASA_CHECK_LAUNCH();
   if (d->choice && slices > 1) {
     hipLaunchKernelGGL(logit_choice_kernel, dim3(d->B), dim3(64), 0, st, a.best, a.choice, slices);
