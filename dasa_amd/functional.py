@@ -903,3 +903,46 @@ def embedding(ids, table, scale=1.0, padding_idx=None):
     if torch.is_grad_enabled() and table.requires_grad:
         return EmbeddingFn.apply(ids, table, scale, padding_idx)
     return ops.embedding(ids, table, scale=scale)
+
+
+class BertEmbedFn(torch.autograd.Function):
+    """BertEmbeddings (vilmodel.py:161-176) with gradients: dropout(LayerNorm(word[ids] + pos[t] + type[0])). The forward is
+    ops.bert_embed, unchanged; the backward recomputes the summed rows and their statistics instead of keeping them
+    ([B, L, H] per call), takes LayerNorm's and sends each row to its word, its position and type 0 by sorted tokens."""
+
+    @staticmethod
+    def forward(ctx, ids, word, pos, types, gamma, beta, eps, p, seed, padding_idx):
+        ctx.eps, ctx.p, ctx.seed, ctx.pad = eps, p, seed, padding_idx
+        ctx.save_for_backward(ids)
+        ctx.params = _Kept((word, pos, types, gamma, beta))
+        return ops.bert_embed(ids, word, pos, types[0], gamma, beta, eps, p, seed)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        word, pos, types, gamma, beta = ctx.params
+        n = ctx.needs_input_grad
+        dy = dy.contiguous()
+        if ctx.p > 0:
+            dy = ops.dropout(dy, ctx.p, ctx.seed)
+        B, L = ids.shape
+        places = torch.arange(L, device=ids.device).expand(B, L).contiguous()
+        zeros = torch.zeros_like(places)
+        x = ops.add2d(ops.embedding(ids, word), ops.embedding(places, pos))      # the forward's order of sums
+        x = ops.add2d(x, ops.embedding(zeros, types))
+        _, saved = ops.layernorm(x, gamma, beta, ctx.eps, save=True)
+        dgamma, dbeta = torch.zeros_like(gamma), torch.zeros_like(beta)
+        dx = ops.layernorm_bwd(dy, saved, gamma, dgamma, dbeta)
+        dword = ops.embedding_bwd(dx, ids, word.shape[0], padding_idx=ctx.pad) if n[1] else None
+        dpos = ops.embedding_bwd(dx, places, pos.shape[0]) if n[2] else None
+        dtypes = ops.embedding_bwd(dx, zeros, types.shape[0]) if n[3] else None
+        return None, dword, dpos, dtypes, dgamma if n[4] else None, dbeta if n[5] else None, None, None, None, None
+
+
+def bert_embed(ids, word, pos, types, gamma, beta, eps, p=0.0, training=False, padding_idx=None):
+    """BertEmbeddings with gradients for its three tables and its LayerNorm (types: the whole token-type table)."""
+    seed = new_seed() if (training and p > 0) else 0
+    p = p if training else 0.0
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (word, pos, types, gamma, beta)):
+        return BertEmbedFn.apply(ids, word, pos, types, gamma, beta, eps, p, seed, padding_idx)
+    return ops.bert_embed(ids, word, pos, types[0], gamma, beta, eps, p, seed)

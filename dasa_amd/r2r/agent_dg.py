@@ -291,6 +291,7 @@ class Seq2SeqAgent(BaseAgent):
         self.encoder.drop = nn.Dropout(p=args.d_dropout_ratio)
         self.encoder.bert.update_lang_bert = self.encoder.bert.config.update_lang_bert = args.d_transformer_update
         self.encoder.bert.update_add_layer = self.encoder.bert.config.update_add_layer = args.d_update_add_layer
+        self.encoder.bert.embeddings.trained = self.encoder.bert.config.update_embeddings = args.d_update_embeddings
 
     # ------------------------------------------------------------------ observation -> tensors
     def _sort_batch(self, obs):

@@ -11,6 +11,7 @@ import torch.nn as nn
 
 from .. import functional as DF
 from .. import ops
+from .._lib import DasaError
 from .param import args
 
 
@@ -236,6 +237,37 @@ class SpeakerDecoder(nn.Module):
         self.projection = nn.Linear(hidden_size, vocab_size)
         self.baseline_projection = nn.Sequential(nn.Linear(hidden_size, 128), nn.ReLU(), nn.Dropout(dropout_ratio),
                                                  nn.Linear(128, 1))
+        self._w4 = {}      # quantize_w4(): 4-bit forms of the word step's linears
+
+    def _word_linears(self):
+        """The weights of a word step's linears, by the name their 4-bit forms are kept under."""
+        att = self.attention_layer
+        return {"ih": self.lstm.weight_ih_l0, "hh": self.lstm.weight_hh_l0, "att_in": att.linear_in.weight,
+                "att_out": att.linear_out.weight, "proj": self.projection.weight}
+
+    def quantize_w4(self, group=64, scale_dtype=torch.float32):
+        """Run the word step's linears on 4-bit weights (ops.quantize_w4) from here on, made from the weights as they
+        are now; the parameters and the state_dict stay as they are. Call again after the weights changed (forward
+        refuses weights that changed since), or dequantize_w4() to go back."""
+        self._w4 = {name: (ops.quantize_w4(W, group, scale_dtype), W, W._version)
+                    for name, W in self._word_linears().items()}
+
+    def dequantize_w4(self):
+        self._w4 = {}
+
+    def _linear(self, name, W, x, b=None, act=None, out=None, beta=0.0):
+        if not self._w4:
+            return ops.linear(x, W, b, act=act, out=out, beta=beta)
+        q, made_from, version = self._w4[name]
+        if W is not made_from or W._version != version or q.device != W.device:
+            raise DasaError(f"SpeakerDecoder: the weight {name!r} changed since quantize_w4(); call it again")
+        return ops.linear_w4(x, q, b, act=act, out=out, beta=beta)
+
+    def _attend(self, h, ctx, mask):
+        """self.attention_layer with output_tilde and output_prob (model.py:268-296) on 4-bit weights."""
+        att = self.attention_layer
+        _, _, wctx = ops.softdot_fwd(self._linear("att_in", att.linear_in.weight, h), ctx, mask)
+        return self._linear("att_out", att.linear_out.weight, torch.cat((wctx, h), 1), act="tanh")
 
     def forward(self, words, ctx, ctx_mask, h0, c0):
         """words [B, L] int64, ctx [B, T, H], ctx_mask [B, T] bool, h0 / c0 [1, B, H] ->
@@ -243,24 +275,25 @@ class SpeakerDecoder(nn.Module):
         if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
             raise NotImplementedError("SpeakerDecoder runs the inference path only (call it under torch.no_grad())")
         B, L = words.shape
-        H, E = self.hidden_size, self.embedding.weight.shape[1]
+        H = self.hidden_size
         training = self.training
-        emb = torch.empty(B * L, E, dtype=torch.float32, device=ctx.device)
-        ops.gather_rows(self.embedding.weight, words.reshape(-1).to(torch.int32), None, None, emb)
-        emb = DF.dropout(emb.view(B, L, E), self.drop.p, training)
+        emb = DF.dropout(ops.embedding(words, self.embedding.weight), self.drop.p, training)
         lw = self.lstm
         h, c = h0.reshape(B, H).contiguous(), c0.reshape(B, H).contiguous()
         outs = []
         for t in range(L):                       # nn.LSTM over the L words (L = 1 while decoding)
-            gates = ops.linear(emb[:, t], lw.weight_ih_l0, lw.bias_ih_l0)
-            ops.linear(h, lw.weight_hh_l0, lw.bias_hh_l0, out=gates, beta=1.0)
+            gates = self._linear("ih", lw.weight_ih_l0, emb[:, t], lw.bias_ih_l0)
+            self._linear("hh", lw.weight_hh_l0, h, lw.bias_hh_l0, out=gates, beta=1.0)
             h, c, _ = ops.lstm_cell_fwd(gates, c)
             outs.append(h)
         x = outs[0].unsqueeze(1) if L == 1 else torch.stack(outs, 1)
         x = DF.dropout(x, self.drop.p, training)
         ctx_x = ctx if L == 1 else ctx.repeat_interleave(L, 0)
         mask_x = ctx_mask if L == 1 else ctx_mask.repeat_interleave(L, 0)
-        x, _ = self.attention_layer(x.reshape(B * L, H), ctx_x.contiguous(), mask_x)
+        if self._w4:
+            x = self._attend(x.reshape(B * L, H), ctx_x.contiguous(), mask_x)
+        else:
+            x, _ = self.attention_layer(x.reshape(B * L, H), ctx_x.contiguous(), mask_x)
         x = DF.dropout(x.view(B, L, H), self.drop.p, training)
-        logit = ops.linear(x, self.projection.weight, self.projection.bias)
+        logit = self._linear("proj", self.projection.weight, x, self.projection.bias)
         return logit, h.unsqueeze(0), c.unsqueeze(0)

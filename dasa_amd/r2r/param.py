@@ -72,6 +72,9 @@ _FLAGS = [
     # mode too (one dropout draw per rollout instead of one per step). Off = the reference's per-step
     # recompute; no gradient changes either way (vilmodel.py:1377-1378 detaches the stack).
     ("--hoist_language", None, "const", False),
+    # not a reference flag: with --d_transformer_update True, train BertEmbeddings' tables and LayerNorm with the
+    # language layers (the reference always does; off = they stay as loaded)
+    ("--d_update_embeddings", None, "const", False),
 ]
 
 README_TRAIN_FLAGS = [

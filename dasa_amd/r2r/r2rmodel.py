@@ -146,6 +146,7 @@ class DicEncoder(nn.Module):
         self.config.img_feature_type = ""
         self.config.update_lang_bert = update
         self.config.update_add_layer = update_add_layer
+        self.config.update_embeddings = args.d_update_embeddings
         self.config.vl_layers = vl_layers
         self.config.la_layers = la_layers
         self.bert = DicModel(self.config)

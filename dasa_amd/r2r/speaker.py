@@ -117,9 +117,15 @@ class Speaker:
         return (img_feats, can_feats), length
 
     # ------------------------------------------------------------------ decoding
-    def infer_batch(self, sampling=False, train=False, featdropmask=None):
+    def infer_batch(self, sampling=False, train=False, featdropmask=None, repetition=None, presence=None,
+                    frequency=None, bias=None, allowed=None):
         """speaker.py:265-350. Returns insts np [B, len] (argmax, or Categorical samples with
-        sampling=True; the train-mode log-prob / hidden / entropy returns are not provided)."""
+        sampling=True; the train-mode log-prob / hidden / entropy returns are not provided).
+
+        repetition / presence / frequency / bias / allowed (none of them in the reference; see ops.logit_rules) rule
+        each word's logits before the choice: penalties count the words the row has written so far, allowed (bool [V]
+        or [B, V], on the device) is joined with the ban of <UNK>. The greedy choice among equal logits is then the
+        lowest index."""
         if train and sampling:
             raise NotImplementedError("speaker training (sampling with gradients) is outside the policy path")
         for m in (self.encoder, self.decoder):
@@ -142,14 +148,28 @@ class Speaker:
             c_t = torch.zeros(1, B, args.rnn_dim, device=self.device)
             ended = np.zeros(B, bool)
             word = torch.full((B, 1), w2i["<BOS>"], dtype=torch.int64, device=self.device)
-            for _ in range(args.maxDecode):
+            ruled = any(r is not None for r in (repetition, presence, frequency, bias, allowed))
+            if ruled:
+                written = torch.full((B, args.maxDecode), -1, dtype=torch.int64, device=self.device)
+                V = self.tok.vocab_size()
+                allowed = torch.ones(V, dtype=torch.bool, device=self.device) if allowed is None else \
+                    allowed.to(torch.bool).clone()
+                allowed[..., w2i["<UNK>"]] = False
+            for t in range(args.maxDecode):
                 logits, h_t, c_t = self.decoder(word, ctx, ctx_mask, h_t, c_t)
                 logits = logits.view(B, -1)
-                logits[:, w2i["<UNK>"]] = -float("inf")            # no <UNK> in inference
+                if ruled:
+                    logits, best = ops.logit_rules(logits, written[:, :t], repetition=repetition, presence=presence,
+                                                   frequency=frequency, bias=bias, allowed=allowed, out=logits,
+                                                   want_choice=True)
+                else:
+                    logits[:, w2i["<UNK>"]] = -float("inf")        # no <UNK> in inference
                 if sampling:
                     word = torch.distributions.Categorical(logits=logits).sample()
                 else:
-                    word = logits.argmax(1)
+                    word = best if ruled else logits.argmax(1)
+                if ruled:
+                    written[:, t] = word
                 cpu_word = word.cpu().numpy().copy()
                 cpu_word[ended] = w2i["<PAD>"]
                 words.append(cpu_word)

@@ -106,7 +106,9 @@ def _fused_weights(owner, mods):
 
 
 class BertEmbeddings(nn.Module):
-    """vilmodel.py:147-176: word + position + token_type(0) -> LayerNorm -> dropout, one kernel."""
+    """vilmodel.py:147-176: word + position + token_type(0) -> LayerNorm -> dropout, one kernel. With `trained` set
+    (config.update_embeddings, --d_update_embeddings) a trained language stack trains the tables and this LayerNorm
+    too, as the reference does; without it they get no gradient."""
 
     def __init__(self, config):
         super().__init__()
@@ -115,10 +117,15 @@ class BertEmbeddings(nn.Module):
         self.token_type_embeddings = nn.Embedding(config.type_vocab_size, config.hidden_size)
         self.LayerNorm = BertLayerNorm(config.hidden_size, eps=config.layer_norm_eps)
         self.dropout = nn.Dropout(config.hidden_dropout_prob)
+        self.trained = bool(getattr(config, "update_embeddings", False))
 
     def forward(self, input_ids, token_type_ids=None, position_ids=None):
         if position_ids is not None or (token_type_ids is not None and bool((token_type_ids != 0).any())):
             raise NotImplementedError("explicit position ids / non-zero token types are not on the DASA path")
+        if self.trained and torch.is_grad_enabled():
+            return DF.bert_embed(input_ids, self.word_embeddings.weight, self.position_embeddings.weight,
+                                 self.token_type_embeddings.weight, self.LayerNorm.weight, self.LayerNorm.bias,
+                                 self.LayerNorm.eps, self.dropout.p, self.training, self.word_embeddings.padding_idx)
         p = self.dropout.p if self.training else 0.0
         return ops.bert_embed(input_ids, self.word_embeddings.weight, self.position_embeddings.weight,
                               self.token_type_embeddings.weight[0], self.LayerNorm.weight, self.LayerNorm.bias,
