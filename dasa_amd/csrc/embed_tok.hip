@@ -126,8 +126,8 @@ int launch_fwd(LookupArgs a, long rows, hipStream_t st) {
 
 // ------------------------------------------------------------------ tokens in sorted order
 constexpr int kSortWaves = 16;
-constexpr int kMaxRange = 512;        // vocabulary rows of one sort workgroup (its counters: 32 KB of LDS)
-constexpr int kList = 256;            // tokens of its range that a wave notes on the first pass
+constexpr int kMaxRange = 896;        // vocabulary rows of one sort workgroup (its counters: 56 KB of LDS)
+constexpr int kList = 1024;           // tokens of its range that a wave notes on the first pass (96 KB of LDS)
 
 struct SortArgs {
   const void* ids;
@@ -137,40 +137,47 @@ struct SortArgs {
   int* order;     // [T] positions in sorted order
 };
 
-// One id as 32 bits: 2^32 - 1, which no vocabulary holds, for the padding id and for ids outside 32 bits.
-__device__ __forceinline__ unsigned token(uint2 v, unsigned pad) { return v.y == 0 && v.x != pad ? v.x : ~0u; }
-__device__ __forceinline__ unsigned token(unsigned v, unsigned pad) { return v != pad ? v : ~0u; }
-__device__ __forceinline__ uint2 no_token(uint2) { return make_uint2(~0u, ~0u); }
-__device__ __forceinline__ unsigned no_token(unsigned) { return ~0u; }
+// The ids of a step as 32-bit tokens: 2^32 - 1, which no vocabulary holds, for an id outside 32 bits.
+__device__ __forceinline__ unsigned low(uint2 v) { return v.x; }
+__device__ __forceinline__ unsigned low(unsigned v) { return v; }
+__device__ __forceinline__ unsigned high(uint2 v) { return v.y; }
+__device__ __forceinline__ unsigned high(unsigned) { return 0; }
 
-// f(position, token) for the ids [t0, t1) of a wave, 64 at a time, U loads in flight; f is called by whole waves
+// f(position, token) for the ids [t0, t1) of a wave, 64 at a time, U loads in flight (and U more of the next group);
+// f is called by whole waves
 template <class W, int U, class F>
-__device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lane, unsigned pad, F f) {
+__device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lane, F f) {
   int t = t0;
-  if (t + 64 * U <= t1) {
+  const int last = t1 - 64 * U;
+  if (t <= last) {
     W v[U], next[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) v[k] = ids[t + lane + 64 * k];
-    for (; t + 64 * U <= t1; t += 64 * U) {
-      const W* p = ids + min(t + 64 * U, t1 - 64 * U) + lane;      // the next group, or the last again
+    for (; t <= last; t += 64 * U) {
+      const W* p = ids + min(t + 64 * U, last) + lane;      // the next group, or the last again
 #pragma unroll
       for (int k = 0; k < U; ++k) next[k] = p[64 * k];
+      unsigned hi = 0;
 #pragma unroll
-      for (int k = 0; k < U; ++k) f(t + 64 * k + lane, token(v[k], pad));
+      for (int k = 0; k < U; ++k) hi |= high(v[k]);
+      if (__builtin_amdgcn_ballot_w64(hi != 0) == 0) {
+#pragma unroll
+        for (int k = 0; k < U; ++k) f(t + 64 * k + lane, low(v[k]));
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < U; ++k) {
+          const W x = ids[t + lane + 64 * k];
+          f(t + 64 * k + lane, high(x) ? ~0u : low(x));
+        }
+      }
 #pragma unroll
       for (int k = 0; k < U; ++k) v[k] = next[k];
     }
   }
-  for (; t < t1; t += 64 * 4) {
-    W v[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = t + 64 * k + lane;
-      v[k] = ids[min(i, t1 - 1)];
-      if (i >= t1) v[k] = no_token(v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f(t + 64 * k + lane, token(v[k], pad));
+#pragma unroll 1
+  for (; t < t1; t += 64) {
+    const W x = ids[min(t + lane, t1 - 1)];
+    f(t + lane, high(x) || t + lane >= t1 ? ~0u : low(x));
   }
 }
 
@@ -178,10 +185,10 @@ __device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lan
 // id at a time: a frequent id is one turn.
 template <class O>
 __device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, int bin, int pos) {
-  unsigned long long m = __ballot(in);
+  unsigned long long m = __builtin_amdgcn_ballot_w64(in);
   while (m) {
     const int b = __builtin_amdgcn_readlane(bin, __builtin_ctzll(m));
-    const unsigned long long same = __ballot(in && bin == b);
+    const unsigned long long same = __builtin_amdgcn_ballot_w64(in && bin == b);
     const int c = cursor[b];
     if ((same >> lane) & 1) order[c + __popcll(same & ((1ull << lane) - 1))] = (O)pos;
     cursor[b] = c + __popcll(same);                  // every lane stores the same value
@@ -191,12 +198,12 @@ __device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, 
 
 template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a) {
-  extern __shared__ int hist[];                    // [waves][R] counts, then write cursors
+  extern __shared__ int lpos[];                    // [waves][kList] positions, [waves][R] counts (then write
+  int* const hist = lpos + kSortWaves * kList;     // cursors), [waves][kList] bins
+  unsigned short* const lbin = reinterpret_cast<unsigned short*>(hist + kSortWaves * a.R);
   __shared__ int below[kSortWaves], wsum[kSortWaves];
-  __shared__ int lpos[kSortWaves][kList];
-  __shared__ unsigned short lbin[kSortWaves][kList];
   const W* ids = reinterpret_cast<const W*>(a.ids);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
   for (int i = tid; i < kSortWaves * a.R; i += 64 * kSortWaves) hist[i] = 0;
   __syncthreads();
@@ -204,16 +211,16 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   const int t0 = min(w * seg, a.T), t1 = min(t0 + seg, a.T);
   int* mine = hist + w * a.R;
   int nb = 0, found = 0;
-  each_token<W, 8>(ids, t0, t1, lane, a.pad, [&](int pos, unsigned u) {
-    nb += __popcll(__ballot(u < lo));
+  each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {
+    nb += __popcll(__builtin_amdgcn_ballot_w64(u < lo && u != a.pad));
     const unsigned bin = u - lo;
-    const bool in = bin < n;
-    unsigned long long m = __ballot(in);
+    const bool in = bin < n && u != a.pad;
+    unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     const int at = found + __popcll(m & ((1ull << lane) - 1));
     if (in && at < kList) {
-      lpos[w][at] = pos;
-      lbin[w][at] = (unsigned short)bin;
+      lpos[w * kList + at] = pos;
+      lbin[w * kList + at] = (unsigned short)bin;
     }
     const int c = __popcll(m);
     found += c;
@@ -222,7 +229,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
     } else {                                       // dense: a frequent id would be one address for most lanes
       while (m) {
         const int b = __builtin_amdgcn_readlane((int)bin, __builtin_ctzll(m));
-        const unsigned long long same = __ballot(in && (int)bin == b);
+        const unsigned long long same = __builtin_amdgcn_ballot_w64(in && (int)bin == b);
         mine[b] += __popcll(same);                 // every lane stores the same value
         m &= ~same;
       }
@@ -258,12 +265,12 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   if (found <= kList) {
     for (int i = 0; i < found; i += 64) {
       const int j = min(i + lane, found - 1);
-      place(mine, a.order, lane, i + lane < found, lbin[w][j], lpos[w][j]);
+      place(mine, a.order, lane, i + lane < found, lbin[w * kList + j], lpos[w * kList + j]);
     }
     return;
   }
-  each_token<W, 8>(ids, t0, t1, lane, a.pad, [&](int pos, unsigned u) {      // a hot range: its ids again
-    place(mine, a.order, lane, u - lo < n, (int)(u - lo), pos);
+  each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {      // a hot range: its ids again
+    place(mine, a.order, lane, u - lo < n && u != a.pad, (int)(u - lo), pos);
   });
 }
 
@@ -297,7 +304,7 @@ struct BwdArgs {
   long ldp;
   void* dtable; long ldt;
   int V, E;
-  unsigned row_blocks;     // blocks of the rows kernel that take table rows; the others take chunks
+  unsigned chunk_blocks;   // blocks of the rows kernel that take chunks (first: they are the longer ones)
   float scale;
   int accumulate;
 };
@@ -346,14 +353,14 @@ __device__ __forceinline__ long id_at(const BwdArgs& a, int pos) {
 template <class T>
 __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  if (blockIdx.x < a.row_blocks) {
-    const long v = (long)blockIdx.x * 4 + w;
+  if (blockIdx.x >= a.chunk_blocks) {
+    const long v = (long)(blockIdx.x - a.chunk_blocks) * 4 + w;
     if (v >= a.V) return;
     const int s = a.start[v], n = a.start[v + 1] - s;
     if (n > kChunk || (a.accumulate && n == 0)) return;
@@ -362,7 +369,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
     if (live) write_row<T>(a, v, col, left, acc);
     return;
   }
-  const long c = (long)(blockIdx.x - a.row_blocks) * 4 + w;
+  const long c = (long)blockIdx.x * 4 + w;
   const int j0 = (int)(c * kChunk), total = a.start[a.V];
   if (j0 >= total) return;
   const int m = min(kChunk, total - j0);
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
 template <class T>
 __device__ __forceinline__ void add_parts(float (&acc)[Vec<T>::N], const BwdArgs& a, long c, int first, int k0, int k1,
                                           int col) {
-#pragma unroll 4
+#pragma unroll 2
   for (int k = k0; k < k1; ++k) {
     const float* p = a.parts + ((c + k) * 2 + (k == 0 ? first : 0)) * a.ldp + col;
 #pragma unroll
@@ -409,7 +416,7 @@ template <class T>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
   __shared__ float sum[kJoinWaves][64][N];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
   const int total = a.start[a.V];
   float acc[N];
@@ -465,7 +472,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   unsigned short* const lbin = lpos + kFewWaves * seg;
   float* const sum = reinterpret_cast<float*>(lpos);       // [waves][64][N]
   const W* ids = reinterpret_cast<const W*>(a.ids);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const unsigned lo = blockIdx.x * (unsigned)g.R, n = min((unsigned)g.R, a.V - lo);
   const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
   for (int i = tid; i < kFewWaves * kFewRange; i += 64 * kFewWaves) hist[0][i] = 0;
@@ -473,10 +480,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   __syncthreads();
   const int t0 = min(w * seg, g.T), t1 = min(t0 + seg, g.T);
   int found = 0;
-  each_token<W, 4>(ids, t0, t1, lane, g.pad, [&](int pos, unsigned u) {
+  each_token<W, 4>(ids, t0, t1, lane, [&](int pos, unsigned u) {
     const unsigned bin = u - lo;
-    const bool in = bin < n;
-    const unsigned long long m = __ballot(in);
+    const bool in = bin < n && u != g.pad;
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     if (in) {
       const int at = found + __popcll(m & ((1ull << lane) - 1));
@@ -574,9 +581,9 @@ inline long part_stride(int E, int bf16) {      // whole units, so a partial uni
 template <class T>
 int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
-  a.row_blocks = (unsigned)((a.V + 3) / 4);
   const long chunks = (tokens + kChunk - 1) / kChunk;
-  const dim3 grid(a.row_blocks + (unsigned)((chunks + 3) / 4), slices);
+  a.chunk_blocks = (unsigned)((chunks + 3) / 4);
+  const dim3 grid(a.chunk_blocks + (unsigned)((a.V + 3) / 4), slices);
   hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
   hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
@@ -632,7 +639,7 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   if (G < 256) G = V < 256 ? V : 256;
   sa.R = (V + G - 1) / G;
   G = (V + sa.R - 1) / sa.R;
-  const size_t lds = (size_t)kSortWaves * sa.R * sizeof(int);
+  const size_t lds = (size_t)kSortWaves * (sa.R * 4 + kList * 6);
   if (ids_bytes == 8) hipLaunchKernelGGL(token_sort_kernel<uint2>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
   else hipLaunchKernelGGL(token_sort_kernel<unsigned>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
   DASA_CHECK_LAUNCH();

@@ -257,20 +257,19 @@ __global__ __launch_bounds__(64 * W, W >= 16 ? 4 : MT == 4 ? 2 : 4) void w4_kern
   }
 }
 
-constexpr int kShareWaves = 8;
 constexpr int kAhead = 4;       // even: the two activation buffers keep their places over a turn of the ring
 
 // The form for more rows: the workgroup's waves own NT column blocks each and walk K together, so the activations'
 // fragments are split into their planes once for the 8 NT blocks, in LDS (two buffers, one barrier a 128-deep block),
 // where each wave reads them back in fragment order.
-template <class T, class S, int MT, int NT, int GPB>
-__global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a) {
+template <class T, class S, int MT, int NT, int GPB, int SW>
+__global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
   typedef XFrag<T> X;
-  constexpr int PL = X::PL, UNITS = MT * 4, PER = (UNITS + kShareWaves - 1) / kShareWaves;   // fragments a wave makes
+  constexpr int PL = X::PL, UNITS = MT * 4, PER = (UNITS + SW - 1) / SW;   // fragments a wave makes
   extern __shared__ float4 smem[];
   bf16x8* frag = reinterpret_cast<bf16x8*>(smem);       // [2][PL][4 steps][MT][64]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int nt0 = (blockIdx.x * kShareWaves + w) * NT, m0 = blockIdx.y * (16 * MT);
+  const int nt0 = (blockIdx.x * SW + w) * NT, m0 = blockIdx.y * (16 * MT);
   const int c16 = lane & 15, kq = lane >> 4;
   floatx4 y[NT][MT];
 #pragma unroll
@@ -282,8 +281,8 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
   auto fetch = [&](int kb, typename X::Raw (&r)[PER]) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int f = u * kShareWaves + w;
-      if (UNITS % kShareWaves && f >= UNITS) continue;
+      const int f = u * SW + w;
+      if (UNITS % SW && f >= UNITS) continue;
       const int m = f % MT, k = kb * 128 + (f / MT) * 32 + kq * 8;
       const T* p = reinterpret_cast<const T*>(a.x) + (long)min(m0 + m * 16 + c16, a.M - 1) * a.ldx + k;
       r[u] = kb * 128 + 128 <= a.K ? X::load(p) : X::load_part(p, a.K - k);
@@ -292,8 +291,8 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
   auto put = [&](int buf, const typename X::Raw (&r)[PER]) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int f = u * kShareWaves + w;
-      if (UNITS % kShareWaves && f >= UNITS) continue;
+      const int f = u * SW + w;
+      if (UNITS % SW && f >= UNITS) continue;
       bf16x8 q[PL];
       X::planes(r[u], q);
 #pragma unroll
@@ -397,14 +396,14 @@ int launch_join(const W4Args& a, int splits, int tiles, hipStream_t st) {
   return 0;
 }
 
-template <class T, class S, int MT, int NT>
+template <class T, class S, int MT, int NT, int SW>
 int launch_shared(const W4Args& a, int g, int splits, hipStream_t st) {
-  const int cols = kShareWaves * NT;
-  const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * kShareWaves);
+  const int cols = SW * NT;
+  const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * SW);
   const size_t lds = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16;
-  if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4>), grid, block, lds, st, a);
-  else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1>), grid, block, lds, st, a);
+  if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4, SW>), grid, block, lds, st, a);
+  else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2, SW>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1, SW>), grid, block, lds, st, a);
   DASA_CHECK_LAUNCH();
   return launch_join<T>(a, splits, (int)grid.y * MT, st);
 }
@@ -424,8 +423,8 @@ int launch_g(const W4Args& a, int g, int splits, hipStream_t st) {
 template <class T, class S>
 int launch_plan(const W4Args& a, int g, const Plan& p, hipStream_t st) {
   if (p.shared) {
-    if (p.mt == 2) return p.nt == 2 ? launch_shared<T, S, 2, 2>(a, g, p.splits, st) : launch_shared<T, S, 2, 1>(a, g, p.splits, st);
-    return p.nt == 2 ? launch_shared<T, S, 4, 2>(a, g, p.splits, st) : launch_shared<T, S, 4, 1>(a, g, p.splits, st);
+    if (p.mt == 2) return p.nt == 2 ? launch_shared<T, S, 2, 2, 8>(a, g, p.splits, st) : launch_shared<T, S, 2, 1, 8>(a, g, p.splits, st);
+    return p.nt == 2 ? launch_shared<T, S, 4, 2, 8>(a, g, p.splits, st) : launch_shared<T, S, 4, 1, 8>(a, g, p.splits, st);
   }
   if (p.mt == 4) return launch_g<T, S, 4, 1, 8>(a, g, p.splits, st);
   if (p.mt == 2) return p.waves == 8 ? launch_g<T, S, 2, 1, 8>(a, g, p.splits, st) : launch_g<T, S, 2, 1, 16>(a, g, p.splits, st);
