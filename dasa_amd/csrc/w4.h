@@ -159,6 +159,43 @@ __device__ __forceinline__ void epilogue(const W4Args& a, float4 s, int n, int r
   }
 }
 
+// four consecutive columns of one output row
+template <class T>
+__device__ __forceinline__ void store4(const W4Args& a, float4 s, int row, int n) {
+  typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef float F __attribute__((ext_vector_type(4), aligned(4)));
+  const int left = a.N - n;
+  if (left <= 0) return;
+  T* o = reinterpret_cast<T*>(a.y) + (long)row * a.ldy + n;
+  float r[4] = {s.x, s.y, s.z, s.w};
+  float b[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.bias) {
+    if (left >= 4) {
+      const F v = *reinterpret_cast<const F*>(a.bias + n);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = v[e];
+    } else {
+      for (int e = 0; e < left; ++e) b[e] = a.bias[n + e];
+    }
+  }
+  V v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float y = 16.f * r[e];
+    if (a.bias) y += b[e];
+    y = act_of(y, a.act);
+    if (a.beta != 0.f && e < left) y += a.beta * (float)o[e];
+    v[e] = (T)y;
+  }
+  if (left >= 4) {
+    *reinterpret_cast<V*>(o) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) o[e] = v[e];
+  }
+}
+
 // MT = 16-row tiles of x, NT = 16-column blocks of a workgroup, GPB = groups of a 128-deep block, W = waves
 template <class T, class S, int MT, int NT, int GPB, int W>
 __global__ __launch_bounds__(64 * W, W >= 16 ? 4 : MT == 4 ? 2 : 4) void w4_kernel(W4Args a) {
@@ -354,15 +391,31 @@ __global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
       __syncthreads();
     }
   }
+  if (a.part) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if (nt0 + t < a.N16)
+          a.part[(((long)blockIdx.z * gridDim.y * MT + blockIdx.y * MT + m) * a.N16 + nt0 + t) * 64 + lane] =
+              make_float4(y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]);
+    return;
+  }
+  // the sums through LDS, so that a row's columns leave in runs of four (a fragment holds four rows of one column:
+  // stored from there, 64 x 30522 bf16 outputs took 4 us more)
+  constexpr int COLS = SW * NT * 16, LD = COLS + 4;
+  float* tile = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const float4 s = make_float4(y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]);
-      if (nt0 + t >= a.N16) continue;
-      if (a.part) a.part[(((long)blockIdx.z * gridDim.y * MT + blockIdx.y * MT + m) * a.N16 + nt0 + t) * 64 + lane] = s;
-      else epilogue<T>(a, s, (nt0 + t) * 16 + c16, m0 + m * 16 + kq * 4);
-    }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile[(m * 16 + kq * 4 + i) * LD + (w * NT + t) * 16 + c16] = y[t][m][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MT * (COLS / 4); i += 64 * SW) {
+    const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
+    if (m0 + r < a.M) store4<T>(a, *reinterpret_cast<const float4*>(tile + r * LD + c), m0 + r, blockIdx.x * COLS + c);
+  }
 }
 
 // The splits of K joined in order: one thread = four output rows of one column.
@@ -400,7 +453,8 @@ template <class T, class S, int MT, int NT, int SW>
 int launch_shared(const W4Args& a, int g, int splits, hipStream_t st) {
   const int cols = SW * NT;
   const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * SW);
-  const size_t lds = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16;
+  const size_t frags = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16, tile = (size_t)16 * MT * (cols * 16 + 4) * 4;
+  const size_t lds = frags > tile ? frags : tile;
   if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4, SW>), grid, block, lds, st, a);
   else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2, SW>), grid, block, lds, st, a);
   else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1, SW>), grid, block, lds, st, a);
