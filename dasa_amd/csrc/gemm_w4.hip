@@ -2,6 +2,8 @@
 // kernels that run once for a weight.
 #include "w4.h"
 
+#include <algorithm>
+
 // gemm_w4_bf16.hip: the instantiations for bf16 activations
 __attribute__((visibility("hidden"))) int dasa_w4_launch_bf16(const w4::W4Args& a, int group, const w4::Plan& p,
                                                               int scale_bf16, hipStream_t st);
@@ -11,37 +13,36 @@ namespace {
 using w4::Plan;
 using w4::W4Args;
 
+// Which form and shape: measured over M = 1 .. 64, N = 992 .. 32768, K = 256 .. 8192 in both types (us):
+//  * few weights per row tile (tiles x row tiles < 3500): the split form with each 16 rows a workgroup of their own.
+//    The weights come from cache for the second rows; holding several row tiles in a workgroup instead leaves the chip
+//    emptier (20 x 4096 x 2240 fp32 8.6 against 11.4, 64 x 992 x 512 fp32 4.1 against 7.8). Column blocks of a
+//    workgroup: as many as still leave about one workgroup a CU, since they share the activations' loads and their
+//    splitting into planes; bf16 rows need no splitting and stop at two (1 x 32768 x 8192 bf16 31.2 against 33.0).
+//  * many weights and more than 16 rows: the shared form (64 x 30522 x 768 bf16 11.6 against 19.8, 64 x 16384 x 4096
+//    fp32 35.7 against 39), two row tiles a workgroup, four where the weights are too many to read twice
+//    (64 x 32768 x 8192 bf16 63 against 83).
+//  * K is split over workgroups, at the price of a second launch (2 us), only where a long K leaves too few of them
+//    (1 x 1000 x 8192 fp32 7.7 against 13.4).
 inline Plan plan_of(int M, int N, int K, int bf16) {
-  Plan p;
-  const int tiles = (N + 15) / 16, Kb = (K + 127) / 128;
-  p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  p.shared = false;
+  Plan p{};
+  const long tiles = (N + 15) / 16, Kb = (K + 127) / 128, rows = (M + 15) / 16, units = tiles * rows;
+  p.mt = 1;
   p.nt = 1;
-  p.waves = Kb > 8 && p.mt < 4 ? 16 : 8;
+  p.waves = 8;
   p.splits = 1;
-  if (p.mt > 1) {
-    const int nt = tiles >= 1024 && Kb >= 16 ? 2 : 1, wgs = (tiles + 8 * nt - 1) / (8 * nt);
-    int s = 256 / wgs;
-    if (s > Kb / 8) s = Kb / 8;
-    if (s < 1) s = 1;
-    if (wgs * s >= 192) {
-      p.shared = true;
-      p.nt = nt;
-      p.splits = s;
-      return p;
-    }
-  } else if (tiles >= 512) {
-    p.nt = bf16 || tiles < 1024 ? 2 : 4;
-    p.waves = p.nt == 4 && tiles <= 1024 && Kb >= 16 ? 16 : 8;
-  } else if (!bf16 && Kb >= 48 && tiles > 128) {
-    p.nt = 4;
-    p.waves = 16;
-    p.splits = 1024 / tiles < Kb / 16 ? 1024 / tiles : Kb / 16;
+  if (rows > 1 && units >= 3500) {
+    p.shared = true;
+    p.mt = rows > 2 && tiles * Kb >= 65536 ? 4 : 2;
+    p.nt = p.mt == 4 || rows > 2 || Kb >= 16 ? 2 : 1;
+    const long wgs = (tiles + 8 * p.nt - 1) / (8 * p.nt) * ((rows + p.mt - 1) / p.mt);
+    p.splits = (int)std::max(1L, std::min(256 / wgs, Kb / 8));
+    return p;
   }
-  if (tiles <= 128 && Kb >= 32) {
-    p.splits = 256 / tiles < Kb / 16 ? 256 / tiles : Kb / 16;
-    if (p.splits > 16) p.splits = 16;
-  }
+  if (Kb >= 48 && (!bf16 || rows > 1)) p.splits = (int)std::max(1L, std::min({Kb / 16, 4L, 1024 / units}));
+  const long fill = units * p.splits;            // workgroups of one column block
+  p.nt = fill < 384 ? 1 : fill < 640 || (bf16 && rows == 1) ? 2 : 4;
+  p.waves = Kb > 8 && fill / p.nt <= 256 ? 16 : 8;
   return p;
 }
 

@@ -196,25 +196,21 @@ __device__ __forceinline__ void store4(const W4Args& a, float4 s, int row, int n
   }
 }
 
-// MT = 16-row tiles of x, NT = 16-column blocks of a workgroup, GPB = groups of a 128-deep block, W = waves
-template <class T, class S, int MT, int NT, int GPB, int W>
-__global__ __launch_bounds__(64 * W, W >= 16 ? 4 : MT == 4 ? 2 : 4) void w4_kernel(W4Args a) {
+// Split form. A workgroup owns 16 rows of x and NT blocks of 16 columns; its W waves take the 128-deep blocks of K in
+// turn, straight from memory, and their sums meet in LDS in wave order. GPB = groups of a 128-deep block.
+template <class T, class S, int NT, int GPB, int W>
+__global__ __launch_bounds__(64 * W, 4) void w4_split_kernel(W4Args a) {
   typedef XFrag<T> X;
   constexpr int PL = X::PL;
-  extern __shared__ float4 part[];          // [W][NT][MT][64]
+  extern __shared__ float4 part[];          // [W][NT][64]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+  const int nt0 = blockIdx.x * NT, m0 = blockIdx.y * 16;
   const int c16 = lane & 15, kq = lane >> 4;
-  floatx4 y[NT][MT];
+  floatx4 y[NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) y[t][m] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) y[t] = floatx4{0.f, 0.f, 0.f, 0.f};
   // a row past the last repeats it: it only reaches output rows that are not stored
-  const T* x[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-    x[m] = reinterpret_cast<const T*>(a.x) + (long)min(m0 + m * 16 + c16, a.M - 1) * a.ldx + kq * 8;
+  const T* x = reinterpret_cast<const T*>(a.x) + (long)min(m0 + c16, a.M - 1) * a.ldx + kq * 8;
   long blk0[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) blk0[t] = (long)min(nt0 + t, a.N16 - 1) * a.Kb;
@@ -229,42 +225,28 @@ __global__ __launch_bounds__(64 * W, W >= 16 ? 4 : MT == 4 ? 2 : 4) void w4_kern
       wq[t] = a.w[(blk0[t] + kb) * 64 + lane];
       load_scales<S, GPB>(a.scales, (blk0[t] + kb) * 16 + c16, sc[t]);
     }
-    floatx4 acc[NT][MT];
-    // activations: the whole block's loads first, or (many rows of fp32) one 32-deep step ahead of its use
-    constexpr int R = MT * sizeof(T) > 8 ? 2 : 4;
-    typename X::Raw raw[R][MT];
-    auto load = [&](int j) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int k = kb * 128 + j * 32;
-        if constexpr (TAIL) raw[j % R][m] = X::load_part(x[m] + k, a.K - k - kq * 8);
-        else raw[j % R][m] = X::load(x[m] + k);
-      }
-    };
-#pragma unroll
-    for (int j = 0; j < R; ++j) load(j);
+    typename X::Raw raw[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      bf16x8 xf[MT][PL];
+      const int k = kb * 128 + j * 32;
+      if constexpr (TAIL) raw[j] = X::load_part(x + k, a.K - k - kq * 8);
+      else raw[j] = X::load(x + k);
+    }
+    floatx4 acc[NT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) X::planes(raw[j % R][m], xf[m]);
-      if (j + R < 4) load(j + R);
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 xf[PL];
+      X::planes(raw[j], xf);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const unsigned word = j == 0 ? wq[t].x : j == 1 ? wq[t].y : j == 2 ? wq[t].z : wq[t].w;
-        const bf16x8 wf = unpack8(word);
+        const bf16x8 wf = unpack8(j == 0 ? wq[t].x : j == 1 ? wq[t].y : j == 2 ? wq[t].z : wq[t].w);
+        if (j % (4 / GPB) == 0) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (j % (4 / GPB) == 0) acc[t][m] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int p = PL - 1; p >= 0; --p)     // small planes first
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[p], wf, acc[t], 0, 0, 0);
+        if (j % (4 / GPB) == 4 / GPB - 1)
 #pragma unroll
-          for (int p = PL - 1; p >= 0; --p)     // small planes first
-            acc[t][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[m][p], wf, acc[t][m], 0, 0, 0);
-          if (j % (4 / GPB) == 4 / GPB - 1) {
-            const float s = sc[t][j / (4 / GPB)];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[t][m][i] += s * acc[t][m][i];
-          }
-        }
+          for (int i = 0; i < 4; ++i) y[t][i] += sc[t][j / (4 / GPB)] * acc[t][i];
       }
     }
   };
@@ -272,41 +254,35 @@ __global__ __launch_bounds__(64 * W, W >= 16 ? 4 : MT == 4 ? 2 : 4) void w4_kern
   if (full >= k0 && full < k1 && (full - k0) % W == w) block(full, std::true_type{});
 
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-      part[((w * NT + t) * MT + m) * 64 + lane] = make_float4(y[t][m][0], y[t][m][1], y[t][m][2], y[t][m][3]);
+  for (int t = 0; t < NT; ++t) part[(w * NT + t) * 64 + lane] = make_float4(y[t][0], y[t][1], y[t][2], y[t][3]);
   __syncthreads();
-  for (int i = threadIdx.x; i < NT * MT * 64; i += 64 * W) {
+  for (int i = threadIdx.x; i < NT * 64; i += 64 * W) {
     float4 s = part[i];
 #pragma unroll
     for (int k = 1; k < W; ++k) {
-      const float4 v = part[k * NT * MT * 64 + i];
+      const float4 v = part[k * NT * 64 + i];
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
-    const int l = i & 63, m = (i >> 6) % MT, t = (i >> 6) / MT;
-    if (a.part) {
-      if (nt0 + t < a.N16)
-        a.part[(((long)blockIdx.z * gridDim.y * MT + blockIdx.y * MT + m) * a.N16 + nt0 + t) * 64 + l] = s;
-      continue;
-    }
-    epilogue<T>(a, s, (nt0 + t) * 16 + (l & 15), m0 + m * 16 + (l >> 4) * 4);
+    const int l = i & 63, t = i >> 6;
+    if (!a.part) epilogue<T>(a, s, (nt0 + t) * 16 + (l & 15), m0 + (l >> 4) * 4);
+    else if (nt0 + t < a.N16) a.part[(((long)blockIdx.z * gridDim.y + blockIdx.y) * a.N16 + nt0 + t) * 64 + l] = s;
   }
 }
 
+constexpr int kShareWaves = 8;
 constexpr int kAhead = 4;       // even: the two activation buffers keep their places over a turn of the ring
 
 // The form for more rows: the workgroup's waves own NT column blocks each and walk K together, so the activations'
 // fragments are split into their planes once for the 8 NT blocks, in LDS (two buffers, one barrier a 128-deep block),
 // where each wave reads them back in fragment order.
-template <class T, class S, int MT, int NT, int GPB, int SW>
-__global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
+template <class T, class S, int MT, int NT, int GPB>
+__global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a) {
   typedef XFrag<T> X;
-  constexpr int PL = X::PL, UNITS = MT * 4, PER = (UNITS + SW - 1) / SW;   // fragments a wave makes
+  constexpr int PL = X::PL, UNITS = MT * 4, PER = (UNITS + kShareWaves - 1) / kShareWaves;   // fragments a wave makes
   extern __shared__ float4 smem[];
   bf16x8* frag = reinterpret_cast<bf16x8*>(smem);       // [2][PL][4 steps][MT][64]
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int nt0 = (blockIdx.x * SW + w) * NT, m0 = blockIdx.y * (16 * MT);
+  const int nt0 = (blockIdx.x * kShareWaves + w) * NT, m0 = blockIdx.y * (16 * MT);
   const int c16 = lane & 15, kq = lane >> 4;
   floatx4 y[NT][MT];
 #pragma unroll
@@ -318,8 +294,8 @@ __global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
   auto fetch = [&](int kb, typename X::Raw (&r)[PER]) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int f = u * SW + w;
-      if (UNITS % SW && f >= UNITS) continue;
+      const int f = u * kShareWaves + w;
+      if (UNITS % kShareWaves && f >= UNITS) continue;
       const int m = f % MT, k = kb * 128 + (f / MT) * 32 + kq * 8;
       const T* p = reinterpret_cast<const T*>(a.x) + (long)min(m0 + m * 16 + c16, a.M - 1) * a.ldx + k;
       r[u] = kb * 128 + 128 <= a.K ? X::load(p) : X::load_part(p, a.K - k);
@@ -328,8 +304,8 @@ __global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
   auto put = [&](int buf, const typename X::Raw (&r)[PER]) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int f = u * SW + w;
-      if (UNITS % SW && f >= UNITS) continue;
+      const int f = u * kShareWaves + w;
+      if (UNITS % kShareWaves && f >= UNITS) continue;
       bf16x8 q[PL];
       X::planes(r[u], q);
 #pragma unroll
@@ -403,7 +379,7 @@ __global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
   }
   // the sums through LDS, so that a row's columns leave in runs of four (a fragment holds four rows of one column:
   // stored from there, 64 x 30522 bf16 outputs took 4 us more)
-  constexpr int COLS = SW * NT * 16, LD = COLS + 4;
+  constexpr int COLS = kShareWaves * NT * 16, LD = COLS + 4;
   float* tile = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -412,7 +388,7 @@ __global__ __launch_bounds__(64 * SW, 2) void w4_shared_kernel(W4Args a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) tile[(m * 16 + kq * 4 + i) * LD + (w * NT + t) * 16 + c16] = y[t][m][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * MT * (COLS / 4); i += 64 * SW) {
+  for (int i = threadIdx.x; i < 16 * MT * (COLS / 4); i += 64 * kShareWaves) {
     const int r = i / (COLS / 4), c = (i % (COLS / 4)) * 4;
     if (m0 + r < a.M) store4<T>(a, *reinterpret_cast<const float4*>(tile + r * LD + c), m0 + r, blockIdx.x * COLS + c);
   }
@@ -434,9 +410,10 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4Args a, int splits, int 
 }
 
 struct Plan {
-  int mt;        // 16-row tiles of x in a workgroup
   bool shared;   // which form
-  int nt, waves; // column blocks of a workgroup (split form) or of a wave (shared form); waves of the split form
+  int mt;        // 16-row tiles of a workgroup (split form: 1)
+  int nt;        // column blocks of a workgroup (split form) or of a wave (shared form)
+  int waves;     // of a workgroup
   int splits;    // of K over workgroups
 };
 
@@ -449,42 +426,39 @@ int launch_join(const W4Args& a, int splits, int tiles, hipStream_t st) {
   return 0;
 }
 
-template <class T, class S, int MT, int NT, int SW>
+template <class T, class S, int MT, int NT>
 int launch_shared(const W4Args& a, int g, int splits, hipStream_t st) {
-  const int cols = SW * NT;
-  const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * SW);
-  const size_t frags = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16, tile = (size_t)16 * MT * (cols * 16 + 4) * 4;
-  const size_t lds = frags > tile ? frags : tile;
-  if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4, SW>), grid, block, lds, st, a);
-  else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2, SW>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1, SW>), grid, block, lds, st, a);
+  constexpr int cols = kShareWaves * NT;
+  const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * kShareWaves);
+  constexpr size_t frags = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16, tile = (size_t)16 * MT * (cols * 16 + 4) * 4;
+  constexpr size_t lds = frags > tile ? frags : tile;
+  if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4>), grid, block, lds, st, a);
+  else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1>), grid, block, lds, st, a);
   DASA_CHECK_LAUNCH();
   return launch_join<T>(a, splits, (int)grid.y * MT, st);
 }
 
-template <class T, class S, int MT, int NT, int W>
-int launch_g(const W4Args& a, int g, int splits, hipStream_t st) {
-  const dim3 grid((a.N16 + NT - 1) / NT, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * W);
-  const size_t lds = (size_t)W * NT * MT * 64 * 16;
-  if (g == 32) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 4, W>), grid, block, lds, st, a);
-  else if (g == 64) hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 2, W>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((w4_kernel<T, S, MT, NT, 1, W>), grid, block, lds, st, a);
+template <class T, class S, int NT, int W>
+int launch_split(const W4Args& a, int g, int splits, hipStream_t st) {
+  const dim3 grid((a.N16 + NT - 1) / NT, (a.M + 15) / 16, splits), block(64 * W);
+  constexpr size_t lds = (size_t)W * NT * 64 * 16;
+  if (g == 32) hipLaunchKernelGGL((w4_split_kernel<T, S, NT, 4, W>), grid, block, lds, st, a);
+  else if (g == 64) hipLaunchKernelGGL((w4_split_kernel<T, S, NT, 2, W>), grid, block, lds, st, a);
+  else hipLaunchKernelGGL((w4_split_kernel<T, S, NT, 1, W>), grid, block, lds, st, a);
   DASA_CHECK_LAUNCH();
-  return launch_join<T>(a, splits, (int)grid.y * MT, st);
+  return launch_join<T>(a, splits, (int)grid.y, st);
 }
 
-// the forms that plan_of() chooses from
 template <class T, class S>
 int launch_plan(const W4Args& a, int g, const Plan& p, hipStream_t st) {
   if (p.shared) {
-    if (p.mt == 2) return p.nt == 2 ? launch_shared<T, S, 2, 2, 8>(a, g, p.splits, st) : launch_shared<T, S, 2, 1, 8>(a, g, p.splits, st);
-    return p.nt == 2 ? launch_shared<T, S, 4, 2, 8>(a, g, p.splits, st) : launch_shared<T, S, 4, 1, 8>(a, g, p.splits, st);
+    if (p.mt == 4) return launch_shared<T, S, 4, 2>(a, g, p.splits, st);
+    return p.nt == 2 ? launch_shared<T, S, 2, 2>(a, g, p.splits, st) : launch_shared<T, S, 2, 1>(a, g, p.splits, st);
   }
-  if (p.mt == 4) return launch_g<T, S, 4, 1, 8>(a, g, p.splits, st);
-  if (p.mt == 2) return p.waves == 8 ? launch_g<T, S, 2, 1, 8>(a, g, p.splits, st) : launch_g<T, S, 2, 1, 16>(a, g, p.splits, st);
-  if (p.nt == 1) return p.waves == 8 ? launch_g<T, S, 1, 1, 8>(a, g, p.splits, st) : launch_g<T, S, 1, 1, 16>(a, g, p.splits, st);
-  if (p.nt == 2) return launch_g<T, S, 1, 2, 8>(a, g, p.splits, st);
-  return p.waves == 8 ? launch_g<T, S, 1, 4, 8>(a, g, p.splits, st) : launch_g<T, S, 1, 4, 16>(a, g, p.splits, st);
+  if (p.nt == 4) return p.waves == 8 ? launch_split<T, S, 4, 8>(a, g, p.splits, st) : launch_split<T, S, 4, 16>(a, g, p.splits, st);
+  if (p.nt == 2) return p.waves == 8 ? launch_split<T, S, 2, 8>(a, g, p.splits, st) : launch_split<T, S, 2, 16>(a, g, p.splits, st);
+  return p.waves == 8 ? launch_split<T, S, 1, 8>(a, g, p.splits, st) : launch_split<T, S, 1, 16>(a, g, p.splits, st);
 }
 
 }  // namespace w4
