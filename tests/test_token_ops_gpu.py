@@ -193,8 +193,9 @@ def _w4(N, K, group, sdt, seed):
 def _check_w4(got, x, W, group, dtype, what, bias=None, extra=None):
     """Products are exact; an fp32 sum adds three planes of every product (an addition off by at most a whole step,
     2^-23), one scaling a group, the joins of the waves and the bias."""
-    xd = x.cpu().double()
-    want, mag = xd @ W.t(), xd.abs() @ W.abs().t()
+    xd = x.to(got.device).double()
+    W = W.to(got.device)
+    want, mag = (xd @ W.t()).cpu(), (xd.abs() @ W.abs().t()).cpu()
     K = W.shape[1]
     tol = mag * (3 * K + 2 * (-(-K // group)) + 16) * 2 * U
     if bias is not None:
@@ -221,9 +222,13 @@ def test_w4_weight_values(dev, N, K, group):
 @pytest.mark.parametrize("M,N,K,group", [(1, 1, 1, 32), (1, 2048, 256, 64), (2, 1000, 512, 128), (15, 17, 33, 32),
                                          (16, 992, 512, 64), (17, 100, 1000, 128), (20, 4096, 2240, 64),
                                          (31, 50, 2241, 32), (33, 130, 127, 64), (64, 8200, 640, 128), (65, 33, 96, 32),
-                                         (150, 8193, 255, 64), (1, 30522, 768, 32)])
+                                         (150, 8193, 255, 64), (1, 30522, 768, 32), (20, 30522, 200, 64),
+                                         (64, 16384, 2100, 64), (40, 65536, 2041, 128), (3, 100, 8000, 32),
+                                         (20, 100, 8000, 64), (48, 2100, 300, 128)])
 def test_linear_w4(dev, dtype, M, N, K, group):
-    for sdt in (F32, BF16):
+    """Every form: 16 rows a workgroup with 1, 2 and 4 column blocks, K split over workgroups, 32 and 64 rows sharing
+    their activations, rows and columns that end inside a tile, an inner size that ends inside a group."""
+    for sdt in (F32, BF16) if N < 20000 else (F32 if dtype == F32 else BF16,):
         codes, scales, W = _w4(N, K, group, sdt, M + N + K)
         w = ops.pack_w4(codes.to(dev), scales.to(dev), K, group)
         x = torch.randn(M, K, generator=_gen(M)).to(dtype)
