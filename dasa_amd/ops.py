@@ -1054,21 +1054,23 @@ def _on_device(what, *ts):
     return cur
 
 
+_FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1}     # the bf16 argument of the entry points
+_ID_BYTES = {torch.int64: 8, torch.int32: 4}
+
+
 def _float_type(t, what):
-    """0 for float32, 1 for bfloat16 (the bf16 argument of the entry points); anything else raises."""
-    if t.dtype == torch.float32:
-        return 0
-    if t.dtype == torch.bfloat16:
-        return 1
-    raise _lib.DasaError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+    """0 for float32, 1 for bfloat16; anything else raises."""
+    k = _FLOAT_TYPES.get(t.dtype)
+    if k is None:
+        raise _lib.DasaError(f"{what}: expected float32 or bfloat16, got {t.dtype}")
+    return k
 
 
 def _ids_bytes(ids, what):
-    if ids.dtype == torch.int64:
-        return 8
-    if ids.dtype == torch.int32:
-        return 4
-    raise _lib.DasaError(f"{what}: expected int64 or int32 ids, got {ids.dtype}")
+    k = _ID_BYTES.get(ids.dtype)
+    if k is None:
+        raise _lib.DasaError(f"{what}: expected int64 or int32 ids, got {ids.dtype}")
+    return k
 
 
 def _row_view(t, what):
@@ -1081,8 +1083,9 @@ def _row_view(t, what):
     return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else N
 
 
-def _out_rows(out, shape, like, what):
-    """Check a caller's output tensor: shape, type, device, rows of one stride. Returns the row stride."""
+def _out_rows(out, shape, like, what, *reads):
+    """Check a caller's output tensor: shape, type, rows of one stride, apart from the tensors that the call reads
+    (or exactly the first of them, where `like` is it and the call works in place). Returns the row stride."""
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype:
         raise _lib.DasaError(f"{what}: out must be {tuple(shape)} {like.dtype}, got {tuple(out.shape)} {out.dtype}")
     if out.numel() == 0:
@@ -1090,7 +1093,27 @@ def _out_rows(out, shape, like, what):
     rows, ld = _rows(out)
     if rows > 1 and ld < shape[-1]:
         raise _lib.DasaError(f"{what}: the rows of out overlap")
-    return max(ld, shape[-1])
+    ld = max(ld, shape[-1])
+    for t in reads:
+        if t is not None and t.numel() and _share_memory(out, ld, t):
+            raise _lib.DasaError(f"{what}: out overlaps a tensor that the call reads")
+    return ld
+
+
+def _share_memory(a, lda, b):
+    """Whether the rows of a (row stride lda) and of b share bytes; b of any layout. Exact for two tensors of one row
+    stride (column blocks of one buffer), else by their address ranges."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+    es = a.element_size()
+    end = lambda t: t.data_ptr() + (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()  # noqa
+    if a.data_ptr() >= end(b) or b.data_ptr() >= end(a):
+        return False
+    if es == b.element_size() and b.dim() > 1 and b.stride(-1) == 1 and b.stride(-2) == lda and \
+            (b.data_ptr() - a.data_ptr()) % es == 0:
+        d = (b.data_ptr() - a.data_ptr()) // es % lda
+        return not (d >= a.shape[-1] and lda - d >= b.shape[-1])
+    return True
 
 
 def embedding(ids, table, scale=1.0, out=None):
@@ -1109,7 +1132,7 @@ def embedding(ids, table, scale=1.0, out=None):
         out = table.new_empty((*ids.shape, E))
         ldo = E
     else:
-        ldo = _out_rows(out, (*ids.shape, E), table, "embedding")
+        ldo = _out_rows(out, (*ids.shape, E), table, "embedding", table)
     T = ids.numel()
     if T == 0 or E == 0:
         return out
@@ -1147,7 +1170,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
         out = dout.new_empty((vocab, E))
         ldo = E
     else:
-        ldo = _out_rows(out, (vocab, E), dout, "embedding_bwd")
+        ldo = _out_rows(out, (vocab, E), dout, "embedding_bwd", dout)
     if vocab == 0 or E == 0:
         return out
     d, T, ldd = _row_view(dout, "embedding_bwd")
@@ -1249,12 +1272,12 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     bf16 = _float_type(x, "linear_w4.x")
     if x.dim() < 1 or x.shape[-1] != K:
         raise _lib.DasaError(f"linear_w4: x {tuple(x.shape)} does not end in K = {K}")
-    if b is not None and (b.dtype != torch.float32 or tuple(b.shape) != (N,) or (N > 1 and b.stride(0) != 1)):
+    if b is not None and (b.dtype != torch.float32 or b.shape != (N,) or (N > 1 and b.stride(0) != 1)):
         raise _lib.DasaError(f"linear_w4: the bias must be a contiguous float32 [{N}]")
     if act not in _ACT_IDS:
         raise _lib.DasaError(f"linear_w4: unknown activation {act!r}")
     dev = _on_device("linear_w4", x, w.tiles, b, out)
-    if torch.is_grad_enabled() and (x.requires_grad or (b is not None and b.requires_grad)):
+    if (x.requires_grad or (b is not None and b.requires_grad)) and torch.is_grad_enabled():
         raise _lib.DasaError("linear_w4 is forward only: call it under torch.no_grad()")
     shape = (*x.shape[:-1], N)
     if out is None:
@@ -1263,7 +1286,7 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
         out = x.new_empty(shape)
         ldo = N
     else:
-        ldo = _out_rows(out, shape, x, "linear_w4")
+        ldo = _out_rows(out, shape, x, "linear_w4", x, b)
     x2, M, ldx = _row_view(x, "linear_w4")
     if M == 0:
         return out
@@ -1277,14 +1300,15 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     return out
 
 
-def _penalty(v, B, what, neutral):
+def _penalty(v, B, dev, what, neutral):
     """(device pointer or None, number) of a penalty given as None, a number or a float32 [B] tensor."""
     if v is None:
         return None, neutral
     if isinstance(v, torch.Tensor):
-        if v.dtype != torch.float32 or v.dim() != 1 or v.shape[0] != B or (B > 1 and v.stride(0) != 1):
+        if v.dtype != torch.float32 or v.shape != (B,) or (B > 1 and v.stride(0) != 1):
             raise _lib.DasaError(f"logit_rules: {what} must be a number or a contiguous float32 [{B}]")
-        _on_device("logit_rules", v)
+        if v.get_device() != dev:
+            _on_device("logit_rules", v)
         return v.data_ptr(), neutral
     v = float(v)
     if not math.isfinite(v) or (what == "repetition" and v <= 0.0):
@@ -1310,7 +1334,7 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     dev = _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
     if V == 0 or B > 65535:
         raise _lib.DasaError(f"logit_rules: logits {tuple(logits.shape)}: 1 token at least, 65535 rows at most")
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if logits.requires_grad and torch.is_grad_enabled():
         raise _lib.DasaError("logit_rules is forward only: call it under torch.no_grad()")
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         raise _lib.DasaError("logit_rules: the rows of logits must be contiguous")
@@ -1323,17 +1347,20 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
         if hlen and B:
             history, _, ldh = _row_view(history, "logit_rules")
             hist = history.data_ptr()
+    nlen = None
     if lengths is not None:
-        if history is None or lengths.dim() != 1 or lengths.shape[0] != B or \
-                lengths.dtype not in (torch.int32, torch.int64):
+        if history is None or lengths.shape != (B,) or lengths.dtype not in _ID_BYTES:
             raise _lib.DasaError(f"logit_rules: lengths must be int32 [{B}] and go with a history")
-        lengths = lengths.to(torch.int32).contiguous()
-    r, r0 = _penalty(repetition, B, "repetition", 1.0)
-    p, p0 = _penalty(presence, B, "presence", 0.0)
-    f, f0 = _penalty(frequency, B, "frequency", 0.0)
+        if lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, hlen).to(torch.int32)
+        lengths = lengths.contiguous()
+        nlen = lengths.data_ptr()
+    r, r0 = _penalty(repetition, B, dev, "repetition", 1.0)
+    p, p0 = _penalty(presence, B, dev, "presence", 0.0)
+    f, f0 = _penalty(frequency, B, dev, "frequency", 0.0)
     ldb = 0
     if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) not in ((V,), (B, V)):
+        if bias.dtype != torch.float32 or (bias.shape != (V,) and bias.shape != (B, V)):
             raise _lib.DasaError(f"logit_rules: bias must be float32 [{V}] or [{B}, {V}]")
         bias = bias.contiguous()
         ldb = V if bias.dim() == 2 else 0
@@ -1342,18 +1369,20 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     if allowed is not None:
         words = allowed.dtype == torch.int32
         n = -(-V // 32) if words else V
-        if not (words or allowed.dtype in (torch.bool, torch.uint8)) or tuple(allowed.shape) not in ((n,), (B, n)):
+        if not (words or allowed.dtype in (torch.bool, torch.uint8)) or \
+                (allowed.shape != (n,) and allowed.shape != (B, n)):
             raise _lib.DasaError(f"logit_rules: allowed must be bool / uint8 [{V}] or [{B}, {V}], or int32 words "
                                  f"[{-(-V // 32)}] or [{B}, {-(-V // 32)}]")
         allowed = allowed.contiguous()
         ldw = n if allowed.dim() == 2 else 0
         bits, byts = (allowed.data_ptr(), None) if words else (None, allowed.data_ptr())
     if out is None:
-        out = logits.new_empty((B, V))
+        out = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty((B, V))
         ldo = V
     else:
-        ldo = _out_rows(out, (B, V), logits, "logit_rules")
-    choice = logits.new_empty((B,), dtype=torch.int64) if want_choice else None
+        same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
+        ldo = _out_rows(out, (B, V), logits, "logit_rules", None if same else logits, bias)
+    choice = torch.empty(B, dtype=torch.int64, device=logits.device) if want_choice else None
     if B:
         L = _lib.lib()
         ws, nws = None, 0
@@ -1362,7 +1391,7 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
             if nws:
                 ws = torch.empty(nws // 8, dtype=torch.int64, device=logits.device)
         d = _lib.LogitRules(logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), ldo, hist, ldh,
-                            None if lengths is None else lengths.data_ptr(), r, p, f,
+                            nlen, r, p, f,
                             None if bias is None else bias.data_ptr(), ldb, bits, ldw, byts, ldw,
                             None if choice is None else choice.data_ptr(), r0, p0, f0, B, V, hlen, nid, bf16)
         _call("dasa_logit_rules", "logit_rules", L.dasa_logit_rules, ctypes.byref(d),

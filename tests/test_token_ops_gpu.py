@@ -494,3 +494,66 @@ def test_word_step_captured_and_on_another_stream(dev):
         for (gr, s, out, grad, st), w in zip(graphs, want):
             for a, b in zip((*out, grad), w):
                 assert torch.equal(a, b)
+
+
+def test_outputs_that_overlap_an_input_are_refused(dev):
+    """out may not share bytes with what the call reads (but logit_rules works in place, and column blocks of one
+    buffer are apart)."""
+    buf = torch.randn(6, 64, device=dev)
+    w = ops.quantize_w4(torch.randn(20, 32, device=dev), 32)
+    want = ops.linear_w4(buf[:, :32].contiguous(), w)
+    got = ops.linear_w4(buf[:, :32], w, out=buf[:, 32:52])
+    assert torch.equal(got, want)
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.linear_w4(buf[:, :32], w, out=buf[:, 31:51])
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.linear_w4(buf[:, 40:], ops.quantize_w4(torch.randn(24, 24, device=dev), 32), out=buf[:, 30:54])
+    x = torch.randn(6, 30, device=dev)
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.logit_rules(x[:5], out=x[1:])
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.logit_rules(x[:, :20], out=x[:, 5:25])
+    assert torch.equal(ops.logit_rules(x[:, :15], out=x[:, 15:]), x[:, :15])
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.embedding(torch.tensor([1, 2], device=dev), x, out=x[:2])
+    with pytest.raises(DasaError, match="overlaps"):
+        ops.embedding_bwd(x, torch.arange(6, device=dev), 6, out=x)
+    with pytest.raises(DasaError, match="rows of out"):
+        ops.embedding(torch.tensor([1, 2], device=dev), x, out=torch.empty(30, device=dev).expand(2, 30))
+
+
+def test_refusals_on_the_device(dev):
+    x = torch.randn(3, 40, device=dev)
+    h = torch.zeros(3, 5, dtype=torch.int64, device=dev)
+    for bad in (dict(history=h[:2]), dict(history=h.float()), dict(lengths=h[:, 0]), dict(repetition=0.0),
+                dict(repetition=float("nan")), dict(presence=float("inf")), dict(frequency=torch.ones(2, device=dev)),
+                dict(repetition=torch.ones(3, device=dev, dtype=torch.float64)), dict(bias=torch.ones(3, device=dev)),
+                dict(bias=torch.ones(40, device=dev, dtype=BF16)), dict(allowed=torch.ones(40, device=dev)),
+                dict(allowed=torch.ones(41, device=dev, dtype=torch.bool)),
+                dict(allowed=torch.ones(40, device=dev, dtype=torch.int32)), dict(out=torch.empty(3, 41, device=dev)),
+                dict(out=torch.empty(3, 40, device=dev, dtype=BF16)), dict(history=h, lengths=h[:2, 0]),
+                dict(history=h, lengths=torch.ones(3, device=dev)), dict(bias=torch.ones(40)), dict(repetition=torch.ones(3))):
+        with pytest.raises(DasaError):
+            ops.logit_rules(x, **bad)
+    with pytest.raises(DasaError, match="rows of logits"):
+        ops.logit_rules(x.t())
+    with pytest.raises(DasaError, match="forward only"):
+        ops.logit_rules(x.clone().requires_grad_())
+    with pytest.raises(DasaError, match="token at least"):
+        ops.logit_rules(torch.empty(3, 0, device=dev))
+    w = ops.quantize_w4(torch.randn(20, 40, device=dev), 32)
+    for bad in (dict(b=torch.ones(19, device=dev)), dict(b=torch.ones(20)), dict(beta=1.0), dict(act="swish"),
+                dict(out=torch.empty(3, 21, device=dev)), dict(out=torch.empty(3, 20, device=dev, dtype=BF16))):
+        with pytest.raises(DasaError):
+            ops.linear_w4(x, w, **bad)
+    with pytest.raises(DasaError, match="forward only"):
+        ops.linear_w4(x.clone().requires_grad_(), w)
+    d = torch.randn(3, 5, 8, device=dev)
+    for a, k in (((d[:2], h, 10), {}), ((d, h, 10), dict(padding_idx=10)), ((d, h, 10), dict(accumulate=True)),
+                 ((d, h, 10), dict(out=torch.empty(10, 9, device=dev))), ((d, h, -1), {}), ((d, h.float(), 10), {})):
+        with pytest.raises(DasaError):
+            ops.embedding_bwd(*a, **k)
+    with pytest.raises(DasaError, match="no rows"):
+        ops.embedding(h, torch.empty(0, 8, device=dev))
+    with pytest.raises(DasaError, match="rows must be contiguous"):
+        ops.embedding(h, torch.randn(8, 10, device=dev).t())
