@@ -137,11 +137,9 @@ struct SortArgs {
   int* order;     // [T] positions in sorted order
 };
 
-// The ids of a step as 32-bit tokens: 2^32 - 1, which no vocabulary holds, for an id outside 32 bits.
-__device__ __forceinline__ unsigned low(uint2 v) { return v.x; }
-__device__ __forceinline__ unsigned low(unsigned v) { return v; }
-__device__ __forceinline__ unsigned high(uint2 v) { return v.y; }
-__device__ __forceinline__ unsigned high(unsigned) { return 0; }
+// An id as a 32-bit token: 2^32 - 1, which no vocabulary holds, for an id outside 32 bits.
+__device__ __forceinline__ unsigned token(uint2 v) { return v.y == 0 ? v.x : ~0u; }
+__device__ __forceinline__ unsigned token(unsigned v) { return v; }
 
 // f(position, token) for the ids [t0, t1) of a wave, 64 at a time, U loads in flight (and U more of the next group);
 // f is called by whole waves
@@ -157,27 +155,16 @@ __device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lan
       const W* p = ids + min(t + 64 * U, last) + lane;      // the next group, or the last again
 #pragma unroll
       for (int k = 0; k < U; ++k) next[k] = p[64 * k];
-      unsigned hi = 0;
 #pragma unroll
-      for (int k = 0; k < U; ++k) hi |= high(v[k]);
-      if (__builtin_amdgcn_ballot_w64(hi != 0) == 0) {
-#pragma unroll
-        for (int k = 0; k < U; ++k) f(t + 64 * k + lane, low(v[k]));
-      } else {
-#pragma unroll 1
-        for (int k = 0; k < U; ++k) {
-          const W x = ids[t + lane + 64 * k];
-          f(t + 64 * k + lane, high(x) ? ~0u : low(x));
-        }
-      }
+      for (int k = 0; k < U; ++k) f(t + 64 * k + lane, token(v[k]));
 #pragma unroll
       for (int k = 0; k < U; ++k) v[k] = next[k];
     }
   }
 #pragma unroll 1
   for (; t < t1; t += 64) {
-    const W x = ids[min(t + lane, t1 - 1)];
-    f(t + lane, high(x) || t + lane >= t1 ? ~0u : low(x));
+    const unsigned u = token(ids[min(t + lane, t1 - 1)]);
+    f(t + lane, t + lane < t1 ? u : ~0u);
   }
 }
 

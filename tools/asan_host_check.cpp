@@ -146,6 +146,53 @@ int main() {
   expect(dasa_gather_rows(fp(0x10), nullptr, 6, nullptr, nullptr, 0, fp(0x20), 4, nullptr) == kInval,
          "gather Fa % 4", 6);
   expect(dasa_f32_split3_bf16(fp(0x10), 12, nullptr, 4, 12, nullptr) != 0, "split3 cols % 8", 12);
+
+  // ---- token operators: workspace sizing and validation before any launch ----
+  for (int T : {0, 1, 64, 1600, 8192, 8193, 131072, 1 << 30})
+    for (int V : {1, 992, 30522, 300000})
+      for (int E : {1, 257, 768, 4096}) {
+        const int64_t ws = dasa_embedding_bwd_workspace(T, V, E);
+        expect(T <= 8192 ? ws == 0 : ws >= 4LL * (T + V + 1), "dasa_embedding_bwd_workspace", T);
+      }
+  expect(dasa_embedding_bwd_workspace(1LL << 31, 10, 8) == 0, "embedding T >= 2^31", 0);
+  expect(dasa_embedding_fwd(fp(0x1000), 7, fp(0x2000), 8, 4, 10, 8, 1.f, 0, fp(0x3000), 8, nullptr, nullptr) == kInval,
+         "embedding ldt < E", 7);
+  expect(dasa_embedding_fwd(fp(0x1000), 8, fp(0x2000), 3, 4, 10, 8, 1.f, 0, fp(0x3000), 8, nullptr, nullptr) == kInval,
+         "embedding id bytes", 3);
+  expect(dasa_embedding_bwd(fp(0x1000), 8, fp(0x2000), 8, 9000, 10, 8, 1.f, -1, 0, fp(0x3000), 8, 0, nullptr, 0,
+                            nullptr) == kInval, "embedding gradient without workspace", 9000);
+  for (int M : {1, 16, 17, 33, 64, 150})
+    for (int N : {1, 992, 4096, 30522, 65536})
+      for (int K : {1, 128, 2240, 8192})
+        for (int bf : {0, 1}) {
+          const int64_t ws = dasa_gemm_w4_workspace(M, N, K, bf);
+          expect(ws >= 0 && ws % 1024 == 0, "dasa_gemm_w4_workspace", M);
+          expect(dasa_w4_weight_bytes(N, K) >= (int64_t)N * K / 2, "dasa_w4_weight_bytes", N);
+          if (ws > 0)
+            expect(dasa_gemm_w4(fp(0x1000), K, bf, fp(0x2000), fp(0x3000), 0, 64, nullptr, 0, 0.f, fp(0x4000), N, M, N, K,
+                                nullptr, 0, nullptr) == kInval, "gemm_w4 without workspace", M);
+        }
+  expect(dasa_gemm_w4(fp(0x1000), 63, 0, fp(0x2000), fp(0x3000), 0, 64, nullptr, 0, 0.f, fp(0x4000), 16, 1, 16, 64,
+                      nullptr, 0, nullptr) == kInval, "gemm_w4 ldx < K", 63);
+  expect(dasa_gemm_w4(fp(0x1000), 64, 0, fp(0x2000), fp(0x3000), 0, 48, nullptr, 0, 0.f, fp(0x4000), 16, 1, 16, 64,
+                      nullptr, 0, nullptr) == kInval, "gemm_w4 group", 48);
+  expect(dasa_w4_quantize(fp(0x1000), 63, 0, 4, 64, 64, (uint8_t*)fp(0x2000), 32, fp(0x3000), 1, 0, nullptr) == kInval,
+         "w4_quantize ldw < K", 63);
+  expect(dasa_w4_layout((uint8_t*)fp(0x1000), 31, fp(0x2000), 1, 0, 4, 64, 64, fp(0x3000), fp(0x4000), nullptr) == kInval,
+         "w4_layout ldc", 31);
+  for (int B : {1, 20, 64, 65535})
+    for (int V : {1, 992, 8192, 8193, 30522, 300000}) {
+      const int64_t ws = dasa_logit_rules_workspace(B, V);
+      expect(V <= 8192 ? ws == 0 : ws >= 16LL * B, "dasa_logit_rules_workspace", V);
+    }
+  dasa_logit_rules_desc rd;
+  std::memset(&rd, 0, sizeof(rd));
+  rd.B = 2; rd.V = 100; rd.logits = fp(0x1000); rd.out = fp(0x2000); rd.ld = 99; rd.ldo = 100;
+  expect(dasa_logit_rules(&rd, nullptr, 0, nullptr) == kInval, "logit_rules ld < V", 99);
+  rd.ld = 100; rd.history = fp(0x3000); rd.L = 4; rd.ldh = 3; rd.ids_bytes = 8;
+  expect(dasa_logit_rules(&rd, nullptr, 0, nullptr) == kInval, "logit_rules ldh < L", 3);
+  expect(dasa_logit_rules(nullptr, nullptr, 0, nullptr) == kInval, "logit_rules NULL", 0);
+
   expect(dasa_set_error_word(nullptr) == 0, "dasa_set_error_word(NULL)", 0);
   expect(dasa_persist_force_timeout(0) == 0, "dasa_persist_force_timeout", 0);
   expect(dasa_set_seed_source(nullptr) == 0, "dasa_set_seed_source(NULL)", 0);
