@@ -6,13 +6,26 @@
 // Used by the word lookup of SpeakerDecoder (model.py:1061) and the word-embedding gradient of BertEmbeddings
 // (vilmodel.py:161-176 under autograd).
 //
+// Lookup: bound by HBM (ids + one row read and one written a token); no arithmetic to speak of. 131072 rows of 1024
+// bf16 from a table of 50021: 75.6 us, 268 MB written and 102 MB of table read at least: 4.9 TB/s, a large copy's 5.2.
+//
 // The gradient is deterministic: the rows of one token are summed in fp32 in the order of their positions, so there
-// is no float atomic. The order comes from a one-launch sort: workgroup g owns the vocabulary range
-// [g R, (g + 1) R), reads every id (T x 8 B, an L2-resident list), counts its own range's tokens per wave
-// segment and the tokens below the range (its base), and writes its tokens' positions at their stable rank. No
-// workgroup waits for another.
+// is no float atomic, and every table row is written once, in its type. What it has to move is dout once and the table
+// once; the sort that gives the order comes on top, so the sort keeps to few launches and small lists:
+//   T <= 8192      one launch: each workgroup sorts its vocabulary range into LDS and sums its rows.
+//                  (1600 x 768 fp32 into 30522 rows: 20.2 us; the table's 94 MB alone take a fill kernel 13.6.)
+//   T <  49152     token_sort_kernel, rows, join. Workgroup g of the sort owns the range [g R, (g + 1) R), reads every
+//                  id (T x 8 B, an L2-resident list), counts its own tokens per wave segment and the tokens below the
+//                  range (its base), and writes its tokens' positions at their stable rank. No workgroup waits for
+//                  another.
+//   above          token_count_kernel, token_place_kernel, rows, join: reading every id in every workgroup is what
+//                  bounds the one-launch sort there.
+//                  (131072 x 1024 bf16, a third of them padding, into 50021 rows: 7.1 + 16.2 us sort, 73.5 rows
+//                  (174 MB read, 102 MB written: 3.8 TB/s; a large sum reads at 4.0), 8.6 join.)
 #include "common.h"
 #include "../../include/dasa_hip.h"
+
+#include <algorithm>
 
 namespace {
 
@@ -183,6 +196,58 @@ __device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, 
   }
 }
 
+// f(position, bin, in, lanes with `in`) for the steps of a wave that hold a token of the range [lo, lo + n)
+template <class W, class F>
+__device__ __forceinline__ void each_in_range(const W* ids, int t0, int t1, int lane, unsigned lo, unsigned n,
+                                              unsigned pad, F f) {
+  each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {
+    const unsigned bin = u - lo;
+    const bool in = bin < n && u != pad;
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
+    if (m) f(pos, (int)bin, in, m);
+  });
+}
+
+// hist[bin] += 1 for the lanes of m; PACK: two bins of 16 bits a word
+template <bool PACK>
+__device__ __forceinline__ void add_bins(int* hist, int bin, bool in, unsigned long long m) {
+  auto add = [&](int b, int c) { atomicAdd(&hist[PACK ? b >> 1 : b], PACK ? c << (16 * (b & 1)) : c); };
+  if (__popcll(m) <= 8) {
+    if (in) add(bin, 1);
+    return;
+  }
+  const int lane = threadIdx.x & 63;               // dense: a frequent id would be one address for most lanes
+  while (m) {
+    const int lead = __builtin_ctzll(m), b = __builtin_amdgcn_readlane(bin, lead);
+    const unsigned long long same = __builtin_amdgcn_ballot_w64(in && bin == b);
+    if (lane == lead) add(b, (int)__popcll(same));
+    m &= ~same;
+  }
+}
+
+// inclusive sum over the workgroup's threads; wsum holds one int a wave
+__device__ __forceinline__ int block_scan(int v, int* wsum) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  if (lane == 63) wsum[w] = v;
+  __syncthreads();
+  for (int k = 0; k < w; ++k) v += wsum[k];
+  return v;
+}
+
+// the wave's part of [t0, t1): multiples of 64 tokens
+__device__ __forceinline__ void wave_part(int& t0, int& t1, int w) {
+  const int part = (((t1 - t0 + kSortWaves - 1) / kSortWaves) + 63) & ~63;
+  const int b = min(t0 + w * part, t1);
+  t1 = min(b + part, t1);
+  t0 = b;
+}
+
+// One launch: a workgroup's base is the number of tokens below its range, which it counts on the way.
 template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a) {
   extern __shared__ int lpos[];                    // [waves][kList] positions, [waves][R] counts (then write
@@ -194,33 +259,23 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
   for (int i = tid; i < kSortWaves * a.R; i += 64 * kSortWaves) hist[i] = 0;
   __syncthreads();
-  const int seg = (((a.T + kSortWaves - 1) / kSortWaves) + 63) & ~63;
-  const int t0 = min(w * seg, a.T), t1 = min(t0 + seg, a.T);
+  int t0 = 0, t1 = a.T;
+  wave_part(t0, t1, w);
   int* mine = hist + w * a.R;
   int nb = 0, found = 0;
   each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {
     nb += __popcll(__builtin_amdgcn_ballot_w64(u < lo && u != a.pad));
     const unsigned bin = u - lo;
     const bool in = bin < n && u != a.pad;
-    unsigned long long m = __builtin_amdgcn_ballot_w64(in);
+    const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     const int at = found + __popcll(m & ((1ull << lane) - 1));
     if (in && at < kList) {
       lpos[w * kList + at] = pos;
       lbin[w * kList + at] = (unsigned short)bin;
     }
-    const int c = __popcll(m);
-    found += c;
-    if (c <= 8) {
-      if (in) atomicAdd(&mine[bin], 1);
-    } else {                                       // dense: a frequent id would be one address for most lanes
-      while (m) {
-        const int b = __builtin_amdgcn_readlane((int)bin, __builtin_ctzll(m));
-        const unsigned long long same = __builtin_amdgcn_ballot_w64(in && (int)bin == b);
-        mine[b] += __popcll(same);                 // every lane stores the same value
-        m &= ~same;
-      }
-    }
+    found += __popcll(m);
+    add_bins<false>(mine, (int)bin, in, m);
   });
   if (lane == 0) below[w] = nb;
   __syncthreads();
@@ -228,17 +283,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
   int tot = 0;
   if (tid < (int)n)
     for (int k = 0; k < kSortWaves; ++k) tot += hist[k * a.R + tid];
-  int incl = tot;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 63) wsum[w] = incl;
-  __syncthreads();
-  int base = 0;
-  for (int k = 0; k < kSortWaves; ++k) base += below[k] + (k < w ? wsum[k] : 0);
-  int at = base + incl - tot;
+  int at = block_scan(tot, wsum) - tot;
+  for (int k = 0; k < kSortWaves; ++k) at += below[k];
   if (tid < (int)n) {
     a.start[lo + tid] = at;
     for (int k = 0; k < kSortWaves; ++k) {
@@ -256,9 +302,183 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
     }
     return;
   }
-  each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {      // a hot range: its ids again
-    place(mine, a.order, lane, u - lo < n && u != a.pad, (int)(u - lo), pos);
+  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long) {
+    place(mine, a.order, lane, in, bin, pos);      // a hot range: its ids again
   });
+}
+
+// Two launches for many tokens: workgroup = (wider range, segment of the tokens). The first counts its ids; the second
+// adds up what lies before each of its ids (smaller ids, and the same id in earlier segments) and places its tokens.
+constexpr int kWideRange = 1600;
+constexpr int kSegmentTokens = 65024;              // of a segment at most: counts and offsets within it fit 16 bits
+
+struct SplitArgs {
+  int ranges, segments;
+  int* counts;     // [segments][V]
+  int* totals;     // [ranges][segments]
+};
+
+__device__ __forceinline__ void segment_of(int T, int segments, int& t0, int& t1) {
+  const int seg = (((T + segments - 1) / segments) + 63) & ~63;
+  t0 = (int)min((long)blockIdx.y * seg, (long)T);
+  t1 = (int)min((long)t0 + seg, (long)T);
+}
+
+template <class W>
+__global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(SortArgs a, SplitArgs p) {
+  __shared__ int hist[kWideRange];
+  __shared__ int found[kSortWaves];
+  const W* ids = reinterpret_cast<const W*>(a.ids);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
+  for (int i = tid; i < (int)n; i += 64 * kSortWaves) hist[i] = 0;
+  __syncthreads();
+  int t0, t1, total = 0;
+  segment_of(a.T, p.segments, t0, t1);
+  wave_part(t0, t1, w);
+  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int, int bin, bool in, unsigned long long m) {
+    total += __popcll(m);
+    add_bins<false>(hist, bin, in, m);
+  });
+  if (lane == 0) found[w] = total;
+  __syncthreads();
+  for (int i = tid; i < (int)n; i += 64 * kSortWaves) p.counts[(long)blockIdx.y * a.V + lo + i] = hist[i];
+  if (tid == 0) {
+    for (int k = 1; k < kSortWaves; ++k) total += found[k];
+    p.totals[blockIdx.x * p.segments + blockIdx.y] = total;
+  }
+}
+
+template <class W>
+__global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a, SplitArgs p) {
+  // a wave's counts, later its offset into an id's run: two ids of 16 bits a word
+  __shared__ int count[kSortWaves][kWideRange / 2];
+  __shared__ int first[kWideRange];                // where an id's tokens of this segment begin
+  extern __shared__ int lpos[];                    // [waves][kList] positions, [waves][kList] bins
+  unsigned short* const lbin = reinterpret_cast<unsigned short*>(lpos + kSortWaves * kList);
+  __shared__ int wsum[kSortWaves], wbase[kSortWaves];
+  const W* ids = reinterpret_cast<const W*>(a.ids);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
+  for (int i = tid; i < kSortWaves * kWideRange / 2; i += 64 * kSortWaves) count[0][i] = 0;
+  // thread = two ids: all their tokens, those of the earlier segments, and the tokens of smaller ranges (asked for
+  // before the scan, which hides them)
+  constexpr int PER = (kWideRange + 64 * kSortWaves - 1) / (64 * kSortWaves);
+  static_assert(PER == 2, "two ids share a counter word");
+  int all[PER] = {0, 0}, before[PER] = {0, 0}, base = 0;
+  for (int k = 0; k < p.segments; ++k) {
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      const int b = tid * PER + q;
+      const int c = b < (int)n ? p.counts[(long)k * a.V + lo + b] : 0;
+      all[q] += c;
+      before[q] += k < (int)blockIdx.y ? c : 0;
+    }
+  }
+  for (int i = tid; i < (int)blockIdx.x * p.segments; i += 64 * kSortWaves) base += p.totals[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) base += __shfl_xor(base, o, 64);
+  if (lane == 0) wbase[w] = base;
+  __syncthreads();
+  int t0, t1, found = 0;
+  segment_of(a.T, p.segments, t0, t1);
+  wave_part(t0, t1, w);
+  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long m) {
+    const int at = found + __popcll(m & ((1ull << lane) - 1));
+    if (in && at < kList) {
+      lpos[w * kList + at] = pos;
+      lbin[w * kList + at] = (unsigned short)bin;
+    }
+    found += __popcll(m);
+    add_bins<true>(count[w], bin, in, m);
+  });
+  int at = block_scan(all[0] + all[1], wsum) - all[0] - all[1];      // (its barrier also ends the counting)
+  for (int k = 0; k < kSortWaves; ++k) at += wbase[k];
+  if (tid * PER < (int)n) {
+    const int second = at + all[0];
+    first[tid * PER] = at + before[0];
+    first[tid * PER + 1] = second + before[1];
+    if (blockIdx.y == 0) {
+      const int v = (int)lo + tid * PER;
+      a.start[v] = at;
+      if (v == a.V - 1) a.start[a.V] = second;
+      if (tid * PER + 1 < (int)n) {
+        a.start[v + 1] = second;
+        if (v + 1 == a.V - 1) a.start[a.V] = second + all[1];
+      }
+    }
+    int c[kSortWaves], run = 0;
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) c[k] = count[k][tid];
+#pragma unroll
+    for (int k = 0; k < kSortWaves; ++k) {
+      count[k][tid] = run;
+      run += c[k];
+    }
+  }
+  __syncthreads();
+  auto put = [&](bool in, int bin, int pos) {        // place(), with the packed cursors
+    unsigned long long m = __builtin_amdgcn_ballot_w64(in);
+    while (m) {
+      const int b = __builtin_amdgcn_readlane(bin, __builtin_ctzll(m)), sh = 16 * (b & 1);
+      const unsigned long long same = __builtin_amdgcn_ballot_w64(in && bin == b);
+      const int word = count[w][b >> 1];
+      if ((same >> lane) & 1) a.order[first[b] + ((word >> sh) & 0xffff) + __popcll(same & ((1ull << lane) - 1))] = pos;
+      count[w][b >> 1] = word + (__popcll(same) << sh);                  // every lane stores the same value
+      m &= ~same;
+    }
+  };
+  if (found <= kList) {
+    for (int i = 0; i < found; i += 64) {
+      const int j = min(i + lane, found - 1);
+      put(i + lane < found, lbin[w * kList + j], lpos[w * kList + j]);
+    }
+    return;
+  }
+  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long) {
+    put(in, bin, pos);
+  });
+}
+
+inline int sort_ranges(int V) {
+  const int need = (V + kWideRange - 1) / kWideRange, most = V < 32 ? V : 32;
+  return need > most ? need : most;
+}
+// One launch against two, 50021 ids, Zipf / uniform / one id: 49152 tokens x 64 bf16, the whole gradient, 34.4 / 28.9 /
+// 64.7 us against 33.6 / 30.8 / 45.3; 131072 tokens, the sort alone, 39 / 30 / 72 against 27.5 / 27.9 / 25.5. Above
+// 4 M tokens the counts of the segments would outgrow the tokens.
+constexpr long kManyTokens = 49152, kMostTokens = 4 << 20;
+
+inline bool split_sort(int64_t T) { return T >= kManyTokens && T <= kMostTokens; }
+inline int sort_segments(int64_t T) { return (int)std::max<int64_t>(8, (T + kSegmentTokens - 1) / kSegmentTokens); }
+
+inline int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
+
+template <class W>
+int launch_sort(SortArgs a, void* split, hipStream_t st) {
+  const dim3 block(64 * kSortWaves);
+  if (split_sort(a.T)) {
+    SplitArgs p;
+    p.segments = sort_segments(a.T);
+    p.ranges = sort_ranges(a.V);
+    a.R = (a.V + p.ranges - 1) / p.ranges;
+    p.ranges = (a.V + a.R - 1) / a.R;
+    p.counts = reinterpret_cast<int*>(split);
+    p.totals = p.counts + (long)p.segments * a.V;
+    const dim3 grid(p.ranges, p.segments);
+    hipLaunchKernelGGL(token_count_kernel<W>, grid, block, 0, st, a, p);
+    DASA_CHECK_LAUNCH();
+    hipLaunchKernelGGL(token_place_kernel<W>, grid, block, (size_t)kSortWaves * kList * 6, st, a, p);
+    DASA_CHECK_LAUNCH();
+    return 0;
+  }
+  int G = (a.V + kMaxRange - 1) / kMaxRange;
+  if (G < 256) G = a.V < 256 ? a.V : 256;
+  a.R = (a.V + G - 1) / G;
+  G = (a.V + a.R - 1) / a.R;
+  hipLaunchKernelGGL(token_sort_kernel<W>, dim3(G), block, (size_t)kSortWaves * (a.R * 4 + kList * 6), st, a);
+  DASA_CHECK_LAUNCH();
+  return 0;
 }
 
 // ------------------------------------------------------------------ gradient rows
@@ -579,7 +799,6 @@ int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
   return 0;
 }
 
-inline int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
 }  // namespace
 
@@ -598,7 +817,8 @@ extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* id
 extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E) {
   if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0) return 0;
   const int64_t chunks = (T + kChunk - 1) / kChunk;
-  return round16(((int64_t)V + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4;
+  const int64_t split = split_sort(T) ? ((int64_t)V + sort_ranges(V)) * sort_segments(T) * 4 : 0;
+  return round16(((int64_t)V + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4 + split;
 }
 
 extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t ids_bytes, int64_t T,
@@ -622,13 +842,8 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   ba.order = sa.order = order;
   ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
   ba.ldp = part_stride(E, bf16);
-  int G = (V + kMaxRange - 1) / kMaxRange;
-  if (G < 256) G = V < 256 ? V : 256;
-  sa.R = (V + G - 1) / G;
-  G = (V + sa.R - 1) / sa.R;
-  const size_t lds = (size_t)kSortWaves * (sa.R * 4 + kList * 6);
-  if (ids_bytes == 8) hipLaunchKernelGGL(token_sort_kernel<uint2>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
-  else hipLaunchKernelGGL(token_sort_kernel<unsigned>, dim3(G), dim3(64 * kSortWaves), lds, st, sa);
-  DASA_CHECK_LAUNCH();
+  void* split = ba.parts + (T + kChunk - 1) / kChunk * 2 * part_stride(E, 1);
+  const int rc = ids_bytes == 8 ? launch_sort<uint2>(sa, split, st) : launch_sort<unsigned>(sa, split, st);
+  if (rc) return rc;
   return bf16 ? launch_rows<__bf16>(ba, T, st) : launch_rows<float>(ba, T, st);
 }

@@ -98,7 +98,9 @@ def _check_bwd(got, dout, ids, V, scale, pad, dtype, what, old=None):
                                         (1600, 30522, 768, "zipf"), (4099, 1001, 257, "zipf"), (5000, 17, 16, "zipf"),
                                         (20000, 100, 256, "zipf"), (20001, 999, 72, "one"), (8192, 8192, 40, "perm"),
                                         (130, 300000, 8, "uniform"), (9000, 300000, 16, "zipf"),
-                                        (8193, 2, 8, "uniform"), (33000, 40, 520, "zipf")])
+                                        (8193, 2, 8, "uniform"), (33000, 40, 520, "zipf"),
+                                        (49152, 2, 8, "uniform"), (60001, 3000, 16, "one"), (50001, 40, 72, "zipf"),
+                                        (131073, 300000, 8, "zipf"), (70000, 70000, 4, "perm")])
 def test_embedding_gradient(dev, dtype, T, V, E, kind):
     g = _gen(T * 3 + V + E)
     if kind == "uniform":
