@@ -12,6 +12,10 @@
 // counts the row's history into LDS while they come (integer atomics: the counts do not depend on their order), and
 // writes the slice. With one slice a row, the workgroup also makes the choice; else each slice leaves its best key
 // and a second launch takes the best of them, one wave a row.
+//
+// Bound by latency at a decoding step's sizes: 20 x 992 fp32 with 120 ids a row 4.4 us, where an empty kernel takes 2.4.
+// 64 x 30522 fp32, 1024 ids: 8.9 + 2.6 us (17 MB: 3.2 at a copy's rate); 16 x 128255 bf16 with a bias a row, 16384 ids:
+// 13.9 + 3.2 (18 MB: 3.5), half of it the history that every slice reads.
 #include "common.h"
 #include "../../include/dasa_hip.h"
 
@@ -187,7 +191,8 @@ struct Shape {
 };
 
 // One slice a row up to 8192 tokens (4 or 8 a thread). Else slices of 8 tokens a thread, as wide as still gives every
-// CU a workgroup (each reads the whole history).
+// CU a workgroup (each reads the whole history). One workgroup a row up to 32768 tokens saves the second launch and
+// loses more: 64 x 30522 fp32, 1024 ids, 16.5 us against 11.8.
 inline Shape shape_of(int B, int V) {
   auto threads = [&](int iter) { return (V + 256 * iter - 1) / (256 * iter) * 64; };
   if (V <= 4096) return {1, threads(1), 1};

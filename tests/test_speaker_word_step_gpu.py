@@ -47,8 +47,6 @@ def _record(spk):
     return seen
 
 
-
-
 def test_infer_batch_with_rules(dev):
     with _speaker() as spk:
         w2i, V = spk.tok.word_to_index, spk.tok.vocab_size()
@@ -127,9 +125,8 @@ def test_speaker_decoder_on_4bit_weights(dev):
         got = dec(words, ctx, mask, h, h)
         one = dec(words[:, :1], ctx, mask, h, h)[0]
         # the same step with the weights replaced by the values the codes stand for: equal up to the fp32 sums of the
-        # two products (K <= 1024 terms each, magnitudes below 0.1 sum |x w| = 30: 30 x 1024 x 2^-24 x 2 < 4e-3; the
-        # observed sums round far better, and the weights' own rounding, 0.5 / 7 of a group's largest, moves logits by
-        # more than 1e-2)
+        # two products (K <= 1024 terms each, magnitudes below 0.1 sum |x w| = 30: 30 x 1024 x 2^-24 x 2 < 4e-3); the
+        # weights' own rounding, up to 0.5 / 7 of a group's largest, moves the logits further than that
         q = {k: v[0].dequantize() for k, v in dec._w4.items()}
         dec.dequantize_w4()
         for k, W in dec._word_linears().items():

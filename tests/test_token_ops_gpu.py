@@ -100,7 +100,8 @@ def _check_bwd(got, dout, ids, V, scale, pad, dtype, what, old=None):
                                         (130, 300000, 8, "uniform"), (9000, 300000, 16, "zipf"),
                                         (8193, 2, 8, "uniform"), (33000, 40, 520, "zipf"),
                                         (49152, 2, 8, "uniform"), (60001, 3000, 16, "one"), (50001, 40, 72, "zipf"),
-                                        (131073, 300000, 8, "zipf"), (70000, 70000, 4, "perm")])
+                                        (131073, 300000, 8, "zipf"), (70000, 70000, 4, "perm"),
+                                        (2**22, 1000, 1, "zipf"), (2**22 + 1, 1000, 1, "zipf")])
 def test_embedding_gradient(dev, dtype, T, V, E, kind):
     g = _gen(T * 3 + V + E)
     if kind == "uniform":
@@ -181,6 +182,35 @@ def test_embedding_autograd(dev, dtype):
         e[7, 3] = 1.0
         f = lambda t: float(((t[ids.cpu()] * 2.0) * dout.cpu().double()).sum())   # noqa: E731
         assert abs((f(t64 + e) - f(t64 - e)) / 2 - float(table.grad[7, 3])) < 1e-4
+
+
+def test_embedding_in_a_captured_training_region(dev):
+    """Forward and backward replayed as graphs on new ids, with an eager graph of the same table alive: the gradients
+    are the eager ones, bit for bit."""
+    from dasa_amd import graph
+    g = _gen(21)
+    emb = torch.nn.Embedding(300, 64).to(dev)
+    region = graph.AutogradGraphs([emb])
+    link = torch.zeros(1, device=dev, requires_grad=True)        # (regions are linked by an input that trains)
+    fn = lambda ids, link: (DF.embedding(ids, emb.weight, scale=3.0, padding_idx=0) + link,)   # noqa: E731
+    for i in range(4):
+        region.new_iteration()
+        ids = torch.randint(0, 300, (5, 40), generator=g)
+        ids[:, 20 + 4 * i:] = 0
+        ids, dy = ids.to(dev), torch.randn(5, 40, 64, generator=g).to(dev)
+        eager = DF.embedding(ids, emb.weight, scale=3.0, padding_idx=0)
+        emb.weight.grad = link.grad = None
+        y, = region.run("rows", fn, (ids, link))
+        assert torch.equal(y, eager)
+        y.backward(dy)
+        got = emb.weight.grad.clone()
+        emb.weight.grad = None
+        eager.backward(dy)
+        assert torch.equal(got, emb.weight.grad)
+        _check_bwd(got, dy, ids, 300, 3.0, 0, F32, i)
+        with torch.no_grad():
+            emb.weight.add_(0.1)                                 # a step between the replays
+    assert region.captures == 1
 
 
 # ------------------------------------------------------------------------------------------ 4-bit weights
