@@ -12,12 +12,11 @@
 // The gradient is deterministic: the rows of one token are summed in fp32 in the order of their positions, so there
 // is no float atomic, and every table row is written once, in its type. What it has to move is dout once and the table
 // once; the sort that gives the order comes on top, so the sort keeps to few launches and small lists:
-//   T <= 8192      one launch: each workgroup sorts its vocabulary range into LDS and sums its rows.
+//   T <= 8192      one launch: each workgroup sorts its share of the ids into LDS and sums its rows.
 //                  (1600 x 768 fp32 into 30522 rows: 20.2 us; the table's 94 MB alone take a fill kernel 13.6.)
-//   T <  49152     token_sort_kernel, rows, join. Workgroup g of the sort owns the range [g R, (g + 1) R), reads every
-//                  id (T x 8 B, an L2-resident list), counts its own tokens per wave segment and the tokens below the
-//                  range (its base), and writes its tokens' positions at their stable rank. No workgroup waits for
-//                  another.
+//   T <  49152     token_sort_kernel, rows, join. A workgroup of the sort owns a share of the ids, reads every token
+//                  (T x 8 B, an L2-resident list), counts its own per wave segment and those of the shares before it
+//                  (its base), and writes its tokens' positions at their stable rank. No workgroup waits for another.
 //   above          token_count_kernel, token_place_kernel, rows, join: reading every id in every workgroup is what
 //                  bounds the one-launch sort there.
 //                  (131072 x 1024 bf16, a third of them padding, into 50021 rows: 7.1 + 16.2 us sort, 73.5 rows
@@ -32,7 +31,9 @@ namespace {
 constexpr unsigned kErrTokenId = 8;   // bit of the error word (ops._ERR_BITS)
 
 // 16 bytes of a row. Rows of odd width or stride start anywhere, so the vector types are element-aligned (global loads
-// and stores take any alignment); the last unit of a row may be partial.
+// and stores take any alignment). The last unit of a row that is no multiple of them ends at the row's end and repeats
+// columns of the unit before it: no lane takes a partial load of its own, whose branch holds the wave's other loads up
+// (gradient of 4099 x 257 fp32 into 1001 rows: 12.2 us against 15.8; lookup of 131072 x 1001 bf16: 98 against 111). NARROW: rows of less than one unit.
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
@@ -43,25 +44,26 @@ template <> struct Vec<__bf16> {
   typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-template <class T>
-__device__ __forceinline__ typename Vec<T>::type load_unit(const T* p, int left) {
+template <bool NARROW, class T>
+__device__ __forceinline__ typename Vec<T>::type load_unit(const T* p, int E) {
   typedef typename Vec<T>::type V;
-  if (left >= Vec<T>::N) return *reinterpret_cast<const V*>(p);
+  if constexpr (!NARROW) return *reinterpret_cast<const V*>(p);
   V v;
 #pragma unroll
-  for (int e = 0; e < Vec<T>::N; ++e) v[e] = e < left ? p[e] : (T)0.f;
+  for (int e = 0; e < Vec<T>::N; ++e) v[e] = e < E ? p[e] : (T)0.f;
   return v;
 }
 
-template <class T>
-__device__ __forceinline__ void store_unit(T* p, int left, typename Vec<T>::type v) {
+// columns from `skip` on
+template <bool NARROW, class T>
+__device__ __forceinline__ void store_unit(T* p, int E, int skip, typename Vec<T>::type v) {
   typedef typename Vec<T>::type V;
-  if (left >= Vec<T>::N) {
+  if (!NARROW && skip == 0) {
     *reinterpret_cast<V*>(p) = v;
   } else {
 #pragma unroll
     for (int e = 0; e < Vec<T>::N; ++e)
-      if (e < left) p[e] = v[e];
+      if (e >= skip && (!NARROW || e < E)) p[e] = v[e];
   }
 }
 
@@ -70,7 +72,7 @@ struct LookupArgs {
   const void* table; long ldt;
   const void* ids;
   void* out; long ldo;
-  unsigned units;        // 16-B units per row, the last one partial if the width is odd
+  unsigned units;        // 16-B units per row
   unsigned total;        // rows * units (< 2^31)
   int V, E;
   float scale;
@@ -79,7 +81,7 @@ struct LookupArgs {
 
 // Thread = ILP units, the ILP table loads in flight together; consecutive threads take consecutive units, so narrow
 // rows still fill a wave's loads.
-template <class T, class I, int ILP>
+template <class T, class I, int ILP, bool NARROW>
 __global__ __launch_bounds__(256) void embedding_fwd_kernel(LookupArgs a) {
   constexpr int N = Vec<T>::N;
   typedef typename Vec<T>::type V;
@@ -91,15 +93,16 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(LookupArgs a) {
   for (int k = 0; k < ILP; ++k) {
     const unsigned u = min(u0 + 256u * k, a.total - 1);
     row[k] = u / a.units;
-    c[k] = (u - row[k] * a.units) * N;
+    c[k] = NARROW ? 0 : min((u - row[k] * a.units) * N, (unsigned)(a.E - N));
     id[k] = (long)ids[row[k]];
   }
   V v[ILP];
 #pragma unroll
   for (int k = 0; k < ILP; ++k) {
     const long r = (id[k] >= 0 && id[k] < a.V) ? id[k] : 0;
-    v[k] = load_unit(reinterpret_cast<const T*>(a.table) + r * a.ldt + c[k], a.E - (int)c[k]);
+    v[k] = load_unit<NARROW>(reinterpret_cast<const T*>(a.table) + r * a.ldt + c[k], a.E);
   }
+  __builtin_amdgcn_sched_barrier(0);     // all loads before the first value is needed (131072 x 1024: 91.5 us without)
 #pragma unroll
   for (int k = 0; k < ILP; ++k) {
     if (u0 + 256u * k >= a.total) continue;
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(LookupArgs a) {
       o[e] = (T)x;
     }
     if (id[k] >= a.V && c[k] == 0 && a.err) atomicOr(a.err, kErrTokenId);
-    store_unit(reinterpret_cast<T*>(a.out) + (long)row[k] * a.ldo + c[k], a.E - (int)c[k], o);
+    store_unit<NARROW>(reinterpret_cast<T*>(a.out) + (long)row[k] * a.ldo + c[k], a.E, 0, o);
   }
 }
 
@@ -128,10 +131,12 @@ int launch_fwd(LookupArgs a, long rows, hipStream_t st) {
     a.out = out + r * a.ldo * (long)sizeof(T);
     a.total = (unsigned)(n * a.units);
     // four units a thread once that still gives every CU eight waves
-    if (a.total >= 4u * 256u * 512u)
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 4>), dim3((a.total + 1023) / 1024), dim3(256), 0, st, a);
+    if (a.E < Vec<T>::N)
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 1, true>), dim3((a.total + 255) / 256), dim3(256), 0, st, a);
+    else if (a.total >= 4u * 256u * 512u)
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 4, false>), dim3((a.total + 1023) / 1024), dim3(256), 0, st, a);
     else
-      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 1>), dim3((a.total + 255) / 256), dim3(256), 0, st, a);
+      hipLaunchKernelGGL((embedding_fwd_kernel<T, I, 1, false>), dim3((a.total + 255) / 256), dim3(256), 0, st, a);
     DASA_CHECK_LAUNCH();
   }
   return 0;
@@ -139,15 +144,45 @@ int launch_fwd(LookupArgs a, long rows, hipStream_t st) {
 
 // ------------------------------------------------------------------ tokens in sorted order
 constexpr int kSortWaves = 16;
-constexpr int kMaxRange = 896;        // vocabulary rows of one sort workgroup (its counters: 56 KB of LDS)
-constexpr int kList = 1024;           // tokens of its range that a wave notes on the first pass (96 KB of LDS)
+constexpr int kMaxBins = 896;        // vocabulary rows of one sort workgroup (its counters: 56 KB of LDS)
+constexpr int kList = 1024;           // tokens of its share that a wave notes on the first pass (96 KB of LDS)
+
+// Which workgroup sorts an id: G = 2^lg owners take the ids in turn (id u: owner u % G, its R bins u / G), since
+// vocabularies are often in the order of their words' frequencies: owners of ranges would leave most tokens to the
+// first (8192 such tokens x 1024 bf16, 50021 ids: 186 us with ranges, 32 in turn). The sorted order is by owner, then bin.
+struct Owners {
+  int lg, R;
+  __device__ __forceinline__ unsigned place(unsigned u) const { return (u & ((1u << lg) - 1)) * R + (u >> lg); }
+};
 
 struct SortArgs {
   const void* ids;
-  int T, V, R;
+  int T, V;
+  Owners own;
   unsigned pad;   // the id without a gradient, or 2^32 - 1
-  int* start;     // [V + 1] first sorted index of every token id
+  int* start;     // [G R + 1] first sorted index of every bin; the last: all tokens
   int* order;     // [T] positions in sorted order
+};
+
+inline Owners owners(int V, int least, int bins) {      // of at least `least` owners (if V has as many), `bins` bins at most
+  Owners o{0, 0};
+  while ((1 << o.lg) < least && (1 << o.lg) < V) ++o.lg;
+  while (((long)V + (1L << o.lg) - 1) >> o.lg > bins) ++o.lg;
+  o.R = (int)(((long)V + (1L << o.lg) - 1) >> o.lg);
+  return o;
+}
+inline int64_t bins_of(const Owners& o) { return ((int64_t)1 << o.lg) * o.R; }
+
+// An owner's tokens among the ids
+struct Mine {
+  unsigned low, V, g, pad;
+  int lg;
+  __device__ __forceinline__ Mine(const SortArgs& a, unsigned owner)
+      : low((1u << a.own.lg) - 1), V(a.V), g(owner), pad(a.pad), lg(a.own.lg) {}
+  __device__ __forceinline__ bool counts(unsigned u) const { return u < V && u != pad; }
+  __device__ __forceinline__ bool owns(unsigned u) const { return (u & low) == g && counts(u); }
+  __device__ __forceinline__ bool below(unsigned u) const { return (u & low) < g && counts(u); }
+  __device__ __forceinline__ int bin(unsigned u) const { return (int)(u >> lg); }
 };
 
 // An id as a 32-bit token: 2^32 - 1, which no vocabulary holds, for an id outside 32 bits.
@@ -181,7 +216,7 @@ __device__ __forceinline__ void each_token(const W* ids, int t0, int t1, int lan
   }
 }
 
-// Write the positions of up to 64 tokens of the range (lanes with `in`, in lane order) at their ranks, one distinct
+// Write the positions of up to 64 tokens of the share (lanes with `in`, in lane order) at their ranks, one distinct
 // id at a time: a frequent id is one turn.
 template <class O>
 __device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, int bin, int pos) {
@@ -196,15 +231,13 @@ __device__ __forceinline__ void place(int* cursor, O* order, int lane, bool in, 
   }
 }
 
-// f(position, bin, in, lanes with `in`) for the steps of a wave that hold a token of the range [lo, lo + n)
+// f(position, bin, in, lanes with `in`) for the steps of a wave that hold a token of the owner
 template <class W, class F>
-__device__ __forceinline__ void each_in_range(const W* ids, int t0, int t1, int lane, unsigned lo, unsigned n,
-                                              unsigned pad, F f) {
+__device__ __forceinline__ void each_of_mine(const W* ids, int t0, int t1, int lane, const Mine& own, F f) {
   each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {
-    const unsigned bin = u - lo;
-    const bool in = bin < n && u != pad;
+    const bool in = own.owns(u);
     const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
-    if (m) f(pos, (int)bin, in, m);
+    if (m) f(pos, own.bin(u), in, m);
   });
 }
 
@@ -247,26 +280,27 @@ __device__ __forceinline__ void wave_part(int& t0, int& t1, int w) {
   t0 = b;
 }
 
-// One launch: a workgroup's base is the number of tokens below its range, which it counts on the way.
+// One launch: an owner's base is the number of tokens of the owners before it, which it counts on the way.
 template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a) {
+  const int R = a.own.R;
   extern __shared__ int lpos[];                    // [waves][kList] positions, [waves][R] counts (then write
   int* const hist = lpos + kSortWaves * kList;     // cursors), [waves][kList] bins
-  unsigned short* const lbin = reinterpret_cast<unsigned short*>(hist + kSortWaves * a.R);
+  unsigned short* const lbin = reinterpret_cast<unsigned short*>(hist + kSortWaves * R);
   __shared__ int below[kSortWaves], wsum[kSortWaves];
   const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
-  for (int i = tid; i < kSortWaves * a.R; i += 64 * kSortWaves) hist[i] = 0;
+  const Mine own(a, blockIdx.x);
+  for (int i = tid; i < kSortWaves * R; i += 64 * kSortWaves) hist[i] = 0;
   __syncthreads();
   int t0 = 0, t1 = a.T;
   wave_part(t0, t1, w);
-  int* mine = hist + w * a.R;
+  int* mine = hist + w * R;
   int nb = 0, found = 0;
   each_token<W, 8>(ids, t0, t1, lane, [&](int pos, unsigned u) {
-    nb += __popcll(__builtin_amdgcn_ballot_w64(u < lo && u != a.pad));
-    const unsigned bin = u - lo;
-    const bool in = bin < n && u != a.pad;
+    nb += __popcll(__builtin_amdgcn_ballot_w64(own.below(u)));
+    const int bin = own.bin(u);
+    const bool in = own.owns(u);
     const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     const int at = found + __popcll(m & ((1ull << lane) - 1));
@@ -275,24 +309,25 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
       lbin[w * kList + at] = (unsigned short)bin;
     }
     found += __popcll(m);
-    add_bins<false>(mine, (int)bin, in, m);
+    add_bins<false>(mine, bin, in, m);
   });
   if (lane == 0) below[w] = nb;
   __syncthreads();
-  // exclusive scan over the range's ids (thread = id), then over the waves of one id
+  // exclusive scan over the bins (thread = bin), then over the waves of one bin
   int tot = 0;
-  if (tid < (int)n)
-    for (int k = 0; k < kSortWaves; ++k) tot += hist[k * a.R + tid];
+  if (tid < R)
+    for (int k = 0; k < kSortWaves; ++k) tot += hist[k * R + tid];
   int at = block_scan(tot, wsum) - tot;
   for (int k = 0; k < kSortWaves; ++k) at += below[k];
-  if (tid < (int)n) {
-    a.start[lo + tid] = at;
+  if (tid < R) {
+    const long p = (long)blockIdx.x * R + tid;
+    a.start[p] = at;
     for (int k = 0; k < kSortWaves; ++k) {
-      const int c = hist[k * a.R + tid];
-      hist[k * a.R + tid] = at;
+      const int c = hist[k * R + tid];
+      hist[k * R + tid] = at;
       at += c;
     }
-    if ((int)lo + tid == a.V - 1) a.start[a.V] = at;
+    if (tid == R - 1 && blockIdx.x == gridDim.x - 1) a.start[p + 1] = at;
   }
   __syncthreads();
   if (found <= kList) {
@@ -302,20 +337,21 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_sort_kernel(SortArgs a)
     }
     return;
   }
-  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long) {
-    place(mine, a.order, lane, in, bin, pos);      // a hot range: its ids again
+  each_of_mine<W>(ids, t0, t1, lane, own, [&](int pos, int bin, bool in, unsigned long long) {
+    place(mine, a.order, lane, in, bin, pos);      // many tokens: the ids again
   });
 }
 
-// Two launches for many tokens: workgroup = (wider range, segment of the tokens). The first counts its ids; the second
-// adds up what lies before each of its ids (smaller ids, and the same id in earlier segments) and places its tokens.
-constexpr int kWideRange = 1600;
+// Two launches for many tokens: workgroup = (owner of more bins, segment of the tokens). The first counts its bins;
+// the second adds up what lies before each (owners and bins before it, and the same bin in earlier segments) and places
+// its tokens.
+constexpr int kWideBins = 1600;
 constexpr int kSegmentTokens = 65024;              // of a segment at most: counts and offsets within it fit 16 bits
 
 struct SplitArgs {
-  int ranges, segments;
-  int* counts;     // [segments][V]
-  int* totals;     // [ranges][segments]
+  int segments;
+  int* counts;     // [segments][G R]
+  int* totals;     // [G][segments]
 };
 
 __device__ __forceinline__ void segment_of(int T, int segments, int& t0, int& t1) {
@@ -326,23 +362,24 @@ __device__ __forceinline__ void segment_of(int T, int segments, int& t0, int& t1
 
 template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(SortArgs a, SplitArgs p) {
-  __shared__ int hist[kWideRange];
+  __shared__ int hist[kWideBins];
   __shared__ int found[kSortWaves];
   const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
-  for (int i = tid; i < (int)n; i += 64 * kSortWaves) hist[i] = 0;
+  const int R = a.own.R;
+  for (int i = tid; i < R; i += 64 * kSortWaves) hist[i] = 0;
   __syncthreads();
   int t0, t1, total = 0;
   segment_of(a.T, p.segments, t0, t1);
   wave_part(t0, t1, w);
-  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int, int bin, bool in, unsigned long long m) {
+  each_of_mine<W>(ids, t0, t1, lane, Mine(a, blockIdx.x), [&](int, int bin, bool in, unsigned long long m) {
     total += __popcll(m);
     add_bins<false>(hist, bin, in, m);
   });
   if (lane == 0) found[w] = total;
   __syncthreads();
-  for (int i = tid; i < (int)n; i += 64 * kSortWaves) p.counts[(long)blockIdx.y * a.V + lo + i] = hist[i];
+  int* counts = p.counts + ((long)blockIdx.y * gridDim.x + blockIdx.x) * R;
+  for (int i = tid; i < R; i += 64 * kSortWaves) counts[i] = hist[i];
   if (tid == 0) {
     for (int k = 1; k < kSortWaves; ++k) total += found[k];
     p.totals[blockIdx.x * p.segments + blockIdx.y] = total;
@@ -351,26 +388,27 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_count_kernel(SortArgs a
 
 template <class W>
 __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a, SplitArgs p) {
-  // a wave's counts, later its offset into an id's run: two ids of 16 bits a word
-  __shared__ int count[kSortWaves][kWideRange / 2];
-  __shared__ int first[kWideRange];                // where an id's tokens of this segment begin
+  // a wave's counts, later its offset into a bin's run: two bins of 16 bits a word
+  __shared__ int count[kSortWaves][kWideBins / 2];
+  __shared__ int first[kWideBins];                // where a bin's tokens of this segment begin
   extern __shared__ int lpos[];                    // [waves][kList] positions, [waves][kList] bins
   unsigned short* const lbin = reinterpret_cast<unsigned short*>(lpos + kSortWaves * kList);
   __shared__ int wsum[kSortWaves], wbase[kSortWaves];
   const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lo = blockIdx.x * (unsigned)a.R, n = min((unsigned)a.R, a.V - lo);
-  for (int i = tid; i < kSortWaves * kWideRange / 2; i += 64 * kSortWaves) count[0][i] = 0;
-  // thread = two ids: all their tokens, those of the earlier segments, and the tokens of smaller ranges (asked for
+  const int R = a.own.R;
+  const long all_bins = (long)gridDim.x * R;
+  for (int i = tid; i < kSortWaves * kWideBins / 2; i += 64 * kSortWaves) count[0][i] = 0;
+  // thread = two bins: all their tokens, those of the earlier segments, and the tokens of the owners before (asked for
   // before the scan, which hides them)
-  constexpr int PER = (kWideRange + 64 * kSortWaves - 1) / (64 * kSortWaves);
-  static_assert(PER == 2, "two ids share a counter word");
+  constexpr int PER = (kWideBins + 64 * kSortWaves - 1) / (64 * kSortWaves);
+  static_assert(PER == 2, "two bins share a counter word");
   int all[PER] = {0, 0}, before[PER] = {0, 0}, base = 0;
   for (int k = 0; k < p.segments; ++k) {
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
       const int b = tid * PER + q;
-      const int c = b < (int)n ? p.counts[(long)k * a.V + lo + b] : 0;
+      const int c = b < R ? p.counts[k * all_bins + (long)blockIdx.x * R + b] : 0;
       all[q] += c;
       before[q] += k < (int)blockIdx.y ? c : 0;
     }
@@ -383,7 +421,7 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a
   int t0, t1, found = 0;
   segment_of(a.T, p.segments, t0, t1);
   wave_part(t0, t1, w);
-  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long m) {
+  each_of_mine<W>(ids, t0, t1, lane, Mine(a, blockIdx.x), [&](int pos, int bin, bool in, unsigned long long m) {
     const int at = found + __popcll(m & ((1ull << lane) - 1));
     if (in && at < kList) {
       lpos[w * kList + at] = pos;
@@ -394,18 +432,16 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a
   });
   int at = block_scan(all[0] + all[1], wsum) - all[0] - all[1];      // (its barrier also ends the counting)
   for (int k = 0; k < kSortWaves; ++k) at += wbase[k];
-  if (tid * PER < (int)n) {
+  if (tid * PER < R) {
     const int second = at + all[0];
     first[tid * PER] = at + before[0];
     first[tid * PER + 1] = second + before[1];
     if (blockIdx.y == 0) {
-      const int v = (int)lo + tid * PER;
-      a.start[v] = at;
-      if (v == a.V - 1) a.start[a.V] = second;
-      if (tid * PER + 1 < (int)n) {
-        a.start[v + 1] = second;
-        if (v + 1 == a.V - 1) a.start[a.V] = second + all[1];
-      }
+      int* start = a.start + (long)blockIdx.x * R + tid * PER;
+      const bool two = tid * PER + 1 < R;
+      start[0] = at;
+      if (two) start[1] = second;
+      if (tid * PER + PER >= R && blockIdx.x == gridDim.x - 1) start[two ? 2 : 1] = second + all[1];
     }
     int c[kSortWaves], run = 0;
 #pragma unroll
@@ -435,15 +471,11 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a
     }
     return;
   }
-  each_in_range<W>(ids, t0, t1, lane, lo, n, a.pad, [&](int pos, int bin, bool in, unsigned long long) {
+  each_of_mine<W>(ids, t0, t1, lane, Mine(a, blockIdx.x), [&](int pos, int bin, bool in, unsigned long long) {
     put(in, bin, pos);
   });
 }
 
-inline int sort_ranges(int V) {
-  const int need = (V + kWideRange - 1) / kWideRange, most = V < 32 ? V : 32;
-  return need > most ? need : most;
-}
 // One launch against two, 50021 ids, Zipf / uniform / one id: 49152 tokens x 64 bf16, the whole gradient, 34.4 / 28.9 /
 // 64.7 us against 33.6 / 30.8 / 45.3; 131072 tokens, the sort alone, 39 / 30 / 72 against 27.5 / 27.9 / 25.5. Above
 // 4 M tokens the counts of the segments would outgrow the tokens.
@@ -454,29 +486,25 @@ inline int sort_segments(int64_t T) { return (int)std::max<int64_t>(8, (T + kSeg
 
 inline int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
+inline Owners sort_owners(int64_t T, int V) { return split_sort(T) ? owners(V, 32, kWideBins) : owners(V, 256, kMaxBins); }
+
 template <class W>
 int launch_sort(SortArgs a, void* split, hipStream_t st) {
   const dim3 block(64 * kSortWaves);
+  const unsigned G = 1u << a.own.lg;
   if (split_sort(a.T)) {
     SplitArgs p;
     p.segments = sort_segments(a.T);
-    p.ranges = sort_ranges(a.V);
-    a.R = (a.V + p.ranges - 1) / p.ranges;
-    p.ranges = (a.V + a.R - 1) / a.R;
     p.counts = reinterpret_cast<int*>(split);
-    p.totals = p.counts + (long)p.segments * a.V;
-    const dim3 grid(p.ranges, p.segments);
+    p.totals = p.counts + p.segments * bins_of(a.own);
+    const dim3 grid(G, p.segments);
     hipLaunchKernelGGL(token_count_kernel<W>, grid, block, 0, st, a, p);
     DASA_CHECK_LAUNCH();
     hipLaunchKernelGGL(token_place_kernel<W>, grid, block, (size_t)kSortWaves * kList * 6, st, a, p);
     DASA_CHECK_LAUNCH();
     return 0;
   }
-  int G = (a.V + kMaxRange - 1) / kMaxRange;
-  if (G < 256) G = a.V < 256 ? a.V : 256;
-  a.R = (a.V + G - 1) / G;
-  G = (a.V + a.R - 1) / a.R;
-  hipLaunchKernelGGL(token_sort_kernel<W>, dim3(G), block, (size_t)kSortWaves * (a.R * 4 + kList * 6), st, a);
+  hipLaunchKernelGGL(token_sort_kernel<W>, dim3(G), block, (size_t)kSortWaves * (a.own.R * 4 + kList * 6), st, a);
   DASA_CHECK_LAUNCH();
   return 0;
 }
@@ -485,14 +513,16 @@ int launch_sort(SortArgs a, void* split, hipStream_t st) {
 // A lane's unit of a slice. Lanes past the row's end take its first unit and store nothing, so that whole waves reach
 // every lane exchange.
 struct Unit {
-  int col, left;
+  int col, skip;   // its first column; the columns that the unit before it writes
   bool live;
 };
 template <class T>
 __device__ __forceinline__ Unit unit_of(int slice, int lane, int E) {
-  const int col = (slice * 64 + lane) * Vec<T>::N;
-  const bool live = col < E;
-  return Unit{live ? col : 0, live ? E - col : E, live};
+  constexpr int N = Vec<T>::N;
+  const int col = (slice * 64 + lane) * N;
+  if (col >= E) return Unit{0, 0, false};
+  const int over = E < N ? 0 : max(col + N - E, 0);
+  return Unit{col - over, over, true};
 }
 
 // A table row of up to kChunk tokens is summed by one wave per slice of 64 units. Longer (hot) rows are cut at the
@@ -507,10 +537,12 @@ struct BwdArgs {
   const void* ids; int ids64;
   const int* start;
   const int* order;
+  Owners own;
   float* parts;            // [chunks][2][ldp] sums of hot rows' parts
   long ldp;
   void* dtable; long ldt;
   int V, E;
+  long bins;               // of the sort: start[bins] is the number of tokens
   unsigned chunk_blocks;   // blocks of the rows kernel that take chunks (first: they are the longer ones)
   float scale;
   int accumulate;
@@ -518,14 +550,15 @@ struct BwdArgs {
 
 // acc += the dout rows of n <= 64 tokens whose positions the lanes hold, tokens lane0 .. lane0 + n in order; K rows in
 // flight at a time.
-template <class T, int K>
-__device__ __forceinline__ int add_rows_by(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
+template <class T, bool NARROW, int K>
+__device__ __forceinline__ int add_rows_by(float (&acc)[Vec<T>::N], const T* d, long ldd, int E, int pos, int lane0,
                                            int j, int n) {
   for (; j + K <= n; j += K) {
     typename Vec<T>::type x[K];
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      x[k] = load_unit(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j + k) * ldd, left);
+      x[k] = load_unit<NARROW>(d + (long)__builtin_amdgcn_readlane(pos, lane0 + j + k) * ldd, E);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -533,23 +566,23 @@ __device__ __forceinline__ int add_rows_by(float (&acc)[Vec<T>::N], const T* d, 
   }
   return j;
 }
-template <class T>
-__device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::N], const T* d, long ldd, int left, int pos, int lane0,
+template <class T, bool NARROW>
+__device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::N], const T* d, long ldd, int E, int pos, int lane0,
                                          int n) {
-  int j = add_rows_by<T, 8>(acc, d, ldd, left, pos, lane0, 0, n);
-  j = add_rows_by<T, 2>(acc, d, ldd, left, pos, lane0, j, n);
-  add_rows_by<T, 1>(acc, d, ldd, left, pos, lane0, j, n);
+  int j = add_rows_by<T, NARROW, 8>(acc, d, ldd, E, pos, lane0, 0, n);
+  j = add_rows_by<T, NARROW, 2>(acc, d, ldd, E, pos, lane0, j, n);
+  add_rows_by<T, NARROW, 1>(acc, d, ldd, E, pos, lane0, j, n);
 }
 
-template <class T>
-__device__ __forceinline__ void write_row(const BwdArgs& a, long v, int col, int left, const float (&acc)[Vec<T>::N]) {
+template <class T, bool NARROW>
+__device__ __forceinline__ void write_row(const BwdArgs& a, long v, int col, int skip, const float (&acc)[Vec<T>::N]) {
   constexpr int N = Vec<T>::N;
   T* o = reinterpret_cast<T*>(a.dtable) + v * a.ldt + col;
   typename Vec<T>::type y;
-  if (a.accumulate) y = load_unit(o, left);
+  if (a.accumulate) y = load_unit<NARROW>(o, a.E);
 #pragma unroll
   for (int e = 0; e < N; ++e) y[e] = (T)(a.accumulate ? (float)y[e] + acc[e] * a.scale : acc[e] * a.scale);
-  store_unit(o, left, y);
+  store_unit<NARROW>(o, a.E, skip, y);
 }
 
 __device__ __forceinline__ long id_at(const BwdArgs& a, int pos) {
@@ -557,11 +590,11 @@ __device__ __forceinline__ long id_at(const BwdArgs& a, int pos) {
 }
 
 // One wave = (table row, slice) or (chunk, slice).
-template <class T>
+template <class T, bool NARROW>
 __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
+  const auto [col, skip, live] = unit_of<T>(blockIdx.y, lane, a.E);
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
   float acc[N];
 #pragma unroll
@@ -569,26 +602,27 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   if (blockIdx.x >= a.chunk_blocks) {
     const long v = (long)(blockIdx.x - a.chunk_blocks) * 4 + w;
     if (v >= a.V) return;
-    const int s = a.start[v], n = a.start[v + 1] - s;
+    const int* at = a.start + a.own.place((unsigned)v);
+    const int s = at[0], n = at[1] - s;
     if (n > kChunk || (a.accumulate && n == 0)) return;
     const int pos = lane < n ? a.order[s + lane] : 0;
-    add_rows<T>(acc, d, a.ldd, left, pos, 0, n);
-    if (live) write_row<T>(a, v, col, left, acc);
+    add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, 0, n);
+    if (live) write_row<T, NARROW>(a, v, col, skip, acc);
     return;
   }
   const long c = (long)blockIdx.x * 4 + w;
-  const int j0 = (int)(c * kChunk), total = a.start[a.V];
+  const int j0 = (int)(c * kChunk), total = a.start[a.bins];
   if (j0 >= total) return;
   const int m = min(kChunk, total - j0);
   const int pos = a.order[j0 + min(lane, m - 1)];
-  const long id = id_at(a, pos);
-  const int rs = a.start[id], re = a.start[id + 1];
+  const int* at = a.start + a.own.place((unsigned)id_at(a, pos));
+  const int rs = at[0], re = at[1];
   const bool hot = re - rs > kChunk;
   float* part = a.parts + c * 2 * a.ldp + col;
   // the row that owns the chunk's first token, then the row that owns its last
   const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
   if (ea > 0) {
-    add_rows<T>(acc, d, a.ldd, left, pos, 0, ea);
+    add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, 0, ea);
     if (live)
 #pragma unroll
       for (int e = 0; e < N; ++e) part[e] = acc[e];
@@ -597,35 +631,51 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   if (sb > 0 && sb < m) {
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    add_rows<T>(acc, d, a.ldd, left, pos, sb, m - sb);
+    add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, sb, m - sb);
     if (live)
 #pragma unroll
       for (int e = 0; e < N; ++e) part[a.ldp + e] = acc[e];
   }
 }
 
-// parts [k0, k1) of the hot row whose first part is slot `first` of chunk c, added in order
+// parts [k0, k1) of the hot row whose first part is slot `first` of chunk c, added in order, eight in flight
 template <class T>
 __device__ __forceinline__ void add_parts(float (&acc)[Vec<T>::N], const BwdArgs& a, long c, int first, int k0, int k1,
                                           int col) {
-#pragma unroll 2
-  for (int k = k0; k < k1; ++k) {
-    const float* p = a.parts + ((c + k) * 2 + (k == 0 ? first : 0)) * a.ldp + col;
+  constexpr int N = Vec<T>::N, K = 8;
+  typedef float V __attribute__((ext_vector_type(N), aligned(4)));
+  auto part = [&](int k) {
+    return *reinterpret_cast<const V*>(a.parts + ((c + k) * 2 + (k == 0 ? first : 0)) * a.ldp + col);
+  };
+  int k = k0;
+  for (; k + K <= k1; k += K) {
+    V x[K];
 #pragma unroll
-    for (int e = 0; e < Vec<T>::N; ++e) acc[e] += p[e];
+    for (int i = 0; i < K; ++i) x[i] = part(k + i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += x[i][e];
+  }
+#pragma unroll 2
+  for (; k < k1; ++k) {
+    const V x = part(k);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += x[e];
   }
 }
 
 // One workgroup = (kJoinWaves chunks, slice). A hot row that starts in a chunk reaches past its end, so the chunk's
 // last token names it. Rows of up to kJoinWaves parts: one wave each. The one longer row that may start in the group
 // (it reaches past the group's end) takes the whole workgroup: the waves add runs of parts, joined in order.
-template <class T>
+template <class T, bool NARROW>
 __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
   __shared__ float sum[kJoinWaves][64][N];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
-  const int total = a.start[a.V];
+  const auto [col, skip, live] = unit_of<T>(blockIdx.y, lane, a.E);
+  const int total = a.start[a.bins];
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
@@ -633,16 +683,18 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   const long j0 = c * kChunk;
   if (j0 < total) {
     const long v = id_at(a, a.order[min(j0 + kChunk, (long)total) - 1]);
-    const int rs = a.start[v], re = a.start[v + 1], n = (re - 1) / kChunk - (int)c + 1;
+    const int* at = a.start + a.own.place((unsigned)v);
+    const int rs = at[0], re = at[1], n = (re - 1) / kChunk - (int)c + 1;
     if (re - rs > kChunk && rs >= j0 && n <= kJoinWaves) {
       add_parts<T>(acc, a, c, rs > j0, 0, n, col);
-      if (live) write_row<T>(a, v, col, left, acc);
+      if (live) write_row<T, NARROW>(a, v, col, skip, acc);
     }
   }
   const long g0 = (long)blockIdx.x * kJoinWaves * kChunk;
   if (g0 >= total) return;
   const long v = id_at(a, a.order[min(g0 + kJoinWaves * kChunk, (long)total) - 1]);
-  const int rs = a.start[v], re = a.start[v + 1];
+  const int* at = a.start + a.own.place((unsigned)v);
+  const int rs = at[0], re = at[1];
   const int c0 = rs / kChunk, n = (re - 1) / kChunk - c0 + 1;
   if (rs < g0 || n <= kJoinWaves) return;
   const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
@@ -656,23 +708,23 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   for (int k = 1; k < kJoinWaves; ++k)
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
-  write_row<T>(a, v, col, left, acc);
+  write_row<T, NARROW>(a, v, col, skip, acc);
 }
 
 // ------------------------------------------------------------------ few tokens: one launch
-// Up to kFewTokens tokens: workgroup = (vocabulary range, slice). It sorts its range's tokens into LDS as above (every
+// Up to kFewTokens tokens: workgroup = (share of the ids, slice). It sorts its tokens into LDS as above (every
 // token of a wave's segment fits its list) and sums its rows itself: ids of up to kChunk tokens a wave each, the others
 // by all waves, whose parts are joined in order. Three launches become one, and no workspace is needed.
 constexpr int kFewTokens = 8192;
 constexpr int kFewWaves = 8;
-constexpr int kFewRange = 256;
+constexpr int kFewBins = 256;
 
 inline int few_segment(int T) { return (((T + kFewWaves - 1) / kFewWaves) + 63) & ~63; }
 
-template <class T, class W>
+template <class T, class W, bool NARROW>
 __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(BwdArgs a, SortArgs g, int seg) {
   constexpr int N = Vec<T>::N;
-  __shared__ int hist[kFewWaves][kFewRange], first[kFewRange + 1], wsum[kFewWaves], hot[kFewRange], nhot;
+  __shared__ int hist[kFewWaves][kFewBins], first[kFewBins + 1], wsum[kFewWaves], hot[kFewBins], nhot;
   // the sorted positions [waves seg]; the waves' tokens [waves][seg] as positions and ids, later the hot rows' sums
   extern __shared__ __attribute__((aligned(16))) unsigned short order[];
   unsigned short* const lpos = order + kFewWaves * seg;
@@ -680,16 +732,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   float* const sum = reinterpret_cast<float*>(lpos);       // [waves][64][N]
   const W* ids = reinterpret_cast<const W*>(a.ids);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const unsigned lo = blockIdx.x * (unsigned)g.R, n = min((unsigned)g.R, a.V - lo);
-  const auto [col, left, live] = unit_of<T>(blockIdx.y, lane, a.E);
-  for (int i = tid; i < kFewWaves * kFewRange; i += 64 * kFewWaves) hist[0][i] = 0;
+  const Mine own(g, blockIdx.x);
+  const int n = (int)((a.V + own.low - blockIdx.x) >> own.lg);     // its ids: blockIdx.x + r G
+  const auto [col, skip, live] = unit_of<T>(blockIdx.y, lane, a.E);
+  for (int i = tid; i < kFewWaves * kFewBins; i += 64 * kFewWaves) hist[0][i] = 0;
   if (tid == 0) nhot = 0;
   __syncthreads();
   const int t0 = min(w * seg, g.T), t1 = min(t0 + seg, g.T);
   int found = 0;
   each_token<W, 4>(ids, t0, t1, lane, [&](int pos, unsigned u) {
-    const unsigned bin = u - lo;
-    const bool in = bin < n && u != g.pad;
+    const int bin = own.bin(u);
+    const bool in = own.owns(u);
     const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     if (in) {
@@ -702,7 +755,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   });
   __syncthreads();
   int tot = 0;
-  if (tid < (int)n)
+  if (tid < n)
     for (int k = 0; k < kFewWaves; ++k) tot += hist[k][tid];
   int incl = tot;
 #pragma unroll
@@ -714,8 +767,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   __syncthreads();
   int at = incl - tot;
   for (int k = 0; k < w; ++k) at += wsum[k];
-  if (tid <= (int)n) first[tid] = at;              // thread n: the total
-  if (tid < (int)n) {
+  if (tid <= n) first[tid] = at;              // thread n: the total
+  if (tid < n) {
     for (int k = 0; k < kFewWaves; ++k) {
       const int c = hist[k][tid];
       hist[k][tid] = at;
@@ -731,14 +784,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   __syncthreads();
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
   float acc[N];
-  for (int r = w; r < (int)n; r += kFewWaves) {
+  for (int r = w; r < n; r += kFewWaves) {
     const int s = first[r], c = first[r + 1] - s;
     if (c > kChunk || (a.accumulate && c == 0)) continue;
     const int pos = lane < c ? order[s + lane] : 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    add_rows<T>(acc, d, a.ldd, left, pos, 0, c);
-    if (live) write_row<T>(a, lo + r, col, left, acc);
+    add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, 0, c);
+    if (live) write_row<T, NARROW>(a, blockIdx.x + ((long)r << own.lg), col, skip, acc);
   }
   const int h = nhot;
   if (h == 0) return;
@@ -749,7 +802,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
     for (int k = k0; k < k1; k += 64) {
       const int pos = order[s + min(k + lane, k1 - 1)];
-      add_rows<T>(acc, d, a.ldd, left, pos, 0, min(64, k1 - k));
+      add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, 0, min(64, k1 - k));
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) sum[(w * 64 + lane) * N + e] = acc[e];
@@ -758,26 +811,29 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
       for (int k = 1; k < kFewWaves; ++k)
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] += sum[(k * 64 + lane) * N + e];
-      write_row<T>(a, lo + r, col, left, acc);
+      write_row<T, NARROW>(a, blockIdx.x + ((long)r << own.lg), col, skip, acc);
     }
     __syncthreads();
   }
 }
 
-template <class T>
-int launch_few(const BwdArgs& a, SortArgs g, hipStream_t st) {
+template <class T, bool NARROW>
+int launch_few_as(const BwdArgs& a, SortArgs g, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
-  int G = (a.V + kFewRange - 1) / kFewRange;
-  if (G < 256) G = a.V < 256 ? a.V : 256;
-  g.R = (a.V + G - 1) / G;
+  g.own = owners(a.V, 256, kFewBins);
   const int seg = few_segment(g.T);
   const size_t lists = (size_t)kFewWaves * seg * 4, sums = (size_t)kFewWaves * 64 * Vec<T>::N * 4;
   const size_t lds = (size_t)kFewWaves * seg * 2 + (lists > sums ? lists : sums);
-  const dim3 grid((a.V + g.R - 1) / g.R, slices), block(64 * kFewWaves);
-  if (a.ids64) hipLaunchKernelGGL((embedding_bwd_few_kernel<T, uint2>), grid, block, lds, st, a, g, seg);
-  else hipLaunchKernelGGL((embedding_bwd_few_kernel<T, unsigned>), grid, block, lds, st, a, g, seg);
+  const dim3 grid(1u << g.own.lg, slices), block(64 * kFewWaves);
+  if (a.ids64) hipLaunchKernelGGL((embedding_bwd_few_kernel<T, uint2, NARROW>), grid, block, lds, st, a, g, seg);
+  else hipLaunchKernelGGL((embedding_bwd_few_kernel<T, unsigned, NARROW>), grid, block, lds, st, a, g, seg);
   DASA_CHECK_LAUNCH();
   return 0;
+}
+
+template <class T>
+int launch_few(const BwdArgs& a, const SortArgs& g, hipStream_t st) {
+  return a.E < Vec<T>::N ? launch_few_as<T, true>(a, g, st) : launch_few_as<T, false>(a, g, st);
 }
 
 inline long part_stride(int E, int bf16) {      // whole units, so a partial unit's sums stay inside
@@ -785,20 +841,23 @@ inline long part_stride(int E, int bf16) {      // whole units, so a partial uni
   return (long)(E + n - 1) / n * n;
 }
 
-template <class T>
-int launch_rows(BwdArgs a, long tokens, hipStream_t st) {
+template <class T, bool NARROW>
+int launch_rows_as(BwdArgs a, long tokens, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   const long chunks = (tokens + kChunk - 1) / kChunk;
   a.chunk_blocks = (unsigned)((chunks + 3) / 4);
   const dim3 grid(a.chunk_blocks + (unsigned)((a.V + 3) / 4), slices);
-  hipLaunchKernelGGL(embedding_bwd_rows_kernel<T>, grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, NARROW>), grid, dim3(256), 0, st, a);
   DASA_CHECK_LAUNCH();
-  hipLaunchKernelGGL(embedding_bwd_join_kernel<T>, dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
+  hipLaunchKernelGGL((embedding_bwd_join_kernel<T, NARROW>), dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
                      dim3(64 * kJoinWaves), 0, st, a);
   DASA_CHECK_LAUNCH();
   return 0;
 }
-
+template <class T>
+int launch_rows(const BwdArgs& a, long tokens, hipStream_t st) {
+  return a.E < Vec<T>::N ? launch_rows_as<T, true>(a, tokens, st) : launch_rows_as<T, false>(a, tokens, st);
+}
 
 }  // namespace
 
@@ -817,8 +876,9 @@ extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* id
 extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E) {
   if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0) return 0;
   const int64_t chunks = (T + kChunk - 1) / kChunk;
-  const int64_t split = split_sort(T) ? ((int64_t)V + sort_ranges(V)) * sort_segments(T) * 4 : 0;
-  return round16(((int64_t)V + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4 + split;
+  const Owners own = sort_owners(T, V);
+  const int64_t split = split_sort(T) ? (bins_of(own) + (1 << own.lg)) * sort_segments(T) * 4 : 0;
+  return round16((bins_of(own) + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4 + split;
 }
 
 extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t ids_bytes, int64_t T,
@@ -834,10 +894,12 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   BwdArgs ba{};
   ba.dout = dout; ba.ldd = (long)ldd; ba.ids = ids; ba.ids64 = ids_bytes == 8;
   ba.dtable = dtable; ba.ldt = (long)ldt; ba.V = V; ba.E = E; ba.scale = scale; ba.accumulate = accumulate;
-  SortArgs sa{ids, (int)T, V, 0, padding_idx < 0 ? ~0u : (unsigned)padding_idx, nullptr, nullptr};
+  SortArgs sa{ids, (int)T, V, Owners{0, 0}, padding_idx < 0 ? ~0u : (unsigned)padding_idx, nullptr, nullptr};
   if (T <= kFewTokens) return bf16 ? launch_few<__bf16>(ba, sa, st) : launch_few<float>(ba, sa, st);
+  ba.own = sa.own = sort_owners(T, V);
+  ba.bins = (long)bins_of(ba.own);
   int* start = reinterpret_cast<int*>(ws);
-  int* order = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + round16(((int64_t)V + 1) * 4));
+  int* order = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + round16((bins_of(ba.own) + 1) * 4));
   ba.start = sa.start = start;
   ba.order = sa.order = order;
   ba.parts = reinterpret_cast<float*>(reinterpret_cast<char*>(order) + round16(T * 4));
