@@ -101,7 +101,9 @@ def _check_bwd(got, dout, ids, V, scale, pad, dtype, what, old=None):
                                         (8193, 2, 8, "uniform"), (33000, 40, 520, "zipf"),
                                         (49152, 2, 8, "uniform"), (60001, 3000, 16, "one"), (50001, 40, 72, "zipf"),
                                         (131073, 300000, 8, "zipf"), (70000, 70000, 4, "perm"),
-                                        (2**22, 1000, 1, "zipf"), (2**22 + 1, 1000, 1, "zipf")])
+                                        (2**22, 1000, 1, "zipf"), (2**22 + 1, 1000, 1, "zipf"),
+                                        (8192, 3, 300, "uniform"), (4097, 60000, 40, "one"), (1601, 9000, 129, "one"),
+                                        (513, 2, 3, "one"), (8000, 9, 7, "zipf"), (6000, 40, 1030, "zipf")])
 def test_embedding_gradient(dev, dtype, T, V, E, kind):
     g = _gen(T * 3 + V + E)
     if kind == "uniform":
