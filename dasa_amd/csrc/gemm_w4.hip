@@ -18,10 +18,13 @@ using w4::W4Args;
 //    The weights come from cache for the second rows; holding several row tiles in a workgroup instead leaves the chip
 //    emptier (20 x 4096 x 2240 fp32 8.6 against 11.4, 64 x 992 x 512 fp32 4.1 against 7.8). Column blocks of a
 //    workgroup: as many as still leave about one workgroup a CU, since they share the activations' loads and their
-//    splitting into planes; bf16 rows need no splitting and stop at two (1 x 32768 x 8192 bf16 31.2 against 33.0).
-//  * many weights and more than 16 rows: the shared form (64 x 30522 x 768 bf16 11.6 against 19.8, 64 x 16384 x 4096
+//    splitting into planes; up to eight bf16 rows, which need no splitting, stop at two (1 x 30522 x 768 bf16 5.1
+//    against 5.9, 16 rows 7.3 against 6.9; 32768 x 8192: one row 30.0 against 30.9, 16 rows 43.0 against 33.9).
+//  * many weights and more than 16 rows: the shared form (64 x 30522 x 768 bf16 11.8 against 19.8, 64 x 16384 x 4096
 //    fp32 35.7 against 39), two row tiles a workgroup, four where the weights are too many to read twice
-//    (64 x 32768 x 8192 bf16 63 against 83).
+//    (64 x 32768 x 8192 bf16 63 against 83). A wave takes two column blocks, one where K is short and the loop is
+//    mostly its start and end (33 x 32768 x 1024 bf16 11.5 against 13.3; three planes a row want two from three row
+//    tiles on, 64 x 30522 x 768 fp32 17.2 against 18.8).
 //  * K is split over workgroups, at the price of a second launch (2 us), only where a long K leaves too few of them
 //    (1 x 1000 x 8192 fp32 7.7 against 13.4).
 inline Plan plan_of(int M, int N, int K, int bf16) {
@@ -34,14 +37,14 @@ inline Plan plan_of(int M, int N, int K, int bf16) {
   if (rows > 1 && units >= 3500) {
     p.shared = true;
     p.mt = rows > 2 && tiles * Kb >= 65536 ? 4 : 2;
-    p.nt = p.mt == 4 || rows > 2 || Kb >= 16 ? 2 : 1;
+    p.nt = p.mt == 4 || Kb >= 16 || (rows > 2 && !bf16) ? 2 : 1;
     const long wgs = (tiles + 8 * p.nt - 1) / (8 * p.nt) * ((rows + p.mt - 1) / p.mt);
     p.splits = (int)std::max(1L, std::min(256 / wgs, Kb / 8));
     return p;
   }
   if (Kb >= 48 && (!bf16 || rows > 1)) p.splits = (int)std::max(1L, std::min({Kb / 16, 4L, 1024 / units}));
   const long fill = units * p.splits;            // workgroups of one column block
-  p.nt = fill < 384 ? 1 : fill < 640 || (bf16 && rows == 1) ? 2 : 4;
+  p.nt = fill < 384 ? 1 : fill < 640 || (bf16 && M <= 8) ? 2 : 4;
   p.waves = Kb > 8 && fill / p.nt <= 256 ? 16 : 8;
   return p;
 }

@@ -20,8 +20,8 @@
 // x are split into planes and held in LDS once for all of them. K may be split over workgroups in both; a second
 // launch then joins the sums in order. Every order is fixed by the shape: results are bitwise reproducible.
 //
-// What bounds it, measured: one row on a wide layer is its weights' bytes (1 x 32768 x 8192 bf16, group 128: 31.2 us for
-// 138 MB = 4.4 TB/s, a large copy reaches 5.2); small layers are a launch (1 x 2048 x 256: 2.8 us); many fp32 rows are
+// What bounds it, measured: one row on a wide layer is its weights' bytes (1 x 32768 x 8192 bf16, group 128: 27.7 us for
+// 138 MB = 5.0 TB/s, a large copy reaches 5.2); small layers are a launch (1 x 2048 x 256: 2.8 us); many fp32 rows are
 // the three planes' matrix instructions (64 x 32768 x 8192: 112 us = 0.92 PFLOP/s of bf16 work).
 #pragma once
 #include "common.h"
@@ -238,6 +238,9 @@ __global__ __launch_bounds__(64 * W, 4) void w4_split_kernel(W4Args a) {
       if constexpr (TAIL) raw[j] = X::load_part(x + k, a.K - k - kq * 8);
       else raw[j] = X::load(x + k);
     }
+    // all loads of the block before its first product (1 x 32768 x 8192 bf16: 33.0 us without); fp32 rows' three planes
+    // need the registers that this would hold (20 x 4096 x 2240: 10.8 us with, 10.0 without)
+    if constexpr (PL == 1) __builtin_amdgcn_sched_barrier(0);
     floatx4 acc[NT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
