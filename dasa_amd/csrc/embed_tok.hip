@@ -29,6 +29,7 @@
 
 namespace {
 
+constexpr int kMostSize = 1 << 30;    // of a table: index arithmetic adds tiles to it in 32 bits
 constexpr unsigned kErrTokenId = 8;   // bit of the error word (ops._ERR_BITS)
 
 // 16 bytes of a row. Rows of odd width or stride start anywhere, so the vector types are element-aligned (global loads
@@ -971,7 +972,8 @@ int launch_rows(const BwdArgs& a, long tokens, hipStream_t st) {
 extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* ids, int32_t ids_bytes, int64_t T,
                                   int32_t V, int32_t E, float scale, int32_t bf16, void* out, int64_t ldo,
                                   uint32_t* err, void* stream) {
-  if (T < 0 || V < 0 || E < 0 || (ids_bytes != 4 && ids_bytes != 8)) return (int)hipErrorInvalidValue;
+  if (T < 0 || V < 0 || E < 0 || V > kMostSize || E > kMostSize || (ids_bytes != 4 && ids_bytes != 8))
+    return (int)hipErrorInvalidValue;
   if (T == 0 || E == 0) return 0;
   if (V == 0 || !table || !ids || !out || ldt < E || ldo < E) return (int)hipErrorInvalidValue;
   LookupArgs a{table, (long)ldt, ids, out, (long)ldo, 0, 0, V, E, scale, err};
@@ -981,7 +983,7 @@ extern "C" int dasa_embedding_fwd(const void* table, int64_t ldt, const void* id
 }
 
 extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E) {
-  if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0) return 0;
+  if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0 || V > kMostSize || E > kMostSize) return 0;
   const int64_t chunks = (T + kChunk - 1) / kChunk;
   const Owners own = sort_owners(T, V);
   const int64_t split = split_sort(T) ? (bins_of(own) + (1 << own.lg)) * sort_segments(T) * 4 : 0;
@@ -991,7 +993,8 @@ extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E)
 extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t ids_bytes, int64_t T,
                                   int32_t V, int32_t E, float scale, int32_t padding_idx, int32_t bf16, void* dtable,
                                   int64_t ldt, int32_t accumulate, void* ws, int64_t ws_bytes, void* stream) {
-  if (T < 0 || T >= (1LL << 31) - 65536 || V < 0 || E < 0 || (ids_bytes != 4 && ids_bytes != 8))
+  if (T < 0 || T >= (1LL << 31) - 65536 || V < 0 || E < 0 || V > kMostSize || E > kMostSize ||
+      (ids_bytes != 4 && ids_bytes != 8))
     return (int)hipErrorInvalidValue;
   if (V == 0 || E == 0) return 0;
   if (!dtable || ldt < E || ws_bytes < dasa_embedding_bwd_workspace(T, V, E) || (T > kFewTokens && !ws))

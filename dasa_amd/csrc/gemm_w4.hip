@@ -57,31 +57,40 @@ struct LayoutArgs {
   int N, K, Kb, N16, g;
 };
 
-// One thread per 32-bit word (eight codes of a row, which keep their order: code ^ 8 is the stored nibble); the first
-// threads of a block also place its scales.
+// Workgroup = 16 rows and four 128-deep blocks, whose codes are 256 B of a row: lines are read whole (32768 x 8192: 88 us
+// with a block a workgroup). Thread = 32 codes of a row, four words of the layout, in which eight codes keep their order:
+// code ^ 8 is the stored nibble. The first threads also place the blocks' scales.
 template <class S>
 __global__ __launch_bounds__(256) void w4_layout_kernel(LayoutArgs a) {
-  typedef unsigned u32u __attribute__((aligned(1)));
-  const long blk = blockIdx.x;                        // (column block, K block)
-  const int nt = (int)(blk / a.Kb), kb = (int)(blk % a.Kb);
-  const int tid = threadIdx.x, c = tid >> 4, unit = tid & 15;      // a row's 64 B are read by 16 threads in a row
-  const int n = nt * 16 + c, k = kb * 128 + unit * 8;
-  unsigned word = 0;                                  // two's complement 0: padding adds nothing
+  typedef unsigned u4u __attribute__((ext_vector_type(4), aligned(1)));
+  const int per = (a.Kb + 3) / 4;
+  const int nt = (int)(blockIdx.x / per), kb0 = (int)(blockIdx.x % per) * 4;
+  const int tid = threadIdx.x, c = tid >> 4, q = tid & 15, kb = kb0 + (q >> 2);
+  const int n = nt * 16 + c, k = kb0 * 128 + q * 32;
+  unsigned word[4] = {0, 0, 0, 0};                    // two's complement 0: padding adds nothing
   if (n < a.N) {
     const unsigned char* p = a.codes + (long)n * a.ldc + (k >> 1);
-    if (k + 8 <= a.K) {
-      word = *reinterpret_cast<const u32u*>(p) ^ 0x88888888u;
+    if (k + 32 <= a.K) {
+      const u4u v = *reinterpret_cast<const u4u*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word[i] = v[i] ^ 0x88888888u;
     } else {
-      for (int i = 0; i < 8 && k + i < a.K; ++i) word |= (((p[i >> 1] >> (4 * (i & 1))) & 15u) ^ 8u) << (4 * i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        for (int e = 0; e < 8 && k + 8 * i + e < a.K; ++e)
+          word[i] |= (((p[4 * i + (e >> 1)] >> (4 * (e & 1))) & 15u) ^ 8u) << (4 * e);
     }
   }
-  a.w[blk * 256 + ((unit & 3) * 16 + c) * 4 + (unit >> 2)] = word;
+  if (kb < a.Kb) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a.w[((long)nt * a.Kb + kb) * 256 + (i * 16 + c) * 4 + (q & 3)] = word[i];
+  }
   const int gpb = 128 / a.g, groups = (a.K + a.g - 1) / a.g;
-  if (tid < gpb * 16) {
-    const int nn = nt * 16 + tid / gpb, gi = kb * gpb + tid % gpb;
-    const bool in = nn < a.N && gi < groups;
-    reinterpret_cast<S*>(a.ws)[blk * gpb * 16 + tid] =
-        in ? reinterpret_cast<const S*>(a.scales)[(long)nn * a.lds_ + gi] : (S)0.f;
+  for (int i = tid; i < 4 * gpb * 16; i += 256) {
+    const int b = kb0 + i / (gpb * 16), j = i % (gpb * 16), nn = nt * 16 + j / gpb, gi = b * gpb + j % gpb;
+    if (b >= a.Kb) continue;
+    reinterpret_cast<S*>(a.ws)[((long)nt * a.Kb + b) * gpb * 16 + j] =
+        nn < a.N && gi < groups ? reinterpret_cast<const S*>(a.scales)[(long)nn * a.lds_ + gi] : (S)0.f;
   }
 }
 
@@ -117,24 +126,26 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(QuantArgs a) {
   }
 }
 
+// N and K of a weight: index arithmetic adds blocks to them in 32 bits
+inline bool sizes_ok(int N, int K) { return N > 0 && K > 0 && N <= 1 << 30 && K <= 1 << 30; }
 inline bool group_ok(int g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
 
 extern "C" int64_t dasa_w4_weight_bytes(int32_t N, int32_t K) {
-  if (N <= 0 || K <= 0) return 0;
+  if (!sizes_ok(N, K)) return 0;
   return (int64_t)((N + 15) / 16) * ((K + 127) / 128) * 1024;
 }
 
 extern "C" int64_t dasa_w4_scale_count(int32_t N, int32_t K, int32_t group) {
-  if (N <= 0 || K <= 0 || !group_ok(group)) return 0;
+  if (!sizes_ok(N, K) || !group_ok(group)) return 0;
   return (int64_t)((N + 15) / 16) * ((K + 127) / 128) * (128 / group) * 16;
 }
 
 extern "C" int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int32_t K, int32_t group,
                                 uint8_t* codes, int64_t ldc, void* scales, int64_t lds, int32_t scale_bf16,
                                 void* stream) {
-  if (N <= 0 || K <= 0 || !group_ok(group) || !W || !codes || !scales || ldw < K || ldc < (K + 1) / 2 ||
+  if (!sizes_ok(N, K) || !group_ok(group) || !W || !codes || !scales || ldw < K || ldc < (K + 1) / 2 ||
       lds < (K + group - 1) / group)
     return (int)hipErrorInvalidValue;
   QuantArgs a{W, (long)ldw, codes, (long)ldc, scales, (long)lds, N, K, group};
@@ -152,12 +163,12 @@ extern "C" int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int3
 
 extern "C" int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16,
                               int32_t N, int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream) {
-  if (N <= 0 || K <= 0 || !group_ok(group) || !codes || !scales || !weight || !scale_tiles || ldc < (K + 1) / 2 ||
+  if (!sizes_ok(N, K) || !group_ok(group) || !codes || !scales || !weight || !scale_tiles || ldc < (K + 1) / 2 ||
       lds < (K + group - 1) / group)
     return (int)hipErrorInvalidValue;
   LayoutArgs a{codes, (long)ldc, scales, (long)lds, reinterpret_cast<unsigned*>(weight), scale_tiles, N, K,
                (K + 127) / 128, (N + 15) / 16, group};
-  const long blocks = (long)a.N16 * a.Kb;
+  const long blocks = (long)a.N16 * ((a.Kb + 3) / 4);
   if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
   if (scale_bf16)
     hipLaunchKernelGGL(w4_layout_kernel<__bf16>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
@@ -168,7 +179,7 @@ extern "C" int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* sca
 }
 
 extern "C" int64_t dasa_gemm_w4_workspace(int32_t M, int32_t N, int32_t K, int32_t bf16) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || M > 65535 * 16 || !sizes_ok(N, K)) return 0;
   const Plan p = plan_of(M, N, K, bf16);
   if (p.splits <= 1) return 0;
   return (int64_t)p.splits * ((M + 16 * p.mt - 1) / (16 * p.mt)) * p.mt * ((N + 15) / 16) * 1024;
@@ -177,7 +188,7 @@ extern "C" int64_t dasa_gemm_w4_workspace(int32_t M, int32_t N, int32_t K, int32
 extern "C" int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, const void* scale_tiles,
                             int32_t scale_bf16, int32_t group, const float* bias, int32_t act, float beta, void* y,
                             int64_t ldy, int32_t M, int32_t N, int32_t K, void* ws, int64_t ws_bytes, void* stream) {
-  if (M < 0 || N <= 0 || K <= 0 || !group_ok(group) || act < DASA_ACT_NONE || act > DASA_ACT_SIGMOID)
+  if (M < 0 || !sizes_ok(N, K) || !group_ok(group) || act < DASA_ACT_NONE || act > DASA_ACT_SIGMOID)
     return (int)hipErrorInvalidValue;
   if (M == 0) return 0;
   if (!x || !weight || !scale_tiles || !y || ldx < K || ldy < N || ((uintptr_t)weight & 15) || M > 65535 * 16)

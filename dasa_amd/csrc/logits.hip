@@ -15,7 +15,7 @@
 //
 // Bound by latency at a decoding step's sizes: 20 x 992 fp32 with 120 ids a row 4.4 us, where an empty kernel takes 2.4.
 // 64 x 30522 fp32, 1024 ids: 8.9 + 2.6 us (17 MB: 3.2 at a copy's rate); 16 x 128255 bf16 with a bias a row, 16384 ids:
-// 13.9 + 3.2 (18 MB: 3.5), half of it the history that every slice reads.
+// 13.9 + 3.2 (18 MB: 3.5), 2.4 of it the history that every slice reads.
 #include "common.h"
 #include "../../include/dasa_hip.h"
 
@@ -186,6 +186,8 @@ __global__ __launch_bounds__(64) void logit_choice_kernel(const unsigned long lo
   if (threadIdx.x == 0) choice[blockIdx.x] = (int64_t)(unsigned)~(unsigned)k;
 }
 
+constexpr int kMostSize = 1 << 30;    // of V and L: index arithmetic adds slices to them in 32 bits
+
 struct Shape {
   int iter, threads, slices;
 };
@@ -214,7 +216,7 @@ void launch(const RulesArgs& a, const Shape& s, int B, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t dasa_logit_rules_workspace(int32_t B, int32_t V) {
-  if (B <= 0 || V <= 0) return 0;
+  if (B <= 0 || V <= 0 || V > kMostSize) return 0;
   const int s = shape_of(B, V).slices;
   return s > 1 ? (int64_t)B * s * 8 : 0;
 }
@@ -222,7 +224,7 @@ extern "C" int64_t dasa_logit_rules_workspace(int32_t B, int32_t V) {
 extern "C" int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_t ws_bytes, void* stream) {
   if (!d || d->B < 0 || d->V < 0) return (int)hipErrorInvalidValue;
   if (d->B == 0) return 0;
-  if (d->V == 0 || d->B > 65535 || d->L < 0 || !d->logits || !d->out || d->ld < d->V || d->ldo < d->V)
+  if (d->V == 0 || d->V > kMostSize || d->B > 65535 || d->L < 0 || d->L > kMostSize || !d->logits || !d->out || d->ld < d->V || d->ldo < d->V)
     return (int)hipErrorInvalidValue;
   if (d->history && ((d->ids_bytes != 4 && d->ids_bytes != 8) || d->ldh < d->L)) return (int)hipErrorInvalidValue;
   if ((d->allowed_bits && d->allowed_bytes) || (d->bias && d->ldb != 0 && d->ldb < d->V) ||

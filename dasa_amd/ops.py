@@ -1157,8 +1157,8 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     vocab = int(vocab)
     if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise _lib.DasaError(f"embedding_bwd: dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)}")
-    if vocab < 0 or vocab >= 2**31 or ids.numel() >= 2**31 - 65536:
-        raise _lib.DasaError("embedding_bwd: the vocabulary and the tokens must be fewer than 2^31")
+    if vocab < 0 or vocab > 2**30 or ids.numel() >= 2**31 - 65536:
+        raise _lib.DasaError("embedding_bwd: at most 2^30 ids in the vocabulary and 2^31 - 65536 tokens")
     if padding_idx is None:
         padding_idx = -1
     elif not 0 <= padding_idx < vocab:

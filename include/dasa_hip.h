@@ -365,7 +365,8 @@ int dasa_gather_rows(const float* ta, const int32_t* ia, int32_t Fa, const float
 /* ---- token embedding (model.py:1061 SpeakerDecoder.embedding, vilmodel.py:161-176 word embeddings) ----------
  * out[i] = scale * table[ids[i]] for T contiguous ids (ids_bytes 4 or 8: int32 / int64), rows of E elements, fp32
  * (bf16 = 0) or bf16 (bf16 = 1; the product is rounded once, RNE). A negative id gives a zero row; an id >= V gives
- * a NaN row and ORs 8 into *err (may be NULL); no memory outside the table is read. ldt / ldo are row strides. */
+ * a NaN row and ORs 8 into *err (may be NULL); no memory outside the table is read. ldt / ldo are row strides. V and E
+ * at most 2^30, here and in the gradient. */
 int dasa_embedding_fwd(const void* table, int64_t ldt, const void* ids, int32_t ids_bytes, int64_t T, int32_t V,
                        int32_t E, float scale, int32_t bf16, void* out, int64_t ldo, uint32_t* err, void* stream);
 /* Its gradient: dtable[v] (+= if accumulate) scale * sum over i with ids[i] == v of dout[i], summed in fp32 in an
@@ -383,7 +384,7 @@ int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t i
  * dasa_w4_quantize: W [N][ldw] (fp32 / bf16) -> codes [N][ldc] (two a byte, the even k in the low half) and scales
  * [N][lds] (fp32 / bf16), s = max |w| / 7 rounded to its type, q = clamp(rne(w / s), -8, 7) + 8; W must be finite.
  * dasa_w4_layout: codes / scales -> the tiles that dasa_gemm_w4 reads: `weight` (dasa_w4_weight_bytes, 16-B
- * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. */
+ * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. N and K at most 2^30. */
 int64_t dasa_w4_weight_bytes(int32_t N, int32_t K);
 int64_t dasa_w4_scale_count(int32_t N, int32_t K, int32_t group);
 int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int32_t K, int32_t group, uint8_t* codes,
@@ -391,7 +392,7 @@ int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int3
 int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16, int32_t N,
                    int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream);
 /* y = act(x W^T + bias) + beta * y: x [M][ldx], y [M][ldy], both fp32 (bf16 = 0) or both bf16; fp32 accumulation at
- * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. Any M, N, K; made for few rows.
+ * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. M at most 1048560; made for few rows.
  * ws: dasa_gemm_w4_workspace(M, N, K, bf16) bytes of scratch, 16-B aligned (0: none). */
 int64_t dasa_gemm_w4_workspace(int32_t M, int32_t N, int32_t K, int32_t bf16);
 int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, const void* scale_tiles,
@@ -407,7 +408,8 @@ int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, c
  * history [B][ldh] int32 / int64 (ids_bytes) or NULL; lengths [B] or NULL (all L); repetition / presence /
  * frequency [B] or NULL (then the numbers *0); bias [V] (ldb = 0) or [B][ldb] or NULL; allowed as bits (bit v % 32
  * of word v / 32; ldbits = 0 shared) or as bytes (0 = not allowed; ldbytes = 0 shared) or neither.
- * ws: dasa_logit_rules_workspace(B, V) bytes of scratch, needed if choice is asked for. B <= 65535. */
+ * ws: dasa_logit_rules_workspace(B, V) bytes of scratch, needed if choice is asked for. B <= 65535, V and L
+ * at most 2^30. */
 typedef struct dasa_logit_rules_desc {
   const void* logits; int64_t ld;
   void* out; int64_t ldo;

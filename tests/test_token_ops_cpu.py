@@ -75,7 +75,8 @@ def test_entry_points_refuse_before_a_launch():
     P = 0x100000
     assert L.dasa_embedding_fwd(P, 8, P, 8, 0, 10, 8, 1.0, 0, P, 8, None, None) == 0           # no tokens
     for T, V, E, nb, ldt, ldo in ((-1, 10, 8, 8, 8, 8), (4, 0, 8, 8, 8, 8), (4, 10, 8, 2, 8, 8), (4, 10, 8, 8, 7, 8),
-                                  (4, 10, 8, 8, 8, 7), (4, -1, 8, 8, 8, 8)):
+                                  (4, 10, 8, 8, 8, 7), (4, -1, 8, 8, 8, 8), (4, 2**30 + 1, 8, 8, 8, 8),
+                                  (4, 10, 2**30 + 1, 8, 2**31, 2**31)):
         assert L.dasa_embedding_fwd(P, ldt, P, nb, T, V, E, 1.0, 0, P, ldo, None, None) == INVALID
     assert L.dasa_embedding_fwd(None, 8, P, 8, 4, 10, 8, 1.0, 0, P, 8, None, None) == INVALID
     assert L.dasa_embedding_bwd_workspace(2**31, 50, 8) == 0 and L.dasa_embedding_bwd_workspace(100, 50, 8) == 0
@@ -87,6 +88,10 @@ def test_entry_points_refuse_before_a_launch():
                                    (-1, 8, 8, 8, P, need), (100, 8, 7, 8, None, 0), (100, 8, 8, 7, None, 0)):
         assert L.dasa_embedding_bwd(P, ldd, P, nb, T, 50, 8, 1.0, -1, 0, P, ldt, 0, ws, n, None) == INVALID
     assert L.dasa_w4_weight_bytes(17, 129) == 2 * 2 * 1024 and L.dasa_w4_weight_bytes(0, 4) == 0
+    assert L.dasa_embedding_bwd(P, 8, P, 8, T0, 2**30 + 1, 8, 1.0, -1, 0, P, 8, 0, P, 2**40, None) == INVALID
+    assert L.dasa_w4_weight_bytes(2**30 + 1, 64) == 0 and L.dasa_w4_weight_bytes(64, 2**31 - 1) == 0
+    assert L.dasa_gemm_w4(P, 2**31, 0, P, P, 0, 64, None, 0, 0.0, P, 4, 1, 4, 2**31 - 1, None, 0, None) == INVALID
+    assert L.dasa_gemm_w4(P, 64, 0, P, P, 0, 64, None, 0, 0.0, P, 4, 65535 * 16 + 1, 4, 64, None, 0, None) == INVALID
     assert L.dasa_w4_scale_count(17, 129, 64) == 2 * 2 * 2 * 16 and L.dasa_w4_scale_count(17, 129, 16) == 0
     assert L.dasa_w4_quantize(P, 64, 0, 4, 64, 16, P, 32, P, 4, 0, None) == INVALID
     assert L.dasa_w4_quantize(P, 63, 0, 4, 64, 64, P, 32, P, 1, 0, None) == INVALID
@@ -103,6 +108,7 @@ def test_entry_points_refuse_before_a_launch():
         return ctypes.byref(d)
     for kw in (dict(V=0), dict(B=-1), dict(B=65536), dict(ld=8999), dict(ldo=8999), dict(ids_bytes=3), dict(ldh=3),
                dict(logits=None), dict(L=-1), dict(bias=P, ldb=8999), dict(allowed_bits=P, ldbits=281),
-               dict(allowed_bytes=P, ldbytes=8999), dict(allowed_bits=P, allowed_bytes=P), dict(choice=P)):
+               dict(allowed_bytes=P, ldbytes=8999), dict(allowed_bits=P, allowed_bytes=P), dict(choice=P),
+               dict(V=2**30 + 1, ld=2**31, ldo=2**31), dict(L=2**30 + 1, ldh=2**31)):
         assert L.dasa_logit_rules(desc(**kw), None, 0, None) == INVALID, kw
     assert L.dasa_logit_rules(desc(B=0), None, 0, None) == 0
