@@ -65,7 +65,8 @@ union Frag {
 // (each from one byte of the word, whose low nibble counts), four merges of the high halves, which hold it all
 __device__ __forceinline__ bf16x8 unpack8(unsigned w) {
   Frag f;
-  const unsigned h = w >> 4;
+  unsigned h = w >> 4;
+  asm("" : "+v"(h));      // kept: extracting the odd nibbles from w takes an instruction each (64 x 14336 x 4096 bf16 22.3 us)
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const float e = __builtin_amdgcn_cvt_off_f32_i4((int)((w >> (8 * b)) & 255u));
@@ -134,18 +135,19 @@ template <> struct XFrag<__bf16> {
   static __device__ __forceinline__ void planes(const Raw& r, bf16x8 (&f)[1]) { f[0] = r.v; }
 };
 
-// the GPB scales of one column of one block
-template <class S, int GPB>
-__device__ __forceinline__ void load_scales(const void* scales, long at, float (&sc)[GPB]) {
+// The GPB scales of one column of one block, in their type: widening them where they are loaded would wait for them there
+// (64 x 32768 x 8192, scales bf16: 61.1 us against 55.8).
+template <class S, int GPB> struct Scales {
   typedef S V __attribute__((ext_vector_type(GPB)));
-  if constexpr (GPB == 1) {
-    sc[0] = (float)reinterpret_cast<const S*>(scales)[at];
-  } else {
-    const V v = reinterpret_cast<const V*>(scales)[at];
-#pragma unroll
-    for (int g = 0; g < GPB; ++g) sc[g] = (float)v[g];
-  }
-}
+  V v;
+  __device__ __forceinline__ void load(const void* scales, long at) { v = reinterpret_cast<const V*>(scales)[at]; }
+  __device__ __forceinline__ float operator[](int g) const { return (float)v[g]; }
+};
+template <class S> struct Scales<S, 1> {
+  S v;
+  __device__ __forceinline__ void load(const void* scales, long at) { v = reinterpret_cast<const S*>(scales)[at]; }
+  __device__ __forceinline__ float operator[](int) const { return (float)v; }
+};
 
 // four consecutive rows of one output column
 template <class T>
@@ -225,11 +227,11 @@ __global__ __launch_bounds__(64 * W, 4) void w4_split_kernel(W4Args a) {
   auto block = [&](int kb, auto tail) {
     constexpr bool TAIL = decltype(tail)::value;
     uint4 wq[NT];
-    float sc[NT][GPB];
+    Scales<S, GPB> sc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       wq[t] = a.w[(blk0[t] + kb) * 64 + lane];
-      load_scales<S, GPB>(a.scales, (blk0[t] + kb) * 16 + c16, sc[t]);
+      sc[t].load(a.scales, (blk0[t] + kb) * 16 + c16);
     }
     typename X::Raw raw[4];
 #pragma unroll
@@ -279,14 +281,18 @@ __global__ __launch_bounds__(64 * W, 4) void w4_split_kernel(W4Args a) {
 }
 
 constexpr int kShareWaves = 8;
-constexpr int kAhead = 4;       // even: the two activation buffers keep their places over a turn of the ring
 
 // The form for more rows: the workgroup's waves own NT column blocks each and walk K together, so the activations'
 // fragments are split into their planes once for the 8 NT blocks, in LDS (two buffers, one barrier a 128-deep block),
 // where each wave reads them back in fragment order.
-template <class T, class S, int MT, int NT, int GPB>
+// TAIL: K ends inside a block (a branch at every load of x otherwise).
+template <class T, class S, int MT, int NT, int GPB, bool TAIL>
 __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a) {
   typedef XFrag<T> X;
+  // weights are asked for AHEAD - 1 blocks early (even: the two activation buffers keep their places over a turn of the
+  // ring). Three early only pay for a long K with registers left (64 x 16384 x 4096 bf16 19.9 us against 21.6; 64 x 30522
+  // x 768 bf16 11.0 against 9.9 with one, fp32 16.6 against 15.7)
+  constexpr int AHEAD = X::PL == 1 && NT > 1 ? 4 : 2;
   constexpr int PL = X::PL, UNITS = MT * 4, PER = (UNITS + kShareWaves - 1) / kShareWaves;   // fragments a wave makes
   extern __shared__ float4 smem[];
   bf16x8* frag = reinterpret_cast<bf16x8*>(smem);       // [2][PL][4 steps][MT][64]
@@ -299,7 +305,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
 #pragma unroll
     for (int m = 0; m < MT; ++m) y[t][m] = floatx4{0.f, 0.f, 0.f, 0.f};
   const int k0 = blockIdx.z * a.per, k1 = min(k0 + a.per, a.Kb);
-  typename X::Raw raw[2][PER];           // activations two blocks ahead, weights kAhead
+  typename X::Raw raw[2][PER];           // activations two blocks ahead
   auto fetch = [&](int kb, typename X::Raw (&r)[PER]) {
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
       if (UNITS % kShareWaves && f >= UNITS) continue;
       const int m = f % MT, k = kb * 128 + (f / MT) * 32 + kq * 8;
       const T* p = reinterpret_cast<const T*>(a.x) + (long)min(m0 + m * 16 + c16, a.M - 1) * a.ldx + k;
-      r[u] = kb * 128 + 128 <= a.K ? X::load(p) : X::load_part(p, a.K - k);
+      r[u] = !TAIL || kb * 128 + 128 <= a.K ? X::load(p) : X::load_part(p, a.K - k);
     }
   };
   auto put = [&](int buf, const typename X::Raw (&r)[PER]) {
@@ -321,17 +327,17 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
       for (int p = 0; p < PL; ++p) frag[((buf * PL + p) * UNITS + f) * 64 + lane] = q[p];
     }
   };
-  uint4 wq[kAhead][NT];
-  float sc[kAhead][NT][GPB];
-  auto weights = [&](int kb, uint4 (&q)[NT], float (&s)[NT][GPB]) {
+  uint4 wq[AHEAD][NT];
+  Scales<S, GPB> sc[AHEAD][NT];
+  auto weights = [&](int kb, uint4 (&q)[NT], Scales<S, GPB> (&s)[NT]) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const long b = (long)min(nt0 + t, a.N16 - 1) * a.Kb + kb;
       q[t] = a.w[b * 64 + lane];
-      load_scales<S, GPB>(a.scales, b * 16 + c16, s[t]);
+      s[t].load(a.scales, b * 16 + c16);
     }
   };
-  auto compute = [&](int buf, const uint4 (&q)[NT], const float (&s)[NT][GPB]) {
+  auto compute = [&](int buf, const uint4 (&q)[NT], const Scales<S, GPB> (&s)[NT]) {
     floatx4 acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -357,20 +363,20 @@ __global__ __launch_bounds__(64 * kShareWaves, 2) void w4_shared_kernel(W4Args a
     }
   };
   if (k0 < k1) {                          // blocks past the last are the last again: loads without branches
+    fetch(k0, raw[0]);
+    weights(k0, wq[0], sc[0]);
+    fetch(min(k0 + 1, k1 - 1), raw[1]);
 #pragma unroll
-    for (int i = 0; i < kAhead - 1; ++i) {
-      if (i < 2) fetch(min(k0 + i, k1 - 1), raw[i]);
-      weights(min(k0 + i, k1 - 1), wq[i], sc[i]);
-    }
+    for (int i = 1; i < AHEAD - 1; ++i) weights(min(k0 + i, k1 - 1), wq[i], sc[i]);
     put(0, raw[0]);
   }
   __syncthreads();
-  for (int kb = k0; kb < k1; kb += kAhead) {
+  for (int kb = k0; kb < k1; kb += AHEAD) {
 #pragma unroll
-    for (int h = 0; h < kAhead; ++h) {
+    for (int h = 0; h < AHEAD; ++h) {
       if (kb + h >= k1) break;
       fetch(min(kb + h + 2, k1 - 1), raw[h & 1]);
-      weights(min(kb + h + kAhead - 1, k1 - 1), wq[(h + kAhead - 1) % kAhead], sc[(h + kAhead - 1) % kAhead]);
+      weights(min(kb + h + AHEAD - 1, k1 - 1), wq[(h + AHEAD - 1) % AHEAD], sc[(h + AHEAD - 1) % AHEAD]);
       compute(h & 1, wq[h], sc[h]);
       put((h & 1) ^ 1, raw[(h & 1) ^ 1]);
       __syncthreads();
@@ -441,9 +447,14 @@ int launch_shared(const W4Args& a, int g, int splits, hipStream_t st) {
   const dim3 grid((a.N16 + cols - 1) / cols, (a.M + 16 * MT - 1) / (16 * MT), splits), block(64 * kShareWaves);
   constexpr size_t frags = (size_t)2 * XFrag<T>::PL * 4 * MT * 64 * 16, tile = (size_t)16 * MT * (cols * 16 + 4) * 4;
   constexpr size_t lds = frags > tile ? frags : tile;
-  if (g == 32) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 4>), grid, block, lds, st, a);
-  else if (g == 64) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 2>), grid, block, lds, st, a);
-  else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, 1>), grid, block, lds, st, a);
+  auto go = [&](auto gpb) {
+    constexpr int GPB = decltype(gpb)::value;
+    if (a.K % 128) hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, GPB, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((w4_shared_kernel<T, S, MT, NT, GPB, false>), grid, block, lds, st, a);
+  };
+  if (g == 32) go(std::integral_constant<int, 4>{});
+  else if (g == 64) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 1>{});
   DASA_CHECK_LAUNCH();
   return launch_join<T>(a, splits, (int)grid.y * MT, st);
 }

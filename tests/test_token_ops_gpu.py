@@ -258,7 +258,8 @@ def test_w4_weight_values(dev, N, K, group):
                                          (31, 50, 2241, 32), (33, 130, 127, 64), (64, 8200, 640, 128), (65, 33, 96, 32),
                                          (150, 8193, 255, 64), (1, 30522, 768, 32), (20, 30522, 200, 64),
                                          (64, 16384, 2100, 64), (40, 65536, 2041, 128), (3, 100, 8000, 32),
-                                         (20, 100, 8000, 64), (48, 2100, 300, 128)])
+                                         (20, 100, 8000, 64), (48, 2100, 300, 128), (20, 30522, 768, 64),
+                                         (33, 30522, 128, 128), (64, 16384, 2048, 32), (50, 65536, 2048, 128)])
 def test_linear_w4(dev, dtype, M, N, K, group):
     """Every form: 16 rows a workgroup with 1, 2 and 4 column blocks, K split over workgroups, 32 and 64 rows sharing
     their activations, rows and columns that end inside a tile, an inner size that ends inside a group."""
