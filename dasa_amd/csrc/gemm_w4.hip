@@ -13,18 +13,22 @@ namespace {
 using w4::Plan;
 using w4::W4Args;
 
-// Which form and shape: measured over M = 1 .. 64, N = 992 .. 32768, K = 256 .. 8192 in both types (us):
-//  * few weights per row tile (tiles x row tiles < 3500): the split form with each 16 rows a workgroup of their own.
-//    The weights come from cache for the second rows; holding several row tiles in a workgroup instead leaves the chip
-//    emptier (20 x 4096 x 2240 fp32 8.6 against 11.4, 64 x 992 x 512 fp32 4.1 against 7.8). Column blocks of a
-//    workgroup: as many as still leave about one workgroup a CU, since they share the activations' loads and their
-//    splitting into planes; up to eight bf16 rows, which need no splitting, stop at two (1 x 30522 x 768 bf16 5.1
-//    against 5.9, 16 rows 7.3 against 6.9; 32768 x 8192: one row 30.0 against 30.9, 16 rows 43.0 against 33.9).
-//  * many weights and more than 16 rows: the shared form (64 x 30522 x 768 bf16 11.8 against 19.8, 64 x 16384 x 4096
-//    fp32 35.7 against 39), two row tiles a workgroup, four where the weights are too many to read twice
-//    (64 x 32768 x 8192 bf16 63 against 83). A wave takes two column blocks, one where K is short and the loop is
-//    mostly its start and end (33 x 32768 x 1024 bf16 11.5 against 13.3; three planes a row want two from three row
-//    tiles on, 64 x 30522 x 768 fp32 17.2 against 18.8).
+// Which form and shape: measured over M = 1 .. 64, N = 992 .. 32768, K = 256 .. 8192 in both types (us). `units` counts
+// column blocks times 16-row tiles.
+//  * few units: the split form with each 16 rows a workgroup of their own. The weights come from cache for the second
+//    rows; holding several row tiles in a workgroup instead leaves the chip emptier (20 x 4096 x 2240 fp32 8.4 against
+//    11.4, 64 x 992 x 512 fp32 4.4 against 7.8). Column blocks of a workgroup: as many as still leave about one
+//    workgroup a CU, since they share the activations' loads and their splitting into planes; up to eight bf16 rows,
+//    which need no splitting, stop at two (1 x 30522 x 768 bf16 5.1 against 5.9, 16 rows 7.3 against 6.9; 32768 x 8192:
+//    one row 30.0 against 30.9, 16 rows 43.0 against 33.9).
+//  * many units and more than 16 rows: the shared form (64 x 30522 x 768 bf16 10.1 against 19.8). From 3500 units; a
+//    short K, which the split form cannot deal to its waves, from 2500 (20 x 20000 x 640 bf16 6.1 against 7.8, but
+//    33 x 16384 x 1024 fp32 13.3 against 10.8), a long one, which can be split over workgroups, from 1500 (33 x 8192 x
+//    8192 fp32 32.3 against 39.2, but 64 x 4096 x 8192 fp32 17.6 against 14.5).
+//    Two row tiles a workgroup, four where the weights are too many to read twice (64 x 32768 x 8192 bf16 63 against
+//    83). Two column blocks a wave if that still fills five eighths of the chip (64 x 16384 x 1024 fp32 13.8 with one
+//    against 17.5; 64 x 12000 x 8192 fp32 55.7 with two against 77.9), one for a short K of bf16 rows, where the loop is
+//    mostly its start and end (33 x 32768 x 1024 bf16 11.5 against 13.3).
 //  * K is split over workgroups, at the price of a second launch (2 us), only where a long K leaves too few of them
 //    (1 x 1000 x 8192 fp32 7.7 against 13.4).
 inline Plan plan_of(int M, int N, int K, int bf16) {
@@ -34,12 +38,13 @@ inline Plan plan_of(int M, int N, int K, int bf16) {
   p.nt = 1;
   p.waves = 8;
   p.splits = 1;
-  if (rows > 1 && units >= 3500) {
+  if (rows > 1 && units >= (Kb >= 32 ? 1500 : Kb < 8 ? 2500 : 3500)) {
     p.shared = true;
     p.mt = rows > 2 && tiles * Kb >= 65536 ? 4 : 2;
-    p.nt = p.mt == 4 || Kb >= 16 || (rows > 2 && !bf16) ? 2 : 1;
-    const long wgs = (tiles + 8 * p.nt - 1) / (8 * p.nt) * ((rows + p.mt - 1) / p.mt);
-    p.splits = (int)std::max(1L, std::min(256 / wgs, Kb / 8));
+    auto wgs = [&](int nt) { return (tiles + 8 * nt - 1) / (8 * nt) * ((rows + p.mt - 1) / p.mt); };
+    auto splits = [&](int nt) { return (int)std::max(1L, std::min(256 / wgs(nt), Kb / 8)); };
+    p.nt = p.mt == 4 || (wgs(2) * splits(2) >= 160 && (Kb >= 16 || !bf16)) ? 2 : 1;
+    p.splits = splits(p.nt);
     return p;
   }
   if (Kb >= 48 && (!bf16 || rows > 1)) p.splits = (int)std::max(1L, std::min({Kb / 16, 4L, 1024 / units}));
