@@ -25,8 +25,8 @@ using w4::W4Args;
 //    short K, which the split form cannot deal to its waves, from 2500 (20 x 20000 x 640 bf16 6.1 against 7.8, but
 //    33 x 16384 x 1024 fp32 13.3 against 10.8), a long one, which can be split over workgroups, from 1500 (33 x 8192 x
 //    8192 fp32 32.3 against 39.2, but 64 x 4096 x 8192 fp32 17.6 against 14.5).
-//    Two row tiles a workgroup, four where the weights are too many to read twice (64 x 32768 x 8192 bf16 63 against
-//    83). Two column blocks a wave if that still fills five eighths of the chip (64 x 16384 x 1024 fp32 13.8 with one
+//    Two row tiles a workgroup, four where the weights are too many to read twice (64 x 12000 x 8192 bf16 24.7 against
+//    30.0). Two column blocks a wave if that still fills five eighths of the chip (64 x 16384 x 1024 fp32 13.8 with one
 //    against 17.5; 64 x 12000 x 8192 fp32 55.7 with two against 77.9), one for a short K of bf16 rows, where the loop is
 //    mostly its start and end (33 x 32768 x 1024 bf16 11.5 against 13.3).
 //  * K is split over workgroups, at the price of a second launch (2 us), only where a long K leaves too few of them
@@ -40,7 +40,7 @@ inline Plan plan_of(int M, int N, int K, int bf16) {
   p.splits = 1;
   if (rows > 1 && units >= (Kb >= 32 ? 1500 : Kb < 8 ? 2500 : 3500)) {
     p.shared = true;
-    p.mt = rows > 2 && tiles * Kb >= 65536 ? 4 : 2;
+    p.mt = rows > 2 && tiles * Kb >= 40000 ? 4 : 2;
     auto wgs = [&](int nt) { return (tiles + 8 * nt - 1) / (8 * nt) * ((rows + p.mt - 1) / p.mt); };
     auto splits = [&](int nt) { return (int)std::max(1L, std::min(256 / wgs(nt), Kb / 8)); };
     p.nt = p.mt == 4 || (wgs(2) * splits(2) >= 160 && (Kb >= 16 || !bf16)) ? 2 : 1;
