@@ -881,12 +881,45 @@ def mha(Q, K, V, addmask, heads, scale, p=0.0, training=False):
 
 
 # ----------------------------------------------------------------------------- token embedding
+class _Use:
+    """Lives as long as the autograd node that holds it."""
+    __slots__ = ("__weakref__",)
+
+
+_USES = {}     # id(leaf) -> (weakref(leaf), the live nodes of eager graphs on the default stream that use it)
+
+
+def _leaf_use(leaves):
+    """A _Use for a node of an eager graph over these leaves, or None inside a capture and on other streams. Refuses a
+    capture while such a graph of one of them lives: its gradient accumulator belongs to the default stream, which the
+    captured backward would wait for, and torch ends the process there (graph.AutogradGraphs captures over aliases)."""
+    leaves = [t for t in leaves if t.requires_grad and t.is_leaf]
+    if torch.cuda.is_current_stream_capturing():
+        for t in leaves:
+            e = _USES.get(id(t))
+            if e is not None and e[0]() is t and len(e[1]):
+                raise ops._lib.DasaError(f"an eager autograd graph of a {tuple(t.shape)} table lives while its training "
+                                         "step is captured: drop it first, or capture with graph.AutogradGraphs")
+        return None
+    if ops._stream() != 0:
+        return None
+    use = _Use()
+    for t in leaves:
+        e = _USES.get(id(t))
+        if e is None or e[0]() is not t:
+            e = _USES[id(t)] = (weakref.ref(t, lambda r, k=id(t): _USES.pop(k, None) if _USES.get(k, (None,))[0] is r
+                                            else None), weakref.WeakSet())
+        e[1].add(use)
+    return use
+
+
 class EmbeddingFn(torch.autograd.Function):
     """table[ids] * scale (nn.Embedding with a factor, model.py:1061); the table's gradient by sorted tokens."""
 
     @staticmethod
     def forward(ctx, ids, table, scale, padding_idx):
         ctx.scale, ctx.pad, ctx.vocab = scale, padding_idx, table.shape[0]
+        ctx.use = _leaf_use((table,))
         ctx.save_for_backward(ids)
         return ops.embedding(ids, table, scale=scale)
 
@@ -913,6 +946,7 @@ class BertEmbedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, word, pos, types, gamma, beta, eps, p, seed, padding_idx):
         ctx.eps, ctx.p, ctx.seed, ctx.pad = eps, p, seed, padding_idx
+        ctx.use = _leaf_use((word, pos, types, gamma, beta))
         ctx.save_for_backward(ids)
         ctx.params = _Kept((word, pos, types, gamma, beta))
         return ops.bert_embed(ids, word, pos, types[0], gamma, beta, eps, p, seed)

@@ -112,3 +112,28 @@ def test_entry_points_refuse_before_a_launch():
                dict(V=2**30 + 1, ld=2**31, ldo=2**31), dict(L=2**30 + 1, ldh=2**31)):
         assert L.dasa_logit_rules(desc(**kw), None, 0, None) == INVALID, kw
     assert L.dasa_logit_rules(desc(B=0), None, 0, None) == 0
+
+
+def test_capture_beside_a_live_eager_graph_is_refused(monkeypatch):
+    """functional's record of live eager graphs, with the stream and the capture state of a device played by the host."""
+    from dasa_amd import functional as DF
+    state = dict(capturing=False, stream=0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(ops, "_stream", lambda: state["stream"])
+    table, other = torch.zeros(4, 2, requires_grad=True), torch.zeros(4, 2, requires_grad=True)
+    use = DF._leaf_use((table, torch.zeros(3)))
+    state["capturing"] = True
+    assert DF._leaf_use((other,)) is None
+    _refused("AutogradGraphs", DF._leaf_use, (other, table))
+    del use                                                    # the eager graph is gone
+    assert DF._leaf_use((table,)) is None
+    state.update(capturing=False, stream=7)                    # a warm-up on a side stream
+    assert DF._leaf_use((table,)) is None
+    state.update(capturing=True)
+    assert DF._leaf_use((table,)) is None
+    key = id(other)
+    state.update(capturing=False, stream=0)
+    keep = DF._leaf_use((other,))
+    assert key in DF._USES
+    del other
+    assert key not in DF._USES and keep is not None

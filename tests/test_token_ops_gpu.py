@@ -215,6 +215,36 @@ def test_embedding_in_a_captured_training_region(dev):
     assert region.captures == 1
 
 
+def test_capture_beside_an_eager_graph_of_the_table_is_refused(dev):
+    """Before anything is recorded; once the eager graph is gone, forward and backward are captured and replayed."""
+    table = torch.randn(50, 16, device=dev).requires_grad_()
+    ids = torch.arange(12, device=dev)
+    dy = torch.randn(12, 16, device=dev)
+    ops.check_device_errors()
+    y = DF.embedding(ids, table)
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=st):
+        one = torch.ones(4, device=dev)
+        with pytest.raises(DasaError, match="AutogradGraphs"):
+            DF.embedding(ids, table)
+        with torch.no_grad():
+            z = DF.embedding(ids, table)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(z, table.detach()[:12]) and float(one.sum()) == 4.0
+    del y
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        grad, = torch.autograd.grad(DF.embedding(ids, table), table, dy)
+    for i in range(3):
+        ids.copy_(torch.randperm(50, generator=_gen(i))[:12].to(dev))
+        want = ops.embedding_bwd(dy, ids, 50)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+
+
 # ------------------------------------------------------------------------------------------ 4-bit weights
 def _w4(N, K, group, sdt, seed):
     g = _gen(seed)
