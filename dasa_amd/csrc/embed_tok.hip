@@ -19,8 +19,8 @@
 //                  (its base), and writes its tokens' positions at their stable rank. No workgroup waits for another.
 //   above          token_count_kernel, token_place_kernel, rows, join: reading every id in every workgroup is what
 //                  bounds the one-launch sort there.
-//                  (131072 x 1024 bf16, a third of them padding, into 50021 rows: 7.1 + 16.2 us sort, 73.5 rows
-//                  (174 MB read, 102 MB written: 3.8 TB/s; a large sum reads at 4.0), 8.6 join.)
+//                  (131072 x 1024 bf16, a third of them padding, into 50021 rows: 7.0 + 16.1 us sort, 72.5 rows
+//                  (174 MB read, 102 MB written: 3.8 TB/s; a large sum reads at 4.0), 7.9 join.)
 #include "common.h"
 #include "../../include/dasa_hip.h"
 
@@ -475,8 +475,8 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a
   });
 }
 
-// One launch against two, 50021 ids, Zipf / uniform / one id: 49152 tokens x 64 bf16, the whole gradient, 34.4 / 28.9 /
-// 64.7 us against 33.6 / 30.8 / 45.3; 131072 tokens, the sort alone, 39 / 30 / 72 against 27.5 / 27.9 / 25.5. Above
+// One launch against two, 50021 ids, Zipf / uniform / one id: 49152 tokens x 64 bf16, the whole gradient, 33.1 / 28.7 /
+// 51.2 us against 30.6 / 30.5 / 30.6; 131072 tokens, the sort alone, 39 / 30 / 72 against 25.4 / 27.7 / 26.4. Above
 // 4 M tokens the counts of the segments would outgrow the tokens.
 constexpr long kManyTokens = 49152, kMostTokens = 4 << 20;
 
@@ -527,8 +527,11 @@ __device__ __forceinline__ Unit unit_of(int unit, int E) {
 // A table row of up to kChunk tokens is summed by one wave per slice of 64 units. Longer (hot) rows are cut at the
 // multiples of kChunk in the sorted order, so that a padding or stop word with a tenth of the tokens does not run on
 // one wave: each chunk leaves the sum of its part of at most two hot rows (one that reaches into it, one that reaches
-// out of it: a hot row is longer than a chunk), and a third launch adds a row's parts in chunk order.
+// out of it: a hot row is longer than a chunk), and a third launch adds a row's parts in chunk order. Where one row owns
+// all chunks of a workgroup, the workgroup leaves one sum, in its first chunk's place (131072 x 1024 bf16 of one id: the
+// join 145 -> 37 us; of Zipf ids 14.7 -> 9.1).
 constexpr int kChunk = 32;
+constexpr int kRowWaves = 4;
 constexpr int kJoinWaves = 16;
 
 struct BwdArgs {
@@ -590,8 +593,9 @@ __device__ __forceinline__ long id_at(const BwdArgs& a, int pos) {
 
 // One wave = (table row, slice) or (chunk, slice).
 template <class T, bool NARROW>
-__global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
+__global__ __launch_bounds__(64 * kRowWaves) void embedding_bwd_rows_kernel(BwdArgs a) {
   constexpr int N = Vec<T>::N;
+  __shared__ float sum[kRowWaves][64][N];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const auto [col, skip, live] = unit_of<T>(blockIdx.y * 64 + lane, a.E);
   const T* d = reinterpret_cast<const T*>(a.dout) + col;
@@ -599,7 +603,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
   if (blockIdx.x >= a.chunk_blocks) {
-    const long v = (long)(blockIdx.x - a.chunk_blocks) * 4 + w;
+    const long v = (long)(blockIdx.x - a.chunk_blocks) * kRowWaves + w;
     if (v >= a.V) return;
     const int* at = a.start + a.own.place((unsigned)v);
     const int s = at[0], n = at[1] - s;
@@ -609,7 +613,7 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
     if (live) write_row<T, NARROW>(a, v, col, skip, acc);
     return;
   }
-  const long c = (long)blockIdx.x * 4 + w;
+  const long c = (long)blockIdx.x * kRowWaves + w;
   const int j0 = (int)(c * kChunk), total = a.start[a.bins];
   if (j0 >= total) return;
   const int m = min(kChunk, total - j0);
@@ -618,6 +622,21 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   const int rs = at[0], re = at[1];
   const bool hot = re - rs > kChunk;
   float* part = a.parts + c * 2 * a.ldp + col;
+  const long b0 = (long)blockIdx.x * kRowWaves * kChunk;
+  const bool whole = rs <= b0 && re >= b0 + kRowWaves * kChunk;
+  if (__builtin_amdgcn_readlane((int)whole, 0)) {          // of the first token, then of every token of the workgroup
+    add_rows<T, NARROW>(acc, d, a.ldd, a.E, pos, 0, m);
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
+    __syncthreads();
+    if (w != 0 || !live) return;
+    for (int k = 1; k < kRowWaves; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += sum[k][lane][e];
+#pragma unroll
+    for (int e = 0; e < N; ++e) part[e] = acc[e];
+    return;
+  }
   // the row that owns the chunk's first token, then the row that owns its last
   const int ea = __builtin_amdgcn_readlane(hot ? min(re - j0, m) : 0, 0);
   if (ea > 0) {
@@ -637,15 +656,33 @@ __global__ __launch_bounds__(256) void embedding_bwd_rows_kernel(BwdArgs a) {
   }
 }
 
-// parts [k0, k1) of the hot row whose first part is slot `first` of chunk c, added in order, eight in flight
+// Where the sums of a hot row's sorted places [rs, re) are: chunks, whole workgroups of them, chunks.
+struct Parts {
+  int c0, first, head, b0, whole, n;
+  __device__ __forceinline__ Parts(int rs, int re) {
+    constexpr int B = kRowWaves * kChunk;
+    c0 = rs / kChunk;
+    first = rs > c0 * kChunk;                     // the slot of the first chunk: another row owns its first token
+    const int last = (re - 1) / kChunk, lo = (int)(((long)rs + B - 1) / B), hi = re / B;
+    b0 = lo;
+    whole = max(hi - lo, 0);
+    head = whole ? lo * kRowWaves - c0 : last + 1 - c0;
+    n = whole ? head + whole + last + 1 - hi * kRowWaves : head;
+  }
+  __device__ __forceinline__ long place(int i) const {
+    if (i < head) return (long)(c0 + i) * 2 + (i == 0 ? first : 0);
+    if (i < head + whole) return (long)(b0 + i - head) * kRowWaves * 2;
+    return (long)((b0 + whole) * kRowWaves + i - head - whole) * 2;
+  }
+};
+
+// parts [k0, k1) of a hot row, added in order, eight in flight
 template <class T>
-__device__ __forceinline__ void add_parts(float (&acc)[Vec<T>::N], const BwdArgs& a, long c, int first, int k0, int k1,
+__device__ __forceinline__ void add_parts(float (&acc)[Vec<T>::N], const BwdArgs& a, const Parts& p, int k0, int k1,
                                           int col) {
   constexpr int N = Vec<T>::N, K = 8;
   typedef float V __attribute__((ext_vector_type(N), aligned(4)));
-  auto part = [&](int k) {
-    return *reinterpret_cast<const V*>(a.parts + ((c + k) * 2 + (k == 0 ? first : 0)) * a.ldp + col);
-  };
+  auto part = [&](int k) { return *reinterpret_cast<const V*>(a.parts + p.place(k) * a.ldp + col); };
   int k = k0;
   for (; k + K <= k1; k += K) {
     V x[K];
@@ -683,9 +720,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   if (j0 < total) {
     const long v = id_at(a, a.order[min(j0 + kChunk, (long)total) - 1]);
     const int* at = a.start + a.own.place((unsigned)v);
-    const int rs = at[0], re = at[1], n = (re - 1) / kChunk - (int)c + 1;
-    if (re - rs > kChunk && rs >= j0 && n <= kJoinWaves) {
-      add_parts<T>(acc, a, c, rs > j0, 0, n, col);
+    const int rs = at[0], re = at[1];
+    const Parts p(rs, re);
+    if (re - rs > kChunk && rs >= j0 && p.n <= kJoinWaves) {
+      add_parts<T>(acc, a, p, 0, p.n, col);
       if (live) write_row<T, NARROW>(a, v, col, skip, acc);
     }
   }
@@ -694,12 +732,13 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
   const long v = id_at(a, a.order[min(g0 + kJoinWaves * kChunk, (long)total) - 1]);
   const int* at = a.start + a.own.place((unsigned)v);
   const int rs = at[0], re = at[1];
-  const int c0 = rs / kChunk, n = (re - 1) / kChunk - c0 + 1;
+  const Parts p(rs, re);
+  const int n = p.n;
   if (rs < g0 || n <= kJoinWaves) return;
   const int per = (n + kJoinWaves - 1) / kJoinWaves, k0 = min(w * per, n), k1 = min(k0 + per, n);
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  add_parts<T>(acc, a, c0, rs > c0 * kChunk, k0, k1, col);
+  add_parts<T>(acc, a, p, k0, k1, col);
 #pragma unroll
   for (int e = 0; e < N; ++e) sum[w][lane][e] = acc[e];
   __syncthreads();
@@ -953,9 +992,9 @@ template <class T, bool NARROW>
 int launch_rows_as(BwdArgs a, long tokens, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   const long chunks = (tokens + kChunk - 1) / kChunk;
-  a.chunk_blocks = (unsigned)((chunks + 3) / 4);
-  const dim3 grid(a.chunk_blocks + (unsigned)((a.V + 3) / 4), slices);
-  hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, NARROW>), grid, dim3(256), 0, st, a);
+  a.chunk_blocks = (unsigned)((chunks + kRowWaves - 1) / kRowWaves);
+  const dim3 grid(a.chunk_blocks + (unsigned)((a.V + kRowWaves - 1) / kRowWaves), slices);
+  hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, NARROW>), grid, dim3(64 * kRowWaves), 0, st, a);
   DASA_CHECK_LAUNCH();
   hipLaunchKernelGGL((embedding_bwd_join_kernel<T, NARROW>), dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
                      dim3(64 * kJoinWaves), 0, st, a);
