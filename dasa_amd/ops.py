@@ -5,6 +5,7 @@ libdasa_hip.so on torch's current stream (so torch.cuda.graph capture records th
 CPU path: a CPU tensor is a usage error and raises.
 """
 import ctypes
+import functools
 import math
 import os
 import weakref
@@ -1073,9 +1074,17 @@ def _ids_bytes(ids, what):
     return k
 
 
+@functools.lru_cache(4096)
+def _workspace_bytes(entry, *sizes):
+    """A token operator's workspace query, which depends on the sizes alone."""
+    return getattr(_lib.lib(), entry)(*sizes)
+
+
 def _row_view(t, what):
-    """[..., N] as (2-D tensor of unit inner stride, rows, row stride >= N): a copy where the layout needs one."""
+    """[..., N] as (tensor of rows of unit inner stride, rows, row stride >= N): a copy where the layout needs one."""
     N = t.shape[-1]
+    if N and t.is_contiguous():
+        return t, t.numel() // N, N
     if t.dim() != 2:
         t = t.reshape(-1, N)
     if N and t.shape[0] and ((N > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < N)):
@@ -1176,7 +1185,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     d, T, ldd = _row_view(dout, "embedding_bwd")
     ids = ids.contiguous()
     L = _lib.lib()
-    nws = L.dasa_embedding_bwd_workspace(T, vocab, E)
+    nws = _workspace_bytes("dasa_embedding_bwd_workspace", T, vocab, E)
     ws = torch.empty(nws, dtype=torch.uint8, device=dout.device) if nws else None
     _call("dasa_embedding_bwd", "embed_bwd", L.dasa_embedding_bwd, d.data_ptr(), ldd, ids.data_ptr(), nb, T, vocab, E,
           float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0,
@@ -1291,7 +1300,7 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     if M == 0:
         return out
     L = _lib.lib()
-    nws = L.dasa_gemm_w4_workspace(M, N, K, bf16)
+    nws = _workspace_bytes("dasa_gemm_w4_workspace", M, N, K, bf16)
     ws = torch.empty(nws // 4, dtype=torch.float32, device=x.device) if nws else None
     _call("dasa_gemm_w4", "gemm_w4", L.dasa_gemm_w4, x2.data_ptr(), ldx, bf16, w.tiles.data_ptr(),
           w.scales.data_ptr(), 1 if w.scales.dtype == torch.bfloat16 else 0, w.group,
@@ -1387,7 +1396,7 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
         L = _lib.lib()
         ws, nws = None, 0
         if want_choice:
-            nws = L.dasa_logit_rules_workspace(B, V)
+            nws = _workspace_bytes("dasa_logit_rules_workspace", B, V)
             if nws:
                 ws = torch.empty(nws // 8, dtype=torch.int64, device=logits.device)
         d = _lib.LogitRules(logits.data_ptr(), max(logits.stride(0), V), out.data_ptr(), ldo, hist, ldh,
