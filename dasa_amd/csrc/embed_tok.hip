@@ -35,7 +35,8 @@ constexpr unsigned kErrTokenId = 8;   // bit of the error word (ops._ERR_BITS)
 // 16 bytes of a row. Rows of odd width or stride start anywhere, so the vector types are element-aligned (global loads
 // and stores take any alignment). The last unit of a row that is no multiple of them ends at the row's end and repeats
 // columns of the unit before it: no lane takes a partial load of its own, whose branch holds the wave's other loads up
-// (gradient of 4099 x 257 fp32 into 1001 rows: 12.2 us against 15.8; lookup of 131072 x 1001 bf16: 98 against 111). NARROW: rows of less than one unit.
+// (gradient of 4099 x 257 fp32 into 1001 rows: 12.2 us against 15.8; lookup of 131072 x 1001 bf16: 98 against
+// 111). NARROW: rows of less than one unit.
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
@@ -166,7 +167,8 @@ struct SortArgs {
   int* order;     // [T] positions in sorted order
 };
 
-inline Owners owners(int V, int least, int bins) {      // of at least `least` owners (if V has as many), `bins` bins at most
+// at least `least` owners (if V has as many), `bins` bins at most
+inline Owners owners(int V, int least, int bins) {
   Owners o{0, 0};
   while ((1 << o.lg) < least && (1 << o.lg) < V) ++o.lg;
   while (((long)V + (1L << o.lg) - 1) >> o.lg > bins) ++o.lg;
@@ -758,7 +760,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void embedding_bwd_join_kernel(Bwd
 //   Hot workgroups (first in the grid) = (larger share, slice of 16 units): the ids of more tokens (padding that no
 //   padding_idx names), which they find with a count of their share first, all groups together. The narrow slices put
 //   an id on several CUs: one CU reads a 1 KB row in 22 cycles, whatever is in flight (4096 x 768 fp32 of one id 139 us
-//   without the hot workgroups, 30 with them; 4099 x 257, two fifths of them one id, 36 and 16; they cost about 0.5 us
+//   without the hot workgroups, 30 with them; 4099 x 257, two fifths of them one id, 36 and 16; they cost about 1 us
 //   where there is no such id).
 constexpr int kFewTokens = 8192;
 constexpr int kFewWaves = 8;
@@ -891,7 +893,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
   }
   __syncthreads();
   int found = 0;
-  auto note = [&](int pos, int bin, bool in) {
+  auto note = [&](int pos, int bin, bool in, auto dense) {
     const unsigned long long m = __builtin_amdgcn_ballot_w64(in);
     if (!m) return;
     if (in) {
@@ -900,15 +902,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void embedding_bwd_few_kernel(Bw
       lbin[w * seg + at] = (unsigned short)bin;
     }
     found += __popcll(m);
-    add_bins<false>(hist[w], bin, in, m);
+    if constexpr (decltype(dense)::value) add_bins<false>(hist[w], bin, in, m);
+    else if (in) atomicAdd(&hist[w][bin], 1);
   };
   if (is_hot)
     each_token<W, 4>(ids, t0, t1, lane, [&](int pos, unsigned u) {
       const int bin = own.bin(u), number = own.owns(u) ? (share[bin >> 1] >> (16 * (bin & 1))) & 0xffff : 0;
-      note(pos, number - 1, number > 0);
+      note(pos, number - 1, number > 0, std::true_type{});
     });
   else
-    each_token<W, 4>(ids, t0, t1, lane, [&](int pos, unsigned u) { note(pos, own.bin(u), own.owns(u)); });
+    each_token<W, 4>(ids, t0, t1, lane,
+                     [&](int pos, unsigned u) { note(pos, own.bin(u), own.owns(u), std::false_type{}); });
   __syncthreads();
   int tot = 0;
   if (tid < n)

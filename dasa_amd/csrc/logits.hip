@@ -224,7 +224,8 @@ extern "C" int64_t dasa_logit_rules_workspace(int32_t B, int32_t V) {
 extern "C" int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_t ws_bytes, void* stream) {
   if (!d || d->B < 0 || d->V < 0) return (int)hipErrorInvalidValue;
   if (d->B == 0) return 0;
-  if (d->V == 0 || d->V > kMostSize || d->B > 65535 || d->L < 0 || d->L > kMostSize || !d->logits || !d->out || d->ld < d->V || d->ldo < d->V)
+  if (d->V == 0 || d->V > kMostSize || d->B > 65535 || d->L < 0 || d->L > kMostSize ||
+      !d->logits || !d->out || d->ld < d->V || d->ldo < d->V)
     return (int)hipErrorInvalidValue;
   if (d->history && ((d->ids_bytes != 4 && d->ids_bytes != 8) || d->ldh < d->L)) return (int)hipErrorInvalidValue;
   if ((d->allowed_bits && d->allowed_bytes) || (d->bias && d->ldb != 0 && d->ldb < d->V) ||

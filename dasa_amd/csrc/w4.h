@@ -67,7 +67,7 @@ union Frag {
 __device__ __forceinline__ bf16x8 unpack8(unsigned w) {
   Frag f;
   unsigned h = w >> 4;
-  asm("" : "+v"(h));      // kept: extracting the odd nibbles from w takes an instruction each (64 x 14336 x 4096 bf16 22.3 us)
+  asm("" : "+v"(h));      // kept: taking the odd nibbles out of w costs an instruction each (64 x 14336 x 4096: 22.3 us)
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const float e = __builtin_amdgcn_cvt_off_f32_i4((int)((w >> (8 * b)) & 255u));
