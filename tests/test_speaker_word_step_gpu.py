@@ -190,3 +190,53 @@ def test_bert_embeddings_gradients_with_dropout_regenerate_the_mask(dev):
     y.backward(torch.ones_like(y))
     want = (keep * 2.0).sum((0, 1))                             # d beta: the kept places times 1 / (1 - p)
     assert float((beta.grad.cpu().double() - want).abs().max()) < 1e-4
+
+
+def test_training_step_reaches_the_tables_on_request(dev):
+    """A finetune iteration of the agent with the language stack trained (--d_transformer_update True): with
+    --d_update_embeddings the tables and the LayerNorm of BertEmbeddings get gradients, and the loss and every other
+    gradient stay as without it."""
+    from dasa_amd import functional as DF
+    from dasa_amd.r2r import param
+    from dasa_amd.r2r.agent_dg import Seq2SeqAgent
+    from dasa_amd.synth import SynthR2RBatch, SynthWorld, init_params
+    res = {}
+    try:
+        for on in (False, True):
+            param.readme_finetune(["--d_vl_layers", "1", "--batchSize", "2", "--maxAction", "2",
+                                   "--d_transformer_update", "True"] + (["--d_update_embeddings"] if on else []))
+            torch.manual_seed(3)
+            env = SynthR2RBatch(SynthWorld(32, 0, 5), 2, seed=701, mode="wander", instr_len=80, variable_len=True)
+            with contextlib.redirect_stdout(io.StringIO()):
+                ag = Seq2SeqAgent(env, "", None, 2, "Dic")
+            for m, s in ((ag.encoder, 1), (ag.decoder, 2), (ag.critic, 3), (ag.adaIn, 4)):
+                init_params(m, s)
+                for sub in m.modules():
+                    if isinstance(sub, torch.nn.Dropout):
+                        sub.p = 0.0
+            param.args.ml_weight = param.args.ml_weight_org
+            assert ag.encoder.bert.update_lang_bert and ag.encoder.bert.embeddings.trained == on
+            table = GI.forced_table(2, 2, seed=GI.FORCED_SEED)
+            ag.force_action_fn = lambda t, lens, table=table: GI.forced_actions(table, t, lens, no_stop=True)
+            ag.zero_grad()
+            ag.accumulate_gradient("sample")
+            loss = ag.loss.item()
+            with DF.defer_bilstm_backward(), DF.defer_weight_grads():
+                ag.loss.backward()
+                DF.flush_bilstm_backward()
+            DF.flush_weight_grads()
+            res[on] = loss, {f"{i}.{k}": p.grad.detach().clone() for i, m in enumerate(ag.models)
+                             for k, p in m.named_parameters() if p.grad is not None}
+            del ag
+    finally:
+        param.readme_train(["--d_vl_layers", "1", "--batchSize", "2", "--maxAction", "5"])
+    (l0, g0), (l1, g1) = res[False], res[True]
+    new = {"0.bert.embeddings." + k for k in ("word_embeddings.weight", "position_embeddings.weight",
+                                              "token_type_embeddings.weight", "LayerNorm.weight", "LayerNorm.bias")}
+    assert l0 == l1 and set(g1) - set(g0) == new and set(g0) <= set(g1)
+    assert any(k.startswith("0.bert.lalayer") for k in g0)
+    for k in g0:                              # the same kernels on the same values: equal bit for bit
+        assert torch.equal(g0[k], g1[k]), k
+    for k in new:
+        assert bool(g1[k].isfinite().all()) and float(g1[k].abs().max()) > 0, k
+    assert bool((g1["0.bert.embeddings.word_embeddings.weight"][0] == 0).all())
