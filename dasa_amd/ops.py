@@ -1055,6 +1055,14 @@ def _on_device(what, *ts):
     return cur
 
 
+def _pair_device(what, a, b, out):
+    """_on_device for the two tensors (and perhaps an output) of a call that is little more than its launch."""
+    d = a.get_device()
+    if d < 0 or b.get_device() != d or _get_device() != d or (out is not None and out.get_device() != d):
+        return _on_device(what, a, b, out)
+    return d
+
+
 _FLOAT_TYPES = {torch.float32: 0, torch.bfloat16: 1}     # the bf16 argument of the entry points
 _ID_BYTES = {torch.int64: 8, torch.int32: 4}
 
@@ -1132,11 +1140,16 @@ def embedding(ids, table, scale=1.0, out=None):
     if table.dim() != 2:
         raise _lib.DasaError(f"embedding: table must be [V, E], got {tuple(table.shape)}")
     bf16, nb = _float_type(table, "embedding.table"), _ids_bytes(ids, "embedding.ids")
-    dev = _on_device("embedding", ids, table, out)
+    dev = _pair_device("embedding", ids, table, out)
     V, E = table.shape
-    if E > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < E:
-        raise _lib.DasaError("embedding: the table's rows must be contiguous")
-    ids = ids.contiguous()
+    if table.is_contiguous():
+        ldt = E
+    else:
+        ldt = max(table.stride(0), E)
+        if E > 1 and table.stride(1) != 1 or V > 1 and table.stride(0) < E:
+            raise _lib.DasaError("embedding: the table's rows must be contiguous")
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     if out is None:
         out = table.new_empty((*ids.shape, E))
         ldo = E
@@ -1150,9 +1163,9 @@ def embedding(ids, table, scale=1.0, out=None):
     err = _ERR.get(dev)
     if err is None and not torch.cuda.is_current_stream_capturing():
         err = _error_word(table.device)
-    _call("dasa_embedding_fwd", "embed", _lib.lib().dasa_embedding_fwd, table.data_ptr(), max(table.stride(0), E),
-          ids.data_ptr(), nb, T, V, E, float(scale), bf16, out.data_ptr(), ldo,
-          None if err is None else err.data_ptr(), _raw_stream(dev), nbytes=T * (nb + 2.0 * E * table.element_size()))
+    _call("dasa_embedding_fwd", "embed", _lib.lib().dasa_embedding_fwd, table.data_ptr(), ldt, ids.data_ptr(), nb, T, V,
+          E, float(scale), bf16, out.data_ptr(), ldo, None if err is None else err.data_ptr(), _raw_stream(dev),
+          nbytes=T * (nb + E * (4.0 if bf16 else 8.0)))
     return out
 
 
@@ -1162,9 +1175,9 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     padding_idx and of ids that do not occur are zero; ids outside the vocabulary are skipped. With out and
     accumulate=True the sums are added into out (rows without tokens are not touched)."""
     bf16, nb = _float_type(dout, "embedding_bwd.dout"), _ids_bytes(ids, "embedding_bwd.ids")
-    dev = _on_device("embedding_bwd", dout, ids, out)
+    dev = _pair_device("embedding_bwd", dout, ids, out)
     vocab = int(vocab)
-    if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+    if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:
         raise _lib.DasaError(f"embedding_bwd: dout {tuple(dout.shape)} does not match ids {tuple(ids.shape)}")
     if vocab < 0 or vocab > 2**30 or ids.numel() >= 2**31 - 65536:
         raise _lib.DasaError("embedding_bwd: at most 2^30 ids in the vocabulary and 2^31 - 65536 tokens")
@@ -1183,13 +1196,15 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     if vocab == 0 or E == 0:
         return out
     d, T, ldd = _row_view(dout, "embedding_bwd")
-    ids = ids.contiguous()
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     L = _lib.lib()
     nws = _workspace_bytes("dasa_embedding_bwd_workspace", T, vocab, E)
     ws = torch.empty(nws, dtype=torch.uint8, device=dout.device) if nws else None
     _call("dasa_embedding_bwd", "embed_bwd", L.dasa_embedding_bwd, d.data_ptr(), ldd, ids.data_ptr(), nb, T, vocab, E,
           float(scale), int(padding_idx), bf16, out.data_ptr(), ldo, 1 if accumulate else 0,
-          None if ws is None else ws.data_ptr(), nws, _raw_stream(dev), nbytes=T * (nb + 1.0 * E * dout.element_size()) + 1.0 * vocab * E * dout.element_size())
+          None if ws is None else ws.data_ptr(), nws, _raw_stream(dev),
+          nbytes=T * nb + (2.0 if bf16 else 4.0) * E * (T + vocab))
     return out
 
 
