@@ -247,10 +247,19 @@ class SpeakerDecoder(nn.Module):
 
     def quantize_w4(self, group=64, scale_dtype=torch.float32):
         """Run the word step's linears on 4-bit weights (ops.quantize_w4) from here on, made from the weights as they
-        are now; the parameters and the state_dict stay as they are. Call again after the weights changed (forward
-        refuses weights that changed since), or dequantize_w4() to go back."""
-        self._w4 = {name: (ops.quantize_w4(W, group, scale_dtype), W, W._version)
+        are now; the parameters and the state_dict stay as they are. Call again after the weights changed, or
+        dequantize_w4() to go back. forward refuses weights that were written in place, replaced or given other storage
+        since (p.data = ..., vector_to_parameters, .to() of another type or device). Writes through p.data (p.data.mul_(),
+        dp.broadcast_params) leave no trace that it could see, and the replay of a captured graph does not look again:
+        quantise after those."""
+        # the detached alias keeps the quantised values' memory, so that no other values can come to its address
+        self._w4 = {name: (ops.quantize_w4(W, group, scale_dtype), W, self._place(W), W.detach())
                     for name, W in self._word_linears().items()}
+
+    @staticmethod
+    def _place(W):
+        """Changes with every visible write to W and with its storage."""
+        return W._version, W.data_ptr(), W.stride(), W.device
 
     def dequantize_w4(self):
         self._w4 = {}
@@ -258,8 +267,8 @@ class SpeakerDecoder(nn.Module):
     def _linear(self, name, W, x, b=None, act=None, out=None, beta=0.0):
         if not self._w4:
             return ops.linear(x, W, b, act=act, out=out, beta=beta)
-        q, made_from, version = self._w4[name]
-        if W is not made_from or W._version != version or q.device != W.device:
+        q, made_from, place, _ = self._w4[name]
+        if W is not made_from or self._place(W) != place:
             raise DasaError(f"SpeakerDecoder: the weight {name!r} changed since quantize_w4(); call it again")
         return ops.linear_w4(x, q, b, act=act, out=out, beta=beta)
 

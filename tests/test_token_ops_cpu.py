@@ -137,3 +137,47 @@ def test_capture_beside_a_live_eager_graph_is_refused(monkeypatch):
     assert key in DF._USES
     del other
     assert key not in DF._USES and keep is not None
+
+
+class _Codes:
+    """Stands for a 4-bit weight where none can be made (no device)."""
+    device = torch.device("cpu")
+
+
+@pytest.mark.parametrize("change", ["in place", "data", "vector", "type and back", "transposed", "address reused",
+                                    "object"])
+def test_speaker_decoder_refuses_4bit_forms_of_other_weights(monkeypatch, change):
+    """quantize_w4() followed by anything that gives a weight other values: forward may not go on with the old codes."""
+    from dasa_amd.r2r import model
+    monkeypatch.setattr(ops, "quantize_w4", lambda W, group, scale_dtype: _Codes())
+    monkeypatch.setattr(ops, "linear_w4", lambda x, q, b, act=None, out=None, beta=0.0: "ran")
+    dec = model.SpeakerDecoder(12, 4, 0, 4, 0.0)
+    dec.quantize_w4()
+    lin = dec.attention_layer.linear_in                     # square: a transposed view keeps its shape
+    run = lambda: dec._linear("att_in", lin.weight, None)   # noqa: E731
+    with torch.no_grad():
+        assert run() == "ran" and run() == "ran"
+        if change == "in place":
+            lin.weight.mul_(2.0)
+        elif change == "data":
+            lin.weight.data = lin.weight.data * 2.0
+        elif change == "vector":
+            v = torch.nn.utils.parameters_to_vector(dec.parameters()) * 2.0
+            torch.nn.utils.vector_to_parameters(v, dec.parameters())
+        elif change == "type and back":
+            dec.half().float()
+        elif change == "transposed":
+            lin.weight.data = lin.weight.data.t()
+        elif change == "address reused":                    # the old values' memory may not come back as new values'
+            at = lin.weight.data_ptr()
+            for _ in range(50):
+                lin.weight.data = torch.empty(0)
+                lin.weight.data = torch.randn(4, 4)
+                assert lin.weight.data_ptr() != at
+        else:
+            lin.weight = torch.nn.Parameter(lin.weight.detach().clone())
+        _refused("changed since", run)
+        dec.quantize_w4()
+        assert run() == "ran"
+        dec.dequantize_w4()
+        assert not dec._w4
