@@ -279,13 +279,15 @@ class SpeakerDecoder(nn.Module):
         return self._linear("att_out", att.linear_out.weight, torch.cat((wctx, h), 1), act="tanh")
 
     def forward(self, words, ctx, ctx_mask, h0, c0):
-        """words [B, L] int64, ctx [B, T, H], ctx_mask [B, T] bool, h0 / c0 [1, B, H] ->
-        (logit [B, L, V], h1 [1, B, H], c1 [1, B, H])."""
+        """words [B, L] int64 (or any type of whole numbers), ctx [B, T, H], ctx_mask [B, T] bool, h0 / c0 [1, B, H]
+        -> (logit [B, L, V], h1 [1, B, H], c1 [1, B, H])."""
         if torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters()):
             raise NotImplementedError("SpeakerDecoder runs the inference path only (call it under torch.no_grad())")
         B, L = words.shape
         H = self.hidden_size
         training = self.training
+        if words.dtype not in (torch.int64, torch.int32):
+            words = words.to(torch.int64)
         emb = DF.dropout(ops.embedding(words, self.embedding.weight), self.drop.p, training)
         lw = self.lstm
         h, c = h0.reshape(B, H).contiguous(), c0.reshape(B, H).contiguous()

@@ -181,3 +181,21 @@ def test_speaker_decoder_refuses_4bit_forms_of_other_weights(monkeypatch, change
         assert run() == "ran"
         dec.dequantize_w4()
         assert not dec._w4
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.uint8, torch.float32])
+def test_speaker_decoder_takes_words_of_any_number_type(monkeypatch, dtype):
+    """forward converts the words for the lookup, which takes int64 and int32."""
+    from dasa_amd.r2r import model
+    seen = []
+
+    def lookup(ids, table):
+        seen.append(ids)
+        raise KeyboardInterrupt                             # the rest of the step needs a device
+    monkeypatch.setattr(ops, "embedding", lookup)
+    dec = model.SpeakerDecoder(12, 4, 0, 4, 0.0)
+    words = torch.tensor([[3], [11], [0]]).to(dtype)
+    with torch.no_grad(), pytest.raises(KeyboardInterrupt):
+        dec(words, None, None, torch.zeros(1, 3, 4), torch.zeros(1, 3, 4))
+    ids, = seen
+    assert ids.dtype in (torch.int64, torch.int32) and torch.equal(ids.long(), words.long())
