@@ -924,6 +924,7 @@ class EmbeddingFn(torch.autograd.Function):
         return ops.embedding(ids, table, scale=scale)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         return None, ops.embedding_bwd(dy, ids, ctx.vocab, scale=ctx.scale, padding_idx=ctx.pad), None, None
@@ -952,6 +953,7 @@ class BertEmbedFn(torch.autograd.Function):
         return ops.bert_embed(ids, word, pos, types[0], gamma, beta, eps, p, seed)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         word, pos, types, gamma, beta = ctx.params

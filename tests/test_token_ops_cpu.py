@@ -199,3 +199,35 @@ def test_speaker_decoder_takes_words_of_any_number_type(monkeypatch, dtype):
         dec(words, None, None, torch.zeros(1, 3, 4), torch.zeros(1, 3, 4))
     ids, = seen
     assert ids.dtype in (torch.int64, torch.int32) and torch.equal(ids.long(), words.long())
+
+
+def _double(f, *leaves):
+    """A second derivative through f's first gradients, with the upstream gradient itself depending on a leaf."""
+    a = torch.ones((), requires_grad=True)
+    y = f()
+    g = torch.autograd.grad((y * a).sum() + a * a, (*leaves, a), create_graph=True)
+    sum(t.sum() for t in g).backward()
+
+
+@pytest.mark.parametrize("which", ["embedding", "bert_embed"])
+def test_second_derivatives_are_refused(monkeypatch, which):
+    """The lookups' backward passes are kernels: differentiating through them raises instead of dropping the part that
+    goes through them. First gradients under create_graph=True are unharmed."""
+    monkeypatch.setattr(DF, "_leaf_use", lambda leaves: None)
+    monkeypatch.setattr(ops, "embedding", lambda ids, table, scale=1.0: table.detach()[ids] * scale)
+    monkeypatch.setattr(ops, "embedding_bwd", lambda d, ids, V, scale=1.0, padding_idx=None:
+                        torch.zeros(V, d.shape[-1]).index_add_(0, ids.reshape(-1), d.detach().reshape(-1, d.shape[-1])) * scale)
+    monkeypatch.setattr(ops, "bert_embed", lambda ids, w, p, t, ga, be, eps, pr, seed: w.detach()[ids])
+    monkeypatch.setattr(ops, "add2d", lambda a, b: a + b)
+    monkeypatch.setattr(ops, "layernorm", lambda x, g, b, eps, save: (x, x))
+    monkeypatch.setattr(ops, "layernorm_bwd", lambda dy, saved, g, dg, db: dy.detach())
+    ids, table = torch.tensor([[1, 3, 1]]), torch.randn(5, 4, requires_grad=True)
+    if which == "embedding":
+        f, leaves = (lambda: DF.embedding(ids, table)), (table,)
+    else:
+        more = [torch.randn(*s, requires_grad=True) for s in ((3, 4), (2, 4), (4,), (4,))]
+        f, leaves = (lambda: DF.bert_embed(ids, table, *more, 1e-12)), (table, *more)
+    first = torch.autograd.grad(f().sum(), leaves, create_graph=True)
+    assert torch.equal(first[0], torch.tensor([0.0, 2, 0, 1, 0])[:, None].expand(5, 4))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        _double(f, *leaves)
