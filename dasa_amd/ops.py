@@ -1136,10 +1136,14 @@ def _share_memory(a, lda, b):
 def embedding(ids, table, scale=1.0, out=None):
     """table[ids] * scale (dasa_embedding_fwd). ids int64 / int32 of any shape; table [V, E] fp32 or bf16, rows may
     be strided; returns [*ids.shape, E] of the table's type, each value rounded once. A negative id gives a zero
-    row; an id >= V gives a NaN row and is reported by check_device_errors()."""
+    row; an id >= V gives a NaN row and is reported by check_device_errors(). Forward only: functional.embedding
+    trains the table."""
     if table.dim() != 2:
         raise _lib.DasaError(f"embedding: table must be [V, E], got {tuple(table.shape)}")
     bf16, nb = _float_type(table, "embedding.table"), _ids_bytes(ids, "embedding.ids")
+    if table.requires_grad and torch.is_grad_enabled():
+        raise _lib.DasaError("embedding is forward only here: functional.embedding has the table's gradient, or call it "
+                             "under torch.no_grad()")
     dev = _pair_device("embedding", ids, table, out)
     V, E = table.shape
     if table.is_contiguous():

@@ -231,3 +231,12 @@ def test_second_derivatives_are_refused(monkeypatch, which):
     assert torch.equal(first[0], torch.tensor([0.0, 2, 0, 1, 0])[:, None].expand(5, 4))
     with pytest.raises(RuntimeError, match="once_differentiable"):
         _double(f, *leaves)
+
+
+def test_lookup_of_a_trained_table_without_a_gradient_is_refused():
+    """ops.embedding makes no graph: in grad mode a table that wants a gradient goes through functional.embedding."""
+    ids, table = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4, requires_grad=True)
+    _refused("forward only", ops.embedding, ids, table)
+    with torch.no_grad():
+        _refused("device tensors", ops.embedding, ids, table)          # as far as host tensors come
+    _refused("device tensors", ops.embedding, ids, table.detach())
