@@ -1328,6 +1328,12 @@ def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     return out
 
 
+def _forward_only(t, what):
+    """A call without a graph refuses a tensor that wants a gradient of it."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _lib.DasaError(f"{what} is forward only: call it under torch.no_grad()")
+
+
 def _penalty(v, B, dev, what, neutral):
     """(device pointer or None, number) of a penalty given as None, a number or a float32 [B] tensor."""
     if v is None:
@@ -1337,6 +1343,7 @@ def _penalty(v, B, dev, what, neutral):
             raise _lib.DasaError(f"logit_rules: {what} must be a number or a contiguous float32 [{B}]")
         if v.get_device() != dev:
             _on_device("logit_rules", v)
+        _forward_only(v, "logit_rules")
         return v.data_ptr(), neutral
     v = float(v)
     if not math.isfinite(v) or (what == "repetition" and v <= 0.0):
@@ -1362,8 +1369,7 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     dev = _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
     if V == 0 or B > 65535:
         raise _lib.DasaError(f"logit_rules: logits {tuple(logits.shape)}: 1 token at least, 65535 rows at most")
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise _lib.DasaError("logit_rules is forward only: call it under torch.no_grad()")
+    _forward_only(logits, "logit_rules")
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         raise _lib.DasaError("logit_rules: the rows of logits must be contiguous")
     hist = ldh = hlen = nid = 0
@@ -1390,6 +1396,7 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     if bias is not None:
         if bias.dtype != torch.float32 or (bias.shape != (V,) and bias.shape != (B, V)):
             raise _lib.DasaError(f"logit_rules: bias must be float32 [{V}] or [{B}, {V}]")
+        _forward_only(bias, "logit_rules")
         bias = bias.contiguous()
         ldb = V if bias.dim() == 2 else 0
     bits = byts = None

@@ -240,3 +240,13 @@ def test_lookup_of_a_trained_table_without_a_gradient_is_refused():
     with torch.no_grad():
         _refused("device tensors", ops.embedding, ids, table)          # as far as host tensors come
     _refused("device tensors", ops.embedding, ids, table.detach())
+
+
+def test_logit_rules_of_arguments_that_want_a_gradient_are_refused(monkeypatch):
+    """Not the logits alone: a bias or a penalty in grad mode would lose its gradient as well."""
+    monkeypatch.setattr(ops, "_on_device", lambda what, *ts: 0)
+    x, leaf = torch.zeros(2, 8), lambda *s: torch.ones(*s, requires_grad=True)   # noqa: E731
+    for kw in (dict(bias=leaf(8)), dict(bias=leaf(2, 8)), dict(repetition=leaf(2)), dict(presence=leaf(2)),
+               dict(frequency=leaf(2))):
+        _refused("forward only", ops.logit_rules, x, **kw)
+    _refused("forward only", ops.logit_rules, x.clone().requires_grad_())
