@@ -1179,6 +1179,7 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     padding_idx and of ids that do not occur are zero; ids outside the vocabulary are skipped. With out and
     accumulate=True the sums are added into out (rows without tokens are not touched)."""
     bf16, nb = _float_type(dout, "embedding_bwd.dout"), _ids_bytes(ids, "embedding_bwd.ids")
+    _forward_only(dout, "embedding_bwd")
     dev = _pair_device("embedding_bwd", dout, ids, out)
     vocab = int(vocab)
     if dout.dim() != ids.dim() + 1 or dout.shape[:-1] != ids.shape:

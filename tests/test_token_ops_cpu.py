@@ -250,3 +250,10 @@ def test_logit_rules_of_arguments_that_want_a_gradient_are_refused(monkeypatch):
                dict(frequency=leaf(2))):
         _refused("forward only", ops.logit_rules, x, **kw)
     _refused("forward only", ops.logit_rules, x.clone().requires_grad_())
+
+
+def test_embedding_bwd_of_a_gradient_that_wants_one_is_refused():
+    d, ids = torch.zeros(3, 4, requires_grad=True), torch.zeros(3, dtype=torch.int64)
+    _refused("forward only", ops.embedding_bwd, d, ids, 5)
+    with torch.no_grad():
+        _refused("device tensors", ops.embedding_bwd, d, ids, 5)
