@@ -1347,9 +1347,10 @@ def _penalty(v, B, dev, what, neutral):
         _forward_only(v, "logit_rules")
         return v.data_ptr(), neutral
     v = float(v)
-    if not math.isfinite(v) or (what == "repetition" and v <= 0.0):
+    x = ctypes.c_float(v).value                # as the kernel will have it
+    if not math.isfinite(x) or (what == "repetition" and x <= 0.0):
         raise _lib.DasaError(f"logit_rules: {what} = {v}")
-    return None, v
+    return None, x
 
 
 def logit_rules(logits, history=None, lengths=None, repetition=None, presence=None, frequency=None, bias=None,

@@ -257,3 +257,12 @@ def test_embedding_bwd_of_a_gradient_that_wants_one_is_refused():
     _refused("forward only", ops.embedding_bwd, d, ids, 5)
     with torch.no_grad():
         _refused("device tensors", ops.embedding_bwd, d, ids, 5)
+
+
+def test_logit_rules_numbers_outside_fp32_are_refused(monkeypatch):
+    """The kernel takes the 32-bit number nearest to a penalty: one that becomes 0 or infinite there is none."""
+    monkeypatch.setattr(ops, "_on_device", lambda what, *ts: 0)
+    x = torch.zeros(2, 8)
+    for kw in (dict(repetition=1e-50), dict(repetition=1e39), dict(presence=1e39), dict(frequency=-1e39),
+               dict(repetition=0.0), dict(repetition=-1.0), dict(presence=float("nan"))):
+        _refused(f"{next(iter(kw))} =", ops.logit_rules, x, **kw)
