@@ -16,6 +16,10 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
     if (_e != hipSuccess) return (int)_e;                     \
   } while (0)
 
+// A launch takes fewer than 2^32 threads in a dimension of its grid.
+constexpr long kMostThreads = (1L << 32) - 1;
+inline bool threads_fit(long blocks, int threads) { return blocks <= kMostThreads / threads; }
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

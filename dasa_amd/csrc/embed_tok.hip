@@ -30,6 +30,7 @@
 namespace {
 
 constexpr int kMostSize = 1 << 30;    // of a table: index arithmetic adds tiles to it in 32 bits
+constexpr int kMostSlices = 65535;    // of a row, in the grid's second dimension
 constexpr unsigned kErrTokenId = 8;   // bit of the error word (ops._ERR_BITS)
 
 // 16 bytes of a row. Rows of odd width or stride start anywhere, so the vector types are element-aligned (global loads
@@ -548,6 +549,7 @@ struct BwdArgs {
   int V, E;
   long bins;               // of the sort: start[bins] is the number of tokens
   unsigned chunk_blocks;   // blocks of the rows kernel that take chunks (first: they are the longer ones)
+  long row0;               // the first table row of the others
   float scale;
   int accumulate;
 };
@@ -605,7 +607,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void embedding_bwd_rows_kernel(BwdA
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
   if (blockIdx.x >= a.chunk_blocks) {
-    const long v = (long)(blockIdx.x - a.chunk_blocks) * kRowWaves + w;
+    const long v = a.row0 + (long)(blockIdx.x - a.chunk_blocks) * kRowWaves + w;
     if (v >= a.V) return;
     const int* at = a.start + a.own.place((unsigned)v);
     const int s = at[0], n = at[1] - s;
@@ -967,7 +969,7 @@ int launch_few_as(const BwdArgs& a, const SortArgs& g, hipStream_t st) {
   f.hot_blocks = g.T > kHot ? f.hot_slices << f.hot.lg : 0;
   f.seg = few_segment(g.T);
   const long blocks = f.hot_blocks + ((long)slices << f.cold.lg);
-  if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
+  if (!threads_fit(blocks, 64 * kFewWaves)) return (int)hipErrorInvalidValue;
   const size_t lists = (size_t)kFewWaves * f.seg * 4, sums = (size_t)kFewWaves * 64 * Vec<T>::N * 4;
   const size_t lds = (size_t)kFewWaves * f.seg * 2 + (lists > sums ? lists : sums);
   const dim3 grid((unsigned)blocks), block(64 * kFewWaves);
@@ -997,9 +999,16 @@ int launch_rows_as(BwdArgs a, long tokens, hipStream_t st) {
   const int slices = (a.E + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N);
   const long chunks = (tokens + kChunk - 1) / kChunk;
   a.chunk_blocks = (unsigned)((chunks + kRowWaves - 1) / kRowWaves);
-  const dim3 grid(a.chunk_blocks + (unsigned)((a.V + kRowWaves - 1) / kRowWaves), slices);
-  hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, NARROW>), grid, dim3(64 * kRowWaves), 0, st, a);
-  DASA_CHECK_LAUNCH();
+  const long blocks = ((long)a.V + kRowWaves - 1) / kRowWaves, most = kMostThreads / (64 * kRowWaves);
+  for (long b = 0; b < blocks;) {            // tables of more than 2^26 rows: several launches
+    const long n = std::min(blocks - b, most - a.chunk_blocks);
+    a.row0 = b * kRowWaves;
+    const dim3 grid(a.chunk_blocks + (unsigned)n, slices);
+    hipLaunchKernelGGL((embedding_bwd_rows_kernel<T, NARROW>), grid, dim3(64 * kRowWaves), 0, st, a);
+    DASA_CHECK_LAUNCH();
+    a.chunk_blocks = 0;
+    b += n;
+  }
   hipLaunchKernelGGL((embedding_bwd_join_kernel<T, NARROW>), dim3((unsigned)((chunks + kJoinWaves - 1) / kJoinWaves), slices),
                      dim3(64 * kJoinWaves), 0, st, a);
   DASA_CHECK_LAUNCH();
@@ -1043,6 +1052,7 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
   if (!dtable || ldt < E || ws_bytes < dasa_embedding_bwd_workspace(T, V, E) || (T > kFewTokens && !ws))
     return (int)hipErrorInvalidValue;
   if (T > 0 && (!ids || !dout || ldd < E)) return (int)hipErrorInvalidValue;
+  if (T > kFewTokens && E > kMostSlices * 64 * Vec<float>::N) return (int)hipErrorInvalidValue;
   hipStream_t st = (hipStream_t)stream;
   BwdArgs ba{};
   ba.dout = dout; ba.ldd = (long)ldd; ba.ids = ids; ba.ids64 = ids_bytes == 8;

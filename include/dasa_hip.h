@@ -366,7 +366,8 @@ int dasa_gather_rows(const float* ta, const int32_t* ia, int32_t Fa, const float
  * out[i] = scale * table[ids[i]] for T contiguous ids (ids_bytes 4 or 8: int32 / int64), rows of E elements, fp32
  * (bf16 = 0) or bf16 (bf16 = 1; the product is rounded once, RNE). A negative id gives a zero row; an id >= V gives
  * a NaN row and ORs 8 into *err (may be NULL); no memory outside the table is read. ldt / ldo are row strides. V and E
- * at most 2^30, here and in the gradient. */
+ * at most 2^30, here and in the gradient (where a table of more than 2^36 elements may be refused, and E above 16776960
+ * with more than 8192 tokens is). */
 int dasa_embedding_fwd(const void* table, int64_t ldt, const void* ids, int32_t ids_bytes, int64_t T, int32_t V,
                        int32_t E, float scale, int32_t bf16, void* out, int64_t ldo, uint32_t* err, void* stream);
 /* Its gradient: dtable[v] (+= if accumulate) scale * sum over i with ids[i] == v of dout[i], summed in fp32 in an

@@ -266,3 +266,14 @@ def test_logit_rules_numbers_outside_fp32_are_refused(monkeypatch):
     for kw in (dict(repetition=1e-50), dict(repetition=1e39), dict(presence=1e39), dict(frequency=-1e39),
                dict(repetition=0.0), dict(repetition=-1.0), dict(presence=float("nan"))):
         _refused(f"{next(iter(kw))} =", ops.logit_rules, x, **kw)
+
+
+def test_gradients_that_no_launch_can_hold_are_refused_at_the_check():
+    """A launch takes fewer than 2^32 threads in a dimension and 65535 workgroups in the second: such sizes are refused
+    before the first kernel. Addresses are made up."""
+    L, P = _lib.lib(), 0x100000
+    for V, E, bf in ((2**30, 600, 1), (2**30, 260, 0), (2**29 + 1, 1030, 1), (2**28 + 1, 2**20, 0)):
+        assert L.dasa_embedding_bwd(P, E, P, 8, 4, V, E, 1.0, -1, bf, P, E, 0, None, 0, None) == INVALID, (V, E)
+    T, E = 9000, 16776961
+    need = L.dasa_embedding_bwd_workspace(T, 50, E)
+    assert L.dasa_embedding_bwd(P, E, P, 8, T, 50, E, 1.0, -1, 0, P, E, 0, P, need, None) == INVALID

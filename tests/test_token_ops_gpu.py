@@ -622,3 +622,27 @@ def test_refusals_on_the_device(dev):
         ops.embedding(h, torch.empty(0, 8, device=dev))
     with pytest.raises(DasaError, match="rows must be contiguous"):
         ops.embedding(h, torch.randn(8, 10, device=dev).t())
+
+
+@pytest.mark.parametrize("dtype,E", [(BF16, 1), (BF16, 8), (F32, 5)])
+def test_embedding_gradient_of_more_rows_than_one_launch_takes(dev, dtype, E):
+    """2^26 rows and some, four of them to a workgroup of 256 threads: more threads than a launch may have. Whole numbers
+    of at most three bits: every sum is exact in fp32, so the gradient is the 64-bit sum, rounded once."""
+    V, T = 2**26 + 3, 8200
+    g = _gen(E)
+    ids = torch.randint(0, V, (T,), generator=g)
+    edge = 2**26 - 264 + torch.arange(-40, 40)                   # where the second launch begins
+    ids[:80], ids[80:90], ids[90:400] = edge, V - 1 - torch.arange(10), V - 1
+    ids[400:500], ids[500] = edge[39], 0
+    dout = torch.randint(-3, 4, (T, E), generator=g).to(dtype)
+    got = ops.embedding_bwd(dout.to(dev), ids.to(dev), V, scale=2.0)
+    rows, at = torch.unique(ids, return_inverse=True)
+    want = torch.zeros(len(rows), E, dtype=torch.float64).index_add_(0, at, dout.double()) * 2.0
+    assert torch.equal(got[rows.to(dev)].cpu(), want.to(dtype))
+    got[rows.to(dev)] = 0
+    assert int(torch.count_nonzero(got)) == 0
+    again = torch.full((V, E), 3.0, dtype=dtype, device=dev)
+    ops.embedding_bwd(dout.to(dev), ids.to(dev), V, out=again, accumulate=True)
+    assert torch.equal(again[rows.to(dev)].cpu(), (want / 2.0 + 3.0).to(dtype))
+    again[rows.to(dev)] = 3.0
+    assert bool((again == 3.0).all())
