@@ -131,8 +131,12 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(QuantArgs a) {
   }
 }
 
-// N and K of a weight: index arithmetic adds blocks to them in 32 bits
-inline bool sizes_ok(int N, int K) { return N > 0 && K > 0 && N <= 1 << 30 && K <= 1 << 30; }
+// N and K of a weight: index arithmetic adds blocks to them in 32 bits, and the layout has a workgroup of 256 threads for
+// 16 x 512 values, of which a launch takes fewer than 2^32 (the products and the quantisation start fewer)
+inline bool sizes_ok(int N, int K) {
+  return N > 0 && K > 0 && N <= 1 << 30 && K <= 1 << 30 &&
+         threads_fit((long)((N + 15) / 16) * ((K + 511) / 512), 256);
+}
 inline bool group_ok(int g) { return g == 32 || g == 64 || g == 128; }
 
 }  // namespace
@@ -155,7 +159,6 @@ extern "C" int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int3
     return (int)hipErrorInvalidValue;
   QuantArgs a{W, (long)ldw, codes, (long)ldc, scales, (long)lds, N, K, group};
   const long total = (long)N * ((K + group - 1) / group);
-  if ((total + 255) / 256 > 0x7fffffffL) return (int)hipErrorInvalidValue;
   const dim3 grid((unsigned)((total + 255) / 256)), block(256);
   hipStream_t st = (hipStream_t)stream;
   if (w_bf16 && scale_bf16) hipLaunchKernelGGL((w4_quantize_kernel<__bf16, __bf16>), grid, block, 0, st, a);
@@ -174,7 +177,6 @@ extern "C" int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* sca
   LayoutArgs a{codes, (long)ldc, scales, (long)lds, reinterpret_cast<unsigned*>(weight), scale_tiles, N, K,
                (K + 127) / 128, (N + 15) / 16, group};
   const long blocks = (long)a.N16 * ((a.Kb + 3) / 4);
-  if (blocks > 0x7fffffffL) return (int)hipErrorInvalidValue;
   if (scale_bf16)
     hipLaunchKernelGGL(w4_layout_kernel<__bf16>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
   else

@@ -385,7 +385,8 @@ int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t i
  * dasa_w4_quantize: W [N][ldw] (fp32 / bf16) -> codes [N][ldc] (two a byte, the even k in the low half) and scales
  * [N][lds] (fp32 / bf16), s = max |w| / 7 rounded to its type, q = clamp(rne(w / s), -8, 7) + 8; W must be finite.
  * dasa_w4_layout: codes / scales -> the tiles that dasa_gemm_w4 reads: `weight` (dasa_w4_weight_bytes, 16-B
- * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. N and K at most 2^30. */
+ * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. N and K at most 2^30, and N (rounded
+ * up to 16) times ceil(K / 512) below 2^28: both size queries are 0 past that, and every call is refused. */
 int64_t dasa_w4_weight_bytes(int32_t N, int32_t K);
 int64_t dasa_w4_scale_count(int32_t N, int32_t K, int32_t group);
 int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int32_t K, int32_t group, uint8_t* codes,

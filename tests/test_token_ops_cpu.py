@@ -277,3 +277,16 @@ def test_gradients_that_no_launch_can_hold_are_refused_at_the_check():
     T, E = 9000, 16776961
     need = L.dasa_embedding_bwd_workspace(T, 50, E)
     assert L.dasa_embedding_bwd(P, E, P, 8, T, 50, E, 1.0, -1, 0, P, E, 0, P, need, None) == INVALID
+
+
+def test_4bit_weights_that_no_launch_can_lay_out_are_refused_at_the_check():
+    """The layout has 256 threads for 16 x 512 values, and a launch takes fewer than 2^32. Addresses are made up."""
+    L, P = _lib.lib(), 0x100000
+    for N, K in ((2**28, 64), (2**28 - 15, 512), (2**27, 513), (2**30, 1), (32768, 2**22), (2**20, 2**30)):
+        assert L.dasa_w4_weight_bytes(N, K) == 0 and L.dasa_w4_scale_count(N, K, 64) == 0, (N, K)
+        g = -(-K // 64)
+        assert L.dasa_w4_quantize(P, K, 0, N, K, 64, P, K, P, g, 0, None) == INVALID, (N, K)
+        assert L.dasa_w4_layout(P, K, P, g, 0, N, K, 64, P, P, None) == INVALID, (N, K)
+        assert L.dasa_gemm_w4(P, K, 0, P, P, 0, 64, None, 0, 0.0, P, N, 1, N, K, None, 0, None) == INVALID, (N, K)
+    for N, K in ((2**28 - 16, 512), (2**27 - 16, 1024), (16, 2**30), (32768, 2**22 - 512)):
+        assert L.dasa_w4_weight_bytes(N, K) == -(-N // 16) * -(-K // 128) * 1024
