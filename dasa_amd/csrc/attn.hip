@@ -940,8 +940,6 @@ __global__ __launch_bounds__(256) void attn_dot_rows_kernel(const float* __restr
   if (t == 0) scores[(long)b * N + n] = s;
 }
 
-inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
 inline int block_threads(int D) {
   const int D4 = D >> 2;
   int T = ((D4 + 63) / 64) * 64;

@@ -19,6 +19,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // A launch takes fewer than 2^32 threads in a dimension of its grid.
 constexpr long kMostThreads = (1L << 32) - 1;
 inline bool threads_fit(long blocks, int threads) { return blocks <= kMostThreads / threads; }
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

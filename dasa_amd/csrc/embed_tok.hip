@@ -1049,7 +1049,8 @@ extern "C" int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids
       (ids_bytes != 4 && ids_bytes != 8))
     return (int)hipErrorInvalidValue;
   if (V == 0 || E == 0) return 0;
-  if (!dtable || ldt < E || ws_bytes < dasa_embedding_bwd_workspace(T, V, E) || (T > kFewTokens && !ws))
+  if (!dtable || ldt < E || ws_bytes < dasa_embedding_bwd_workspace(T, V, E) ||
+      (T > kFewTokens && (!ws || !aligned16(ws))))
     return (int)hipErrorInvalidValue;
   if (T > 0 && (!ids || !dout || ldd < E)) return (int)hipErrorInvalidValue;
   if (T > kFewTokens && E > kMostSlices * 64 * Vec<float>::N) return (int)hipErrorInvalidValue;

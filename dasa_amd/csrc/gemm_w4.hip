@@ -171,8 +171,8 @@ extern "C" int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int3
 
 extern "C" int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16,
                               int32_t N, int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream) {
-  if (!sizes_ok(N, K) || !group_ok(group) || !codes || !scales || !weight || !scale_tiles || ldc < (K + 1) / 2 ||
-      lds < (K + group - 1) / group)
+  if (!sizes_ok(N, K) || !group_ok(group) || !codes || !scales || !weight || !scale_tiles || !aligned16(weight) ||
+      !aligned16(scale_tiles) || ldc < (K + 1) / 2 || lds < (K + group - 1) / group)
     return (int)hipErrorInvalidValue;
   LayoutArgs a{codes, (long)ldc, scales, (long)lds, reinterpret_cast<unsigned*>(weight), scale_tiles, N, K,
                (K + 127) / 128, (N + 15) / 16, group};
@@ -198,14 +198,15 @@ extern "C" int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void
   if (M < 0 || !sizes_ok(N, K) || !group_ok(group) || act < DASA_ACT_NONE || act > DASA_ACT_SIGMOID)
     return (int)hipErrorInvalidValue;
   if (M == 0) return 0;
-  if (!x || !weight || !scale_tiles || !y || ldx < K || ldy < N || ((uintptr_t)weight & 15) || M > 65535 * 16)
+  if (!x || !weight || !scale_tiles || !y || ldx < K || ldy < N || !aligned16(weight) || !aligned16(scale_tiles) ||
+      M > 65535 * 16)
     return (int)hipErrorInvalidValue;
   Plan p = plan_of(M, N, K, bf16);
   W4Args a{x, (long)ldx, reinterpret_cast<const uint4*>(weight), scale_tiles, bias, y, (long)ldy, beta, act, M, N, K,
            (K + 127) / 128, (N + 15) / 16, 0, nullptr};
   a.per = (a.Kb + p.splits - 1) / p.splits;
   if (p.splits > 1) {
-    if (!ws || ws_bytes < dasa_gemm_w4_workspace(M, N, K, bf16)) return (int)hipErrorInvalidValue;
+    if (!ws || !aligned16(ws) || ws_bytes < dasa_gemm_w4_workspace(M, N, K, bf16)) return (int)hipErrorInvalidValue;
     a.part = reinterpret_cast<float4*>(ws);
   }
   hipStream_t st = (hipStream_t)stream;

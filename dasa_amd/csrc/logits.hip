@@ -234,7 +234,7 @@ extern "C" int dasa_logit_rules(const dasa_logit_rules_desc* d, void* ws, int64_
     return (int)hipErrorInvalidValue;
   const Shape sh = shape_of(d->B, d->V);
   const int slices = sh.slices;
-  if (d->choice && slices > 1 && (!ws || ws_bytes < dasa_logit_rules_workspace(d->B, d->V)))
+  if (d->choice && slices > 1 && (!ws || !aligned16(ws) || ws_bytes < dasa_logit_rules_workspace(d->B, d->V)))
     return (int)hipErrorInvalidValue;
   RulesArgs a{};
   a.logits = d->logits; a.ld = d->ld; a.out = d->out; a.ldo = d->ldo;

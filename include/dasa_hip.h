@@ -384,8 +384,8 @@ int dasa_embedding_bwd(const void* dout, int64_t ldd, const void* ids, int32_t i
  * A weight is (q - 8) * s with q in 0..15 and one scale s for each run of `group` (32, 64 or 128) values of a row.
  * dasa_w4_quantize: W [N][ldw] (fp32 / bf16) -> codes [N][ldc] (two a byte, the even k in the low half) and scales
  * [N][lds] (fp32 / bf16), s = max |w| / 7 rounded to its type, q = clamp(rne(w / s), -8, 7) + 8; W must be finite.
- * dasa_w4_layout: codes / scales -> the tiles that dasa_gemm_w4 reads: `weight` (dasa_w4_weight_bytes, 16-B
- * aligned) and `scale_tiles` (dasa_w4_scale_count elements), once for a weight. N and K at most 2^30, and N (rounded
+ * dasa_w4_layout: codes / scales -> the tiles that dasa_gemm_w4 reads: `weight` (dasa_w4_weight_bytes) and
+ * `scale_tiles` (dasa_w4_scale_count elements), both 16-B aligned, once for a weight. N and K at most 2^30, and N (rounded
  * up to 16) times ceil(K / 512) below 2^28: both size queries are 0 past that, and every call is refused. */
 int64_t dasa_w4_weight_bytes(int32_t N, int32_t K);
 int64_t dasa_w4_scale_count(int32_t N, int32_t K, int32_t group);
@@ -410,7 +410,7 @@ int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, c
  * history [B][ldh] int32 / int64 (ids_bytes) or NULL; lengths [B] or NULL (all L); repetition / presence /
  * frequency [B] or NULL (then the numbers *0); bias [V] (ldb = 0) or [B][ldb] or NULL; allowed as bits (bit v % 32
  * of word v / 32; ldbits = 0 shared) or as bytes (0 = not allowed; ldbytes = 0 shared) or neither.
- * ws: dasa_logit_rules_workspace(B, V) bytes of scratch, needed if choice is asked for. B <= 65535, V and L
+ * ws: dasa_logit_rules_workspace(B, V) bytes of scratch, 16-B aligned, needed if choice is asked for. B <= 65535, V and L
  * at most 2^30. */
 typedef struct dasa_logit_rules_desc {
   const void* logits; int64_t ld;

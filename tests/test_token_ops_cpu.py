@@ -290,3 +290,24 @@ def test_4bit_weights_that_no_launch_can_lay_out_are_refused_at_the_check():
         assert L.dasa_gemm_w4(P, K, 0, P, P, 0, 64, None, 0, 0.0, P, N, 1, N, K, None, 0, None) == INVALID, (N, K)
     for N, K in ((2**28 - 16, 512), (2**27 - 16, 1024), (16, 2**30), (32768, 2**22 - 512)):
         assert L.dasa_w4_weight_bytes(N, K) == -(-N // 16) * -(-K // 128) * 1024
+
+
+def test_entry_points_refuse_buffers_that_are_not_aligned():
+    """The header asks for 16-B alignment of tiles, scale tiles and workspaces, which are read in 16-B vectors."""
+    L, P = _lib.lib(), 0x100000
+    for off in (2, 4, 8):
+        assert L.dasa_gemm_w4(P, 64, 0, P, P + off, 0, 32, None, 0, 0.0, P, 4, 2, 4, 64, None, 0, None) == INVALID
+        assert L.dasa_gemm_w4(P, 64, 0, P + off, P, 0, 32, None, 0, 0.0, P, 4, 2, 4, 64, None, 0, None) == INVALID
+        assert L.dasa_w4_layout(P, 32, P, 2, 0, 4, 64, 32, P + off, P, None) == INVALID
+        assert L.dasa_w4_layout(P, 32, P, 2, 0, 4, 64, 32, P, P + off, None) == INVALID
+        need = L.dasa_gemm_w4_workspace(1, 1000, 8192, 0)
+        assert need > 0
+        assert L.dasa_gemm_w4(P, 8192, 0, P, P, 0, 32, None, 0, 0.0, P, 1000, 1, 1000, 8192, P + off, need, None) == INVALID
+        need = L.dasa_embedding_bwd_workspace(9000, 50, 8)
+        assert L.dasa_embedding_bwd(P, 8, P, 8, 9000, 50, 8, 1.0, -1, 0, P, 8, 0, P + off, need, None) == INVALID
+        need = L.dasa_logit_rules_workspace(2, 9000)
+        assert need > 0
+        d = _lib.LogitRules()
+        for k, v in dict(B=2, V=9000, logits=P, ld=9000, out=P, ldo=9000, repetition0=1.0, choice=P).items():
+            setattr(d, k, v)
+        assert L.dasa_logit_rules(ctypes.byref(d), P + off, need, None) == INVALID
