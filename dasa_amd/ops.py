@@ -1213,6 +1213,9 @@ def embedding_bwd(dout, ids, vocab, scale=1.0, padding_idx=None, out=None, accum
     return out
 
 
+_W4_GROUPS = (32, 64, 128)
+
+
 class W4Weight:
     """A weight [N, K] in 4 bits with one scale for each `group` values of a row, laid out for linear_w4: the value
     is (code - 8) * scale, code in 0..15. Made once by quantize_w4 or pack_w4 and kept by the program (its tensors
@@ -1221,6 +1224,13 @@ class W4Weight:
     __slots__ = ("tiles", "scales", "shape", "group", "nbytes")
 
     def __init__(self, tiles, scales, shape, group):
+        N, K = shape
+        blocks = -(-N // 16) * -(-K // 128)
+        if N < 1 or K < 1 or group not in _W4_GROUPS or tiles.dtype != torch.int32 or tiles.numel() != blocks * 256 or \
+                scales.dtype not in _FLOAT_TYPES or scales.numel() != blocks * 16 * (128 // group) or \
+                not (tiles.is_contiguous() and scales.is_contiguous()) or tiles.device != scales.device:
+            raise _lib.DasaError(f"W4Weight: tiles {tiles.dtype} {tuple(tiles.shape)} and scales {scales.dtype} "
+                                 f"{tuple(scales.shape)} do not hold [{N}, {K}] in groups of {group}")
         self.tiles, self.scales, self.shape, self.group = tiles, scales, tuple(shape), group
         self.nbytes = tiles.numel() * 4 + scales.numel() * scales.element_size()
 
@@ -1238,9 +1248,6 @@ class W4Weight:
         q = q.permute(0, 3, 1, 4, 2, 5).reshape(n16 * 16, kb * 128)    # k = 128 block + 32 step + 8 quarter + nibble
         s = self.scales.view(n16, kb, 16, 128 // self.group).transpose(1, 2).reshape(n16 * 16, -1).float()
         return (q * s.repeat_interleave(self.group, 1))[:N, :K].contiguous()
-
-
-_W4_GROUPS = (32, 64, 128)
 
 
 def _w4_group(group, what):

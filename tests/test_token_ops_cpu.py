@@ -311,3 +311,16 @@ def test_entry_points_refuse_buffers_that_are_not_aligned():
         for k, v in dict(B=2, V=9000, logits=P, ld=9000, out=P, ldo=9000, repetition0=1.0, choice=P).items():
             setattr(d, k, v)
         assert L.dasa_logit_rules(ctypes.byref(d), P + off, need, None) == INVALID
+
+
+def test_4bit_weight_of_tensors_that_do_not_hold_it_is_refused():
+    """linear_w4 reads what the shape says: tiles or scales of another size, type or device never get that far."""
+    tiles, scales = torch.zeros(2 * 2 * 256, dtype=torch.int32), torch.zeros(2 * 2 * 2 * 16)
+    assert ops.W4Weight(tiles, scales, (17, 129), 64).nbytes == 4 * (tiles.numel() + scales.numel())
+    for t, s, shape, group in ((tiles[:-1], scales, (17, 129), 64), (tiles, scales[:-1], (17, 129), 64),
+                               (tiles, scales, (33, 129), 64), (tiles, scales, (17, 257), 64),
+                               (tiles, scales, (17, 129), 32), (tiles, scales, (17, 129), 48),
+                               (tiles.float(), scales, (17, 129), 64), (tiles, scales.half(), (17, 129), 64),
+                               (tiles[::2], scales, (1, 129), 64), (tiles, scales, (0, 129), 64),
+                               (tiles, scales.to("meta"), (17, 129), 64)):
+        _refused("W4Weight", ops.W4Weight, t, s, shape, group)
