@@ -1425,7 +1425,8 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
         ldo = V
     else:
         same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
-        ldo = _out_rows(out, (B, V), logits, "logit_rules", None if same else logits, bias)
+        ldo = _out_rows(out, (B, V), logits, "logit_rules", None if same else logits, bias,
+                        *(v for v in (repetition, presence, frequency) if isinstance(v, torch.Tensor)))
     choice = torch.empty(B, dtype=torch.int64, device=logits.device) if want_choice else None
     if B:
         L = _lib.lib()

@@ -324,3 +324,13 @@ def test_4bit_weight_of_tensors_that_do_not_hold_it_is_refused():
                                (tiles[::2], scales, (1, 129), 64), (tiles, scales, (0, 129), 64),
                                (tiles, scales.to("meta"), (17, 129), 64)):
         _refused("W4Weight", ops.W4Weight, t, s, shape, group)
+
+
+def test_logit_rules_out_over_a_penalty_is_refused(monkeypatch):
+    """Other workgroups may still read a row's penalties when the first has written its slice."""
+    monkeypatch.setattr(ops, "_on_device", lambda what, *ts: 0)
+    buf = torch.ones(40)
+    x, out = torch.zeros(2, 8), buf[10:26].view(2, 8)
+    for name in ("repetition", "presence", "frequency"):
+        for at in (9, 10, 17, 25):
+            _refused("overlaps", ops.logit_rules, x, out=out, **{name: buf[at:at + 2]})
