@@ -37,3 +37,46 @@ def test_embedding_gradient_is_exact(dev, T, V, E, kind):
         acc = old.to(dtype).to(dev)
         ops.embedding_bwd(d, d32, V, padding_idx=pad, out=acc, accumulate=True)
         tc.check_gradient(acc, dout, ids, V, pad=pad, old=old)
+
+
+# each form of the products: 16 rows a workgroup with one, two and four column blocks, on 8 and 16 waves, K split over
+# workgroups or not; 32 rows sharing their activations with one and two column blocks a wave, K split or not; 64 rows, K
+# split or not; rows, columns and K that end inside a tile
+PRODUCTS = [(1, 1, 1, 32), (15, 17, 33, 32), (1, 2048, 256, 64), (16, 992, 1100, 64), (48, 2100, 300, 128),
+            (20, 4096, 2240, 64), (7, 7000, 1100, 32), (1, 30522, 768, 32), (16, 12000, 300, 64), (64, 4096, 8192, 128),
+            (3, 100, 8000, 32), (1, 1000, 8192, 128), (16, 5000, 6200, 32), (8, 7000, 6200, 64), (20, 30522, 200, 64),
+            (33, 30522, 768, 128), (150, 8193, 255, 64), (64, 16384, 2048, 32), (17, 24000, 4100, 64),
+            (64, 7000, 8191, 32), (33, 8192, 8192, 128), (40, 65536, 2041, 128), (50, 65536, 2048, 64),
+            (64, 12000, 8192, 64), (64, 12000, 8190, 32), (64, 21000, 4096, 128), (50, 21000, 4095, 32)]
+
+
+@pytest.mark.parametrize("M,N,K,group", PRODUCTS)
+def test_linear_w4_is_exact(dev, M, N, K, group):
+    """Whole numbers through every form in both types, with either type of scale and a bias; fp32 rows whose second and
+    third plane count; single values of 24 bits at many k."""
+    g = tc.gen(M + N + K + group)
+    codes, scales = tc.w4_weight(N, K, group, "powers", g)
+    codes = codes.to(dev)
+    W = tc.w4_values(codes, scales.to(dev), K, group)
+    bias = torch.randint(-50, 50, (N,), generator=g).to(dev)
+    x = tc.whole_rows(M, K, g).to(dev)
+    want = x @ W.t()
+    for sdt in (F32, BF16):
+        w = ops.pack_w4(codes, scales.to(sdt).to(dev), K, group)
+        for dtype in (F32, BF16):
+            tc.check_rounded(ops.linear_w4(x.to(dtype), w), want)
+            tc.check_rounded(ops.linear_w4(x.to(dtype), w, bias.float()), want + bias)
+    scales = torch.full_like(scales, 0.25).to(dev)
+    W = tc.w4_values(codes, scales, K, group)
+    w = ops.pack_w4(codes, scales, K, group)
+    x = tc.three_plane_rows(M, K, g).to(dev)
+    tc.check_rounded(ops.linear_w4(x.float(), w), x @ W.t())
+    scales = tc.w4_weight(N, K, group, "any", g)[1].to(dev)
+    W = tc.w4_values(codes, scales, K, group)
+    w = ops.pack_w4(codes, scales, K, group)
+    for i in range(3):
+        x = tc.single_rows(torch.randint(0, K, (M,), generator=g), K, g).to(dev)
+        tc.check_single(ops.linear_w4(x.float(), w), x, W)
+    for dtype, planes in ((F32, 3), (BF16, 1)):
+        x = torch.randn(M, K, generator=g).to(dtype).to(dev)
+        tc.check_groups(ops.linear_w4(x, w), x.double(), W, group, planes)
