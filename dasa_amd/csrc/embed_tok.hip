@@ -14,11 +14,11 @@
 // once; the sort that gives the order comes on top, so the sort keeps to few launches and small lists:
 //   T <= 8192      one launch: each workgroup sorts its share of the ids into LDS and sums its rows.
 //                  (1600 x 768 fp32 into 30522 rows: 20.8 us; the table's 94 MB alone take a fill kernel 13.6.)
-//   T <  49152     token_sort_kernel, rows, join. A workgroup of the sort owns a share of the ids, reads every token
+//   more           token_sort_kernel, rows, join. A workgroup of the sort owns a share of the ids, reads every token
 //                  (T x 8 B, an L2-resident list), counts its own per wave segment and those of the shares before it
 //                  (its base), and writes its tokens' positions at their stable rank. No workgroup waits for another.
-//   above          token_count_kernel, token_place_kernel, rows, join: reading every id in every workgroup is what
-//                  bounds the one-launch sort there.
+//   T >= 49152     (more for large tables: split_sort) token_count_kernel, token_place_kernel, rows, join: reading every
+//                  id in every workgroup is what bounds the one-launch sort there.
 //                  (131072 x 1024 bf16, a third of them padding, into 50021 rows: 7.0 + 16.1 us sort, 72.5 rows
 //                  (174 MB read, 102 MB written: 3.8 TB/s; a large sum reads at 4.0), 7.9 join.)
 #include "common.h"
@@ -478,23 +478,34 @@ __global__ __launch_bounds__(64 * kSortWaves) void token_place_kernel(SortArgs a
   });
 }
 
-// One launch against two, 50021 ids, Zipf / uniform / one id: 49152 tokens x 64 bf16, the whole gradient, 33.1 / 28.7 /
-// 51.2 us against 30.6 / 30.5 / 30.6; 131072 tokens, the sort alone, 39 / 30 / 72 against 25.4 / 27.7 / 26.4. Above
-// 4 M tokens the counts of the segments would outgrow the tokens.
-constexpr long kManyTokens = 49152, kMostTokens = 4 << 20;
+// One launch against two (whole gradient of 8-wide bf16 rows, us; Zipf / uniform / one id). Two launches read every id
+// twice in each of their G owners, one launch once in at least 256, and places a frequent id's tokens by one workgroup:
+// two are taken from 1536 tokens an owner on, 49152 at least.
+//     50021 ids, G 32:  49152 tokens 32 / 32 / 35, one launch 34 / 30 / 55;  131072: 43 / 45 / 56, 60 / 49 / 116
+//    100000 ids, G 64:  49152 tokens 46 / 46 / 51, one launch 41 / 37 / 62;  131072: 61 / 63 / 80, 67 / 57 / 122
+//    200000 ids, G 128: 131072 tokens 99 / 100 / 112, one launch 81 / 71 / 136;  524288: 202 / 217 / 268, 333 / 174 / 432
+// Placing reads the counts of all segments in every segment, bins segments^2 in all: two launches up to 256 a token.
+//     50021 ids: 16.8 M tokens (200 a token) 4.9 / 5.3 / 7.2 ms, one launch 9.9 / 6.0 / 13.3
+//                33.6 M (399) 14.7 / 15.4 / 18.9, one launch 20.5 / 12.2 / 27.7
+//    200000 ids: 4.2 M (202) 1.8 / 1.9 / 2.2, one launch 2.4 / 1.5 / 3.2;  16.8 M (800) 15.2 / 15.6 / 17.2, 10.0 / 6.0 / 13.3
+constexpr long kOwnerTokens = 1536, kCountsToken = 256;
 
-inline bool split_sort(int64_t T) { return T >= kManyTokens && T <= kMostTokens; }
 inline int sort_segments(int64_t T) { return (int)std::max<int64_t>(8, (T + kSegmentTokens - 1) / kSegmentTokens); }
+inline bool split_sort(int64_t T, int V) {
+  const Owners o = owners(V, 32, kWideBins);
+  const int64_t s = sort_segments(T);
+  return T >= kOwnerTokens * std::max(32L, 1L << o.lg) && bins_of(o) * s * s <= kCountsToken * T;
+}
 
 inline int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
-inline Owners sort_owners(int64_t T, int V) { return split_sort(T) ? owners(V, 32, kWideBins) : owners(V, 256, kMaxBins); }
+inline Owners sort_owners(int64_t T, int V) { return split_sort(T, V) ? owners(V, 32, kWideBins) : owners(V, 256, kMaxBins); }
 
 template <class W>
 int launch_sort(SortArgs a, void* split, hipStream_t st) {
   const dim3 block(64 * kSortWaves);
   const unsigned G = 1u << a.own.lg;
-  if (split_sort(a.T)) {
+  if (split_sort(a.T, a.V)) {
     SplitArgs p;
     p.segments = sort_segments(a.T);
     p.counts = reinterpret_cast<int*>(split);
@@ -1038,7 +1049,7 @@ extern "C" int64_t dasa_embedding_bwd_workspace(int64_t T, int32_t V, int32_t E)
   if (T <= kFewTokens || T >= (1LL << 31) || V < 0 || E < 0 || V > kMostSize || E > kMostSize) return 0;
   const int64_t chunks = (T + kChunk - 1) / kChunk;
   const Owners own = sort_owners(T, V);
-  const int64_t split = split_sort(T) ? (bins_of(own) + (1 << own.lg)) * sort_segments(T) * 4 : 0;
+  const int64_t split = split_sort(T, V) ? (bins_of(own) + (1 << own.lg)) * sort_segments(T) * 4 : 0;
   return round16((bins_of(own) + 1) * 4) + round16(T * 4) + chunks * 2 * part_stride(E, 1) * 4 + split;
 }
 

@@ -334,3 +334,14 @@ def test_logit_rules_out_over_a_penalty_is_refused(monkeypatch):
     for name in ("repetition", "presence", "frequency"):
         for at in (9, 10, 17, 25):
             _refused("overlaps", ops.logit_rules, x, out=out, **{name: buf[at:at + 2]})
+
+
+def test_gradient_sort_has_no_step_at_4_million_tokens():
+    """The two-launch sort, whose counts are part of the workspace, ends where its counts outweigh the tokens, not at a
+    number of tokens: one more token never needs much less workspace, except there."""
+    need = lambda T, V: _lib.lib().dasa_embedding_bwd_workspace(T, V, 8)   # noqa: E731
+    for V in (2, 1000, 50021, 102400):
+        for T in (2**22, 2**23):
+            assert 0 <= need(T + 1, V) - need(T, V) < 4096, (T, V)
+    assert need(393216, 300000) - need(393215, 300000) > 8 * 300000 * 4      # begins at 1536 tokens an owner
+    assert need(2**22, 300000) < 2**22 * 8                                   # and has ended

@@ -15,7 +15,11 @@ GRADIENTS = [(20, 992, 256, "uniform"), (1600, 3000, 96, "zipf"), (4099, 1001, 2
              (8192, 2, 1030, "one"), (8193, 2, 8, "uniform"), (9000, 300000, 16, "zipf"), (20001, 999, 72, "one"),
              (33000, 40, 520, "zipf"), (49151, 60, 3, "runs"), (30011, 50, 260, "runs"), (49152, 2, 8, "uniform"),
              (60001, 3000, 16, "one"), (50001, 40, 72, "zipf"), (100003, 90, 24, "runs"), (131073, 300000, 8, "zipf"),
-             (131072, 1000, 1030, "runs"), (2**22, 1000, 3, "zipf"), (2**22 + 1, 1000, 3, "zipf"), (2**22, 7, 1, "one")]
+             (131072, 1000, 1030, "runs"), (2**22, 1000, 3, "zipf"), (2**22 + 1, 1000, 3, "zipf"), (2**22, 7, 1, "one"),
+             # the two-launch sort of larger tables, below and above where it begins, and where its counts end it
+             (98303, 100000, 5, "zipf"), (98304, 100000, 5, "zipf"), (393215, 300000, 3, "zipf"),
+             (393216, 300000, 3, "runs"), (3 * 2**20, 300000, 1, "zipf"), (2**22, 300000, 1, "zipf"),
+             (2**22, 102400, 1, "runs")]
 
 
 @pytest.mark.parametrize("T,V,E,kind", GRADIENTS)
