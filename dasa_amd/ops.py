@@ -1300,8 +1300,9 @@ def quantize_w4(W, group=64, scale_dtype=torch.float32):
 
 def linear_w4(x, w, b=None, act=None, out=None, beta=0.0):
     """y = act(x @ W^T + b) (+ beta * out) with a W4Weight (dasa_gemm_w4); forward only. x [..., K] fp32 or bf16
-    (row-strided ok), b [N] fp32, y of x's type. Accumulates in fp32 at fp32 accuracy. Made for the few rows of a
-    decoding step: the weights are read once for every 64 rows."""
+    (row-strided ok), b [N] fp32, y of x's type. Accumulates in fp32 at fp32 accuracy (|x| from 2^-110 to 2^121). Made
+    for the few rows of a decoding step: the weights are read and unpacked once for every 16 rows where they are few and
+    come from cache, for every 32 or 64 rows where they are many."""
     if not isinstance(w, W4Weight):
         raise _lib.DasaError("linear_w4: the weight must be a W4Weight (quantize_w4 / pack_w4)")
     N, K = w.shape
