@@ -394,7 +394,8 @@ int dasa_w4_quantize(const void* W, int64_t ldw, int32_t w_bf16, int32_t N, int3
 int dasa_w4_layout(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int32_t scale_bf16, int32_t N,
                    int32_t K, int32_t group, void* weight, void* scale_tiles, void* stream);
 /* y = act(x W^T + bias) + beta * y: x [M][ldx], y [M][ldy], both fp32 (bf16 = 0) or both bf16; fp32 accumulation at
- * fp32 accuracy, deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. M at most 1048560; made for few rows.
+ * fp32 accuracy for |x| from 2^-110 to 2^121 (below, the lower of an fp32 value's three bf16 pieces are flushed: 2^-7 of
+ * the value is left at 2^-126; above, a group's sum before its scale can overflow), deterministic; bias [N] fp32 or NULL, act as in enum dasa_act. M at most 1048560; made for few rows.
  * ws: dasa_gemm_w4_workspace(M, N, K, bf16) bytes of scratch, 16-B aligned (0: none). */
 int64_t dasa_gemm_w4_workspace(int32_t M, int32_t N, int32_t K, int32_t bf16);
 int dasa_gemm_w4(const void* x, int64_t ldx, int32_t bf16, const void* weight, const void* scale_tiles,

@@ -84,3 +84,21 @@ def test_linear_w4_is_exact(dev, M, N, K, group):
     for dtype, planes in ((F32, 3), (BF16, 1)):
         x = torch.randn(M, K, generator=g).to(dtype).to(dev)
         tc.check_groups(ops.linear_w4(x, w), x.double(), W, group, planes)
+
+
+@pytest.mark.parametrize("M,N,K", [(16, 64, 256), (64, 16384, 2048), (64, 12000, 8192)])
+def test_linear_w4_range(dev, M, N, K):
+    """The ends of the range at which fp32 rows keep fp32 accuracy: 24-bit values of 2^-110, and rows of 2^121, whose
+    groups sum up to 2^127 before a small scale."""
+    g = tc.gen(K)
+    codes = (tc.w4_weight(N, K, 128, "any", g)[0] | 0x11).to(dev)
+    scales = torch.ones(N, -(-K // 128), device=dev)
+    x = tc.single_rows(torch.randint(0, K, (M,), generator=g), K, g)
+    x = (torch.sign(x) * torch.ldexp(2 * torch.frexp(x)[0].abs(), torch.tensor(-110))).to(dev)
+    assert torch.equal(x.float().double(), x)
+    tc.check_single(ops.linear_w4(x.float(), ops.pack_w4(codes, scales, K, 128)), x, tc.w4_values(codes, scales, K, 128))
+    codes = torch.zeros_like(codes)                              # every weight is -8 times its scale
+    w = ops.pack_w4(codes, scales * 2.0**-30, K, 128)
+    x = torch.full((M, K), 2.0**121, device=dev)
+    assert bool((ops.linear_w4(x, w) == -K * 2.0**94).all())
+    assert bool((ops.linear_w4(-x.to(BF16), w) == torch.tensor(K * 2.0**94).to(BF16).to(dev)).all())
