@@ -36,8 +36,9 @@ FAMILIES = {
     "embed": ("hbm", "embed_kernel / embedding_fwd_kernel"),
     "ada_gate": ("hbm", "ada_gate_*_kernel"),
     "gather": ("hbm", "gather_rows_kernel"),
-    "embed_bwd": ("hbm", "token_sort_kernel + embedding_bwd_*_kernel"),
-    "gemm_w4": ("hbm", "w4_kernel"),
+    "embed_bwd": ("hbm", "embedding_bwd_few_kernel / token_sort_kernel (token_count_kernel + token_place_kernel) + "
+                         "embedding_bwd_rows_kernel + embedding_bwd_join_kernel"),
+    "gemm_w4": ("hbm", "w4_split_kernel / w4_shared_kernel (+ w4_join_kernel)"),
     "logit_rules": ("hbm", "logit_rules_kernel (+ logit_choice_kernel)"),
     "elementwise": ("hbm", "various"),
     "lstm_cell": ("hbm", "lstm_cell_*_kernel"),

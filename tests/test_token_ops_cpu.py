@@ -345,3 +345,18 @@ def test_gradient_sort_has_no_step_at_4_million_tokens():
             assert 0 <= need(T + 1, V) - need(T, V) < 4096, (T, V)
     assert need(393216, 300000) - need(393215, 300000) > 8 * 300000 * 4      # begins at 1536 tokens an owner
     assert need(2**22, 300000) < 2**22 * 8                                   # and has ended
+
+
+def test_profile_families_name_kernels_that_exist():
+    """The profile looks a family's kernel up by its first word."""
+    import glob
+    import os
+    import re
+
+    from dasa_amd import build, prof
+    text = "".join(open(f).read() for f in glob.glob(os.path.join(build.CSRC, "*")))
+    for family in ("embed", "embed_bwd", "gemm_w4", "logit_rules"):
+        names = re.findall(r"\w+_kernel", prof.FAMILIES[family][1])
+        assert names and prof.FAMILIES[family][1].split(" ")[0] == names[0], family
+        for n in names:
+            assert re.search(rf"void {n}\(", text), (family, n)
