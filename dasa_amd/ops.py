@@ -1343,6 +1343,9 @@ def _forward_only(t, what):
         raise _lib.DasaError(f"{what} is forward only: call it under torch.no_grad()")
 
 
+_F32_MOST, _F32_LEAST = torch.finfo(torch.float32).max, 2.0**-149
+
+
 def _penalty(v, B, dev, what, neutral):
     """(device pointer or None, number) of a penalty given as None, a number or a float32 [B] tensor."""
     if v is None:
@@ -1352,13 +1355,13 @@ def _penalty(v, B, dev, what, neutral):
             raise _lib.DasaError(f"logit_rules: {what} must be a number or a contiguous float32 [{B}]")
         if v.get_device() != dev:
             _on_device("logit_rules", v)
-        _forward_only(v, "logit_rules")
+        if v.requires_grad:
+            _forward_only(v, "logit_rules")
         return v.data_ptr(), neutral
     v = float(v)
-    x = ctypes.c_float(v).value                # as the kernel will have it
-    if not math.isfinite(x) or (what == "repetition" and x <= 0.0):
+    if not -_F32_MOST <= v <= _F32_MOST or (what == "repetition" and v < _F32_LEAST):     # the kernel takes it in fp32
         raise _lib.DasaError(f"logit_rules: {what} = {v}")
-    return None, x
+    return None, v
 
 
 def logit_rules(logits, history=None, lengths=None, repetition=None, presence=None, frequency=None, bias=None,
@@ -1379,7 +1382,8 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     dev = _on_device("logit_rules", logits, history, lengths, bias, allowed, out)
     if V == 0 or B > 65535:
         raise _lib.DasaError(f"logit_rules: logits {tuple(logits.shape)}: 1 token at least, 65535 rows at most")
-    _forward_only(logits, "logit_rules")
+    if logits.requires_grad:
+        _forward_only(logits, "logit_rules")
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
         raise _lib.DasaError("logit_rules: the rows of logits must be contiguous")
     hist = ldh = hlen = nid = 0
@@ -1406,7 +1410,8 @@ def logit_rules(logits, history=None, lengths=None, repetition=None, presence=No
     if bias is not None:
         if bias.dtype != torch.float32 or (bias.shape != (V,) and bias.shape != (B, V)):
             raise _lib.DasaError(f"logit_rules: bias must be float32 [{V}] or [{B}, {V}]")
-        _forward_only(bias, "logit_rules")
+        if bias.requires_grad:
+            _forward_only(bias, "logit_rules")
         bias = bias.contiguous()
         ldb = V if bias.dim() == 2 else 0
     bits = byts = None
