@@ -913,6 +913,13 @@ def _leaf_use(leaves):
     return use
 
 
+def _first_derivative(backward):
+    """once_differentiable for a backward of kernels, put on only where a graph of it is asked for: otherwise grad mode
+    is off as it is, and the two context managers would cost each call 2 us."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, dy: (guarded if torch.is_grad_enabled() else backward)(ctx, dy)
+
+
 class EmbeddingFn(torch.autograd.Function):
     """table[ids] * scale (nn.Embedding with a factor, model.py:1061); the table's gradient by sorted tokens."""
 
@@ -924,7 +931,7 @@ class EmbeddingFn(torch.autograd.Function):
         return ops.embedding(ids, table, scale=scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         return None, ops.embedding_bwd(dy, ids, ctx.vocab, scale=ctx.scale, padding_idx=ctx.pad), None, None
@@ -953,7 +960,7 @@ class BertEmbedFn(torch.autograd.Function):
         return ops.bert_embed(ids, word, pos, types[0], gamma, beta, eps, p, seed)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_derivative
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
         word, pos, types, gamma, beta = ctx.params
