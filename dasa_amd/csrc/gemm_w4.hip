@@ -108,6 +108,8 @@ struct QuantArgs {
 
 // One thread per (row, group): s = max |w| / 7, q = clamp(rne(w / s), -8, 7) + 8; an all-zero group has s = 0, q = 8.
 // The scale is rounded to its stored type first, so the codes are nearest to the values they will stand for.
+// Once for a weight, so left simple: the thread reads its group twice, a cache line a thread (32768 x 8192 fp32: 9.3 to
+// 10.2 ms = 110 GB/s, where a large sum reads at 4.0 TB/s).
 template <class T, class S>
 __global__ __launch_bounds__(256) void w4_quantize_kernel(QuantArgs a) {
   const int groups = (a.K + a.g - 1) / a.g;

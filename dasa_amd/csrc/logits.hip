@@ -13,9 +13,9 @@
 // writes the slice. With one slice a row, the workgroup also makes the choice; else each slice leaves its best key
 // and a second launch takes the best of them, one wave a row.
 //
-// Bound by latency at a decoding step's sizes: 20 x 992 fp32 with 120 ids a row 4.4 us, where an empty kernel takes 2.4.
-// 64 x 30522 fp32, 1024 ids: 8.9 + 2.6 us (17 MB: 3.2 at a copy's rate); 16 x 128255 bf16 with a bias a row, 16384 ids:
-// 13.9 + 3.2 (18 MB: 3.5), 2.4 of it the history that every slice reads.
+// Bound by latency at a decoding step's sizes: 20 x 992 fp32 with 120 ids a row 4.3 us, where an empty kernel takes 2.4.
+// 64 x 30522 fp32, 1024 ids: 8.9 + 2.5 us (17 MB: 3.2 at a copy's rate); 16 x 128255 bf16 with a bias a row, 16384 ids:
+// 13.8 + 3.0 (18 MB: 3.5), 2.4 of it the history that every slice reads.
 #include "common.h"
 #include "../../include/dasa_hip.h"
 

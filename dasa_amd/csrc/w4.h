@@ -21,9 +21,9 @@
 // x are split into planes and held in LDS once for all of them. K may be split over workgroups in both; a second
 // launch then joins the sums in order. Every order is fixed by the shape: results are bitwise reproducible.
 //
-// What bounds it, measured: one row on a wide layer is its weights' bytes (1 x 32768 x 8192 bf16, group 128: 27.0 us for
-// 138 MB = 5.1 TB/s, a large copy reaches 5.2); small layers are a launch (1 x 2048 x 256 fp32: 3.4 us, an empty kernel
-// 2.4); 64 bf16 rows of a short K are the unpacking and the stores (64 x 30522 x 768: 9.9 us, of them 2.5 the stores);
+// What bounds it, measured: one row on a wide layer is its weights' bytes (1 x 32768 x 8192 bf16, group 128: 27.1 us for
+// 138 MB = 5.1 TB/s, a large copy reaches 5.2); small layers are a launch (1 x 2048 x 256 fp32: 3.1 us, an empty kernel
+// 2.4); 64 bf16 rows of a short K are the unpacking and the stores (64 x 30522 x 768: 10.4 us, of them 2.5 the stores);
 // many fp32 rows are the three planes' matrix instructions (64 x 32768 x 8192: 108 us = 0.95 PFLOP/s of bf16 work).
 #pragma once
 #include "common.h"
